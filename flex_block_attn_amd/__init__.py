@@ -23,6 +23,7 @@ from .video import (
     tile_tokens,
     untile_tokens,
 )
+from .window import WindowAttnFunc, window_attn_func
 
 __all__ = [
     "flex_block_attn_func",
@@ -46,4 +47,6 @@ __all__ = [
     "ssta_3d_attention",
     "tile_tokens",
     "untile_tokens",
+    "window_attn_func",
+    "WindowAttnFunc",
 ]

@@ -8,6 +8,7 @@
 
 #include "../../include/fba.h"
 #include "fba_kernels.h"
+#include "fba_window.h"
 
 namespace {
 
@@ -875,6 +876,101 @@ int32_t fba_bwd_tiled(const void* q, const void* k, const void* v, const void* o
                       void* split_ws, int64_t split_ws_bytes, void* hip_stream) {
   return bwd_impl(q, k, v, o, d_o, lse, stats, dq, dk, dv, qt_cnt, qt_ent, kt_cnt, kt_ent, mask_bh, B, Hq, Hkv, Sq, Skv, head_dim,
                   q_block, k_block, split_ws, split_ws_bytes, hip_stream, true);
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------------------------
+// attention under a sliding window
+// ---------------------------------------------------------------------------------------------------------------------
+namespace {
+
+int check_window(int32_t has_lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks) {
+  if (B <= 0 || Hq <= 0 || Hkv <= 0 || Sq <= 0 || Skv <= 0)
+    return fail(FBA_ERR_INVALID, "B, Hq, Hkv, Sq, Skv must be positive (got %d %d %d %d %d)", B, Hq, Hkv, Sq, Skv);
+  if (Hq % Hkv != 0) return fail(FBA_ERR_INVALID, "Hq (%d) must be a multiple of Hkv (%d)", Hq, Hkv);
+  if (window < 1) return fail(FBA_ERR_INVALID, "window (%d) must be at least 1", window);
+  if (sinks < 0) return fail(FBA_ERR_INVALID, "sinks (%d) must not be negative", sinks);
+  if (has_lengths && Sq != Skv) return fail(FBA_ERR_INVALID, "lengths need Sq (%d) and Skv (%d) to be equal", Sq, Skv);
+  if (Sq > 1 << 28 || Skv > 1 << 28 || (int64_t)B * Hq * Sq >= 1LL << 29 || (int64_t)B * Hkv * Skv >= 1LL << 29)
+    return fail(FBA_ERR_UNSUPPORTED, "Sq and Skv may be 2^28 at most, B*Hq*Sq and B*Hkv*Skv below 2^29 (got %d %d %d %d %d)", B, Hq, Hkv, Sq, Skv);
+  return FBA_OK;
+}
+
+int take_strided(fba::Strided& to, const fba_strided* t, const char* name) {
+  if (t == nullptr || t->ptr == nullptr) return fail(FBA_ERR_INVALID, "%s is null", name);
+  if (!aligned16(t->ptr)) return fail(FBA_ERR_INVALID, "%s is not 16-byte aligned", name);
+  if ((t->batch | t->head | t->row) & 7) return fail(FBA_ERR_INVALID, "%s: strides must be multiples of 8 elements", name);
+  if (t->batch < 0 || t->head < 0 || t->row < 0 || t->batch > 1LL << 40 || t->head > 1LL << 40)
+    return fail(FBA_ERR_INVALID, "%s: strides must not be negative, nor beyond 2^40 elements", name);
+  if (t->row > 1LL << 24) return fail(FBA_ERR_UNSUPPORTED, "%s: rows may be 2^24 elements apart at most, got %lld", name, (long long)t->row);
+  to = {(char*)t->ptr, t->batch * 2, t->head * 2, (uint32_t)(t->row * 2)};
+  return FBA_OK;
+}
+
+int fill_window(fba::WindowParams& p, float* stats, const int32_t* lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim,
+                int32_t window, int32_t sinks, int32_t causal, int32_t type) {
+  if (head_dim != 128) return fail(FBA_ERR_INVALID, "head_dim must be 128, got %d", head_dim);
+  if (type != FBA_BF16 && type != FBA_FP16) return fail(FBA_ERR_INVALID, "type must be FBA_BF16 or FBA_FP16, got %d", type);
+  if (int rc = check_window(lengths != nullptr, B, Hq, Hkv, Sq, Skv, window, sinks)) return rc;
+  if (stats == nullptr) return fail(FBA_ERR_INVALID, "stats is null");
+  p.lse = stats;
+  p.neg_delta = stats + (int64_t)B * Hq * Sq;
+  p.lengths = lengths;
+  p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
+  p.window = window < (Sq > Skv ? Sq : Skv) ? window : (Sq > Skv ? Sq : Skv);  // no two positions are further apart
+  p.sinks = sinks < Skv ? sinks : Skv;
+  p.causal = causal != 0;
+  p.scale = 1.f / 11.313708498984761f;
+  p.scale_log2e = 1.4426950408889634f / 11.313708498984761f;
+  return FBA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, float* stats, const int32_t* lengths, int32_t B,
+                       int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
+                       void* hip_stream) {
+  fba::WindowParams p{};
+  if (int rc = fill_window(p, stats, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
+  if (int rc = take_strided(p.q, q, "q")) return rc;
+  if (int rc = take_strided(p.k, k, "k")) return rc;
+  if (int rc = take_strided(p.v, v, "v")) return rc;
+  if (int rc = take_strided(p.o, o, "o")) return rc;
+  hipError_t e = fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "window forward launch");
+}
+
+int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal) {
+  fba::WindowParams p{};
+  float stats;
+  const int32_t lengths = 0;
+  if (fill_window(p, &stats, has_lengths ? &lengths : nullptr, B, Hkv, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
+  return fba::plan_window_bwd(p);
+}
+
+int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* d_o, float* stats,
+                       const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
+                       int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
+                       void* hip_stream) {
+  fba::WindowParams p{};
+  if (int rc = fill_window(p, stats, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
+  if (int rc = take_strided(p.q, q, "q")) return rc;
+  if (int rc = take_strided(p.k, k, "k")) return rc;
+  if (int rc = take_strided(p.v, v, "v")) return rc;
+  if (int rc = take_strided(p.o, o, "o")) return rc;
+  if (int rc = take_strided(p.d_o, d_o, "d_o")) return rc;
+  if (int rc = take_strided(p.dq, dq, "dq")) return rc;
+  if (int rc = take_strided(p.dk, dk, "dk")) return rc;
+  if (int rc = take_strided(p.dv, dv, "dv")) return rc;
+  const int64_t need = fba::plan_window_bwd(p);
+  if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need))
+    return fail(FBA_ERR_INVALID, "ws must be 16-byte aligned and hold %lld bytes (fba_window_workspace_bytes), got %lld", (long long)need, (long long)ws_bytes);
+  p.parts = (float*)ws;
+  hipError_t e = fba::launch_window_bwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "window backward launch");
 }
 
 }  // extern "C"

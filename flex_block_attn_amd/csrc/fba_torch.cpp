@@ -42,7 +42,7 @@ constexpr int64_t kXcds = 8;
 #define FBA_FUNCTIONS(X)                                                                                                \
   X(fba_version) X(fba_last_error) X(fba_split_workspace_bytes) X(fba_lists_cut) X(fba_pair_slots_bounds) X(fba_tile_slots_bounds)        \
   X(fba_fwd) X(fba_fwd_tiled) X(fba_fwd_blocks) X(fba_fwd_blocks_use) X(fba_fwd_mask_copy) X(fba_fwd_takes_mask) X(fba_bwd_mask) X(fba_bwd_takes_mask) X(fba_bwd) X(fba_bwd_handover) X(fba_bwd_tiled_cut) X(fba_bwd_dense) \
-  X(fba_resize_rows) X(fba_resize_mask)
+  X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd)
 
 struct Library {
 #define DECLARE(f) decltype(&::f) f = nullptr;
@@ -667,6 +667,163 @@ std::vector<at::Tensor> backward_on_lists(const at::Tensor& q, const at::Tensor&
   return run_backward(p, q, k, v, o, lse, d_o, l, bounds, mode, dense, limit, split_bytes);
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// attention under a sliding window
+// ---------------------------------------------------------------------------------------------------------------------
+// What a call may be left to: `attention`'s reasons for the Python autograd functions.
+bool transformed(std::initializer_list<const at::Tensor*> tensors) {
+  if (torch::jit::tracer::isTracing()) return true;
+  if (c10::impl::tls_local_dispatch_key_set().included_.has(c10::DispatchKey::FuncTorchDynamicLayerFrontMode)) return true;
+  for (const at::Tensor* t : tensors)
+    if (t->_fw_grad(0).defined()) return true;
+  return false;
+}
+
+// Can the kernels read it by these strides?  Dense rows of 128, everything else at multiples of 16 bytes; strides of a dimension of one do not count.
+bool takes_strides(const at::Tensor& t) {
+  if (t.dim() != 4 || t.size(3) != kHeadDim || t.stride(3) != 1 || (reinterpret_cast<uintptr_t>(t.data_ptr()) & 15) != 0) return false;
+  for (int d = 0; d < 3; ++d)
+    if (t.size(d) > 1 && (t.stride(d) % 8 != 0 || t.stride(d) < 0 || t.stride(d) > (d == 2 ? 1LL << 24 : 1LL << 40))) return false;
+  return true;
+}
+fba_strided strided(const at::Tensor& t) {
+  auto stride = [&](int d) { return t.size(d) > 1 ? t.stride(d) : 0; };
+  return {t.data_ptr(), stride(0), stride(1), stride(2)};
+}
+
+struct Window : torch::CustomClassHolder {
+  int64_t window, sinks;
+  bool causal;
+  at::Tensor lengths;  // undefined: none
+  const int32_t* lengths_ptr() const { return lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr; }
+};
+int32_t type_of(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FBA_FP16 : FBA_BF16; }
+
+// -> o, and statistics with room for those of backward
+std::pair<at::Tensor, at::Tensor> run_window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Window& w) {
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor o = at::empty_like(q);
+  if (!takes_strides(o)) o = at::empty(q.sizes(), q.options());
+  at::Tensor stats = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {o, stats};
+  if (k.numel() == 0) {  // there is nothing to see
+    o.zero_();
+    return {o, stats};
+  }
+  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o);
+  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, stats.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
+                           w.sinks, w.causal, type_of(q), current_stream(q)));
+  return {o, stats};
+}
+
+std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
+                                            at::Tensor d_o, const Window& w) {
+  const c10::DeviceGuard guard(q.device());
+  std::vector<at::Tensor> grads;
+  for (const at::Tensor* t : {&q, &k, &v}) {
+    grads.push_back(at::empty_like(*t));
+    if (!takes_strides(grads.back())) grads.back() = at::empty(t->sizes(), t->options());
+  }
+  if (q.numel() == 0 || k.numel() == 0) {
+    for (at::Tensor& t : grads) t.zero_();
+    return grads;
+  }
+  d_o = d_o.to(q.scalar_type());
+  if (!takes_strides(d_o)) d_o = d_o.clone(at::MemoryFormat::Contiguous);
+  const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
+  SplitWorkspace ws(q, bytes);
+  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
+                    dv = strided(grads[2]);
+  check(lib.fba_window_bwd(&sq, &sk, &sv, &so, &sd, stats.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
+                           q.size(2), k.size(2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
+  return grads;
+}
+
+struct WindowAttention : torch::autograd::Function<WindowAttention> {
+  static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, c10::intrusive_ptr<Window> w) {
+    if (w->lengths.defined()) w->lengths = w->lengths.clone();  // the caller may write to theirs before backward comes
+    auto [o, stats] = run_window_forward(q, k, v, *w);
+    ctx->save_for_backward({q, k, v, o, stats});
+    ctx->saved_data["w"] = c10::IValue::make_capsule(std::move(w));
+    return o;
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto capsule = ctx->saved_data["w"].toCapsule();
+    const Window& w = *static_cast<Window*>(capsule.get());
+    // What a saved-tensor hook hands back is read by raw pointer.
+    for (int i = 0; i < 5; ++i) {
+      const at::Tensor& t = saved[i];
+      TORCH_CHECK_VALUE(t.defined() && t.device() == grads[0].device(), "saved tensors must come back on ", grads[0].device());
+      TORCH_CHECK_TYPE(t.scalar_type() == (i < 4 ? saved[0].scalar_type() : at::kFloat) && (i == 4 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
+                       "saved tensors must come back in their types");
+      TORCH_CHECK_VALUE(i == 4 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
+    }
+    TORCH_CHECK_VALUE(saved[0].sizes() == grads[0].sizes() && saved[3].sizes() == grads[0].sizes() && saved[1].sizes() == saved[2].sizes() &&
+                          saved[4].numel() == 2 * saved[0].size(0) * saved[0].size(1) * saved[0].size(2) && saved[1].size(0) == saved[0].size(0) &&
+                          saved[1].size(1) > 0 == saved[1].numel() > 0 && (saved[1].numel() == 0 || saved[0].size(1) % saved[1].size(1) == 0),
+                      "saved tensors must come back in their shapes");
+    const auto g = run_window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], grads[0], w);
+    return {g[0], g[1], g[2], at::Tensor()};
+  }
+};
+
+// A whole number of 32 bits, or `none` for None; false for anything else.
+bool int32_of(pybind11::handle object, int64_t none, int64_t* value) {
+  if (object.is_none()) {
+    *value = none;
+    return none >= 0;
+  }
+  int overflow = 0;
+  if (!PyLong_CheckExact(object.ptr())) return false;
+  *value = PyLong_AsLongLongAndOverflow(object.ptr(), &overflow);
+  return overflow == 0 && *value >= -0x80000000LL && *value <= 0x7fffffffLL;
+}
+
+constexpr int64_t kNoWindow = 0x7fffffff;
+
+// window_attn_func for arguments that need no preparation; nothing for all others, which Python then prepares or reports.
+c10::optional<at::Tensor> window_attention(pybind11::handle q_, pybind11::handle k_, pybind11::handle v_, pybind11::handle window, pybind11::handle sinks,
+                                           bool causal, pybind11::handle lengths_) {
+  for (pybind11::handle t : {q_, k_, v_})
+    if (!THPVariable_CheckTypeExact(Py_TYPE(t.ptr()))) return c10::nullopt;
+  if (!lengths_.is_none() && !THPVariable_CheckTypeExact(Py_TYPE(lengths_.ptr()))) return c10::nullopt;
+  auto w = c10::make_intrusive<Window>();
+  if (!int32_of(window, kNoWindow, &w->window) || !int32_of(sinks, -1, &w->sinks) || w->window < 1 || w->sinks < 0) return c10::nullopt;
+  w->causal = causal;
+  const at::Tensor q = THPVariable_Unpack(q_.ptr()), k = THPVariable_Unpack(k_.ptr()), v = THPVariable_Unpack(v_.ptr());
+  if (!lengths_.is_none()) w->lengths = THPVariable_Unpack(lengths_.ptr());
+  pybind11::gil_scoped_release no_gil;
+  if (transformed({&q, &k, &v})) return c10::nullopt;
+  for (const at::Tensor* t : {&q, &k, &v})
+    if (!t->is_cuda() || t->device() != q.device() || t->scalar_type() != q.scalar_type() || !takes_strides(*t)) return c10::nullopt;
+  if (q.scalar_type() != at::kBFloat16 && q.scalar_type() != at::kHalf) return c10::nullopt;
+  if (q.numel() == 0 || k.numel() == 0 || k.size(0) != q.size(0) || v.sizes() != k.sizes() || q.size(1) % k.size(1) != 0) return c10::nullopt;
+  if (w->lengths.defined() && (w->lengths.device() != q.device() || w->lengths.scalar_type() != at::kInt || w->lengths.dim() != 1 || w->lengths.size(0) != q.size(0) ||
+                               !w->lengths.is_contiguous() || q.size(2) != k.size(2)))
+    return c10::nullopt;
+  if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return WindowAttention::apply(q, k, v, std::move(w));
+  return run_window_forward(q, k, v, *w).first;
+}
+
+// The two passes for the Python autograd function; arguments have been checked and prepared.
+Window window_of(int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
+  Window w;
+  w.window = window;
+  w.sinks = sinks;
+  w.causal = causal;
+  if (lengths) w.lengths = *lengths;
+  return w;
+}
+std::pair<at::Tensor, at::Tensor> window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks, bool causal,
+                                                 const c10::optional<at::Tensor>& lengths) {
+  return run_window_forward(q, k, v, window_of(window, sinks, causal, lengths));
+}
+std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
+                                        const at::Tensor& d_o, int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
+  return run_window_backward(q, k, v, o, stats, d_o, window_of(window, sinks, causal, lengths));
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -679,5 +836,8 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward_on_mask", &forward_on_mask, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("backward_takes_mask", &backward_takes_mask_of);
   m.def("backward_on_mask", &backward_on_mask, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("window_attention", &window_attention);
+  m.def("window_forward", &window_forward, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("window_backward", &window_backward, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("backward", &backward_on_lists, pybind11::call_guard<pybind11::gil_scoped_release>());
 }

@@ -1,0 +1,265 @@
+// Forward of attention under a sliding window with sinks: gfx950, head_dim 128, bf16 or fp16 in / fp32 accumulate.
+//
+// One work-group of 4 waves owns 128 consecutive query rows of one (batch, head); wave w owns rows [32w, 32w+32).  Its keys are the slabs of 32 that hold
+// sinks some row sees, and those from the first row's window to the last row's.  Everything is transposed, as in the other forward kernels (lane = query row):
+//   S^T[key, q] = K Q^T,  P^T = exp2(c S^T - c m[q]),  O^T[d, q] += V^T P^T          c = log2(e) / sqrt(128)
+// with a running reference m and sum l per lane.  While the VALU turns S_t into P_t, the matrix pipe computes S_{t+1} and adds P_{t-1} V_{t-1} into O.  K and V
+// slabs travel global -> LDS directly into two rings of four buffers, four steps ahead.
+//
+// A slab that all 32 rows of a wave see whole needs no mask, one that none of them sees no work; of a window's slabs only the first and the last two or so
+// are masked, by two compares for every score.
+#include <type_traits>
+
+#include "fba_types.h"
+#include "fba_window.h"
+
+namespace fba {
+
+namespace {
+
+constexpr int kSlab = 32;
+constexpr int kSlabBytes = kSlab * kRowBytes;  // 8 KiB
+constexpr int kRing = 4;
+constexpr float kLazy = 8.f;             // log2 headroom before the softmax reference is raised
+constexpr float kNoReference = -3e38f;   // of a row that has met no score yet: finite, so that exp2 never sees inf - inf
+
+template <int N>
+using IC = std::integral_constant<int, N>;
+
+enum Kind { kNone, kFull, kMasked };
+
+}  // namespace
+
+template <typename T>
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2))) void window_fwd_kernel(const WindowParams p) {
+  extern __shared__ __attribute__((aligned(16))) char smem[];  // K ring [4][8 KiB] | V ring [4][8 KiB]
+  using x8 = x8_of<T>;
+  const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
+  const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+  int item = window_item(blockIdx.x, p.chunk);
+  if (item >= p.items) return;
+  // the query heads of a group together, then from tile to tile, late (under a long causal window: long) tiles first
+  const int group = p.Hq / p.Hkv;
+  const int g = item % group;
+  item /= group;
+  const int tile = p.tiles - 1 - item % p.tiles;
+  item /= p.tiles;
+  const int hkv = item % p.Hkv, b = item / p.Hkv, hq = hkv * group + g;
+
+  const int len = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.Skv) : p.Skv;
+  const int rows = p.lengths != nullptr ? len : p.Sq;  // that are not padding
+  const int shift = p.lengths != nullptr ? 0 : p.Skv - p.Sq;
+  const int row0 = tile * kWindowTile, ahead = p.causal ? 0 : p.window - 1;
+  const int last_row = min(row0 + kWindowTile, rows) - 1;  // below row0: all padding
+  // sinks that position `at` sees
+  auto sinks_at = [&](int at) { return min(min(p.sinks, len), p.causal ? at + 1 : p.sinks); };
+
+  // slabs of the tile
+  int n_sink = 0, first = 0, n = 0;
+  if (last_row >= row0 && len > 0) {
+    const int low = max(0, row0 + shift - p.window + 1), high = min(len - 1, last_row + shift + ahead);
+    n_sink = (max(0, sinks_at(last_row + shift)) + kSlab - 1) / kSlab;
+    first = max(low / kSlab, n_sink);
+    n = n_sink + (high >= low ? max(0, high / kSlab + 1 - first) : 0);
+  }
+  auto slab_of = [&](int t) { return t < n_sink ? t : first + t - n_sink; };
+
+  // what this lane's row sees: keys lo .. hi and those below sk; what the wave's rows see
+  const int wrow0 = row0 + wave * 32, row = wrow0 + l32, at = row + shift;
+  const bool there = row < rows;
+  const int hi = there ? min(len - 1, at + ahead) : -1, lo = at - p.window + 1, sk = there ? sinks_at(at) : 0;
+  const int wave_first = wrow0 + shift, wave_last = min(wrow0 + 32, rows) - 1 + shift;
+  const bool idle = wrow0 >= rows, whole = wrow0 + 32 <= rows;  // (rows of padding see nothing)
+  const int all_hi = min(len - 1, wave_first + ahead), all_lo = wave_last - p.window + 1, all_sk = sinks_at(wave_first);
+  const int any_hi = min(len - 1, wave_last + ahead), any_lo = wave_first - p.window + 1, any_sk = sinks_at(wave_last);
+  auto kind_of = [&](int t) -> int {
+    if (t >= n || idle) return kNone;
+    const int k0 = slab_of(t) * kSlab, k1 = k0 + kSlab - 1;
+    if (whole && ((k1 <= all_hi && k0 >= all_lo) || k1 < all_sk)) return kFull;
+    return (k0 <= any_hi && k1 >= any_lo) || k0 < any_sk ? kMasked : kNone;
+  };
+
+  const char* const kp = p.k.ptr + b * p.k.batch + hkv * p.k.head;
+  const char* const vp = p.v.ptr + b * p.v.batch + hkv * p.v.head;
+  const int64_t k_step = (int64_t)p.k.row * kSlab, v_step = (int64_t)p.v.row * kSlab;
+
+  f32x16 acc[4];
+  float l_run = 0.f, m_run = kNoReference;
+  const float c = p.scale_log2e;
+#pragma unroll
+  for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+    for (int r = 0; r < 16; ++r) acc[mb][r] = 0.f;
+
+  if (n > 0) {
+    // Q as the B operand: lane holds row l32, d = 16 ks + 8 h .. +7 (rows behind the last: that one)
+    x8 qreg[8];
+    const char* qp = p.q.ptr + b * p.q.batch + hq * p.q.head + (int64_t)min(row, rows - 1) * p.q.row;
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) qreg[ks] = *reinterpret_cast<const x8*>(qp + 32 * ks + 16 * h);
+    RowMajorOffsets rm;
+    rm.init(lane);
+    TransposedOffsets tr;
+    tr.init(lane);
+    RowDma k_dma, v_dma;
+    k_dma.init(wave, lane, p.k.row, len - 1);
+    v_dma.init(wave, lane, p.v.row, len - 1);
+    const LdsPtr k_lds = lds_ptr(smem), v_lds = lds_ptr(smem + kRing * kSlabBytes);
+    const uint32_t k_dst = lds_addr(smem), v_dst = k_dst + kRing * kSlabBytes;
+    // past the last slab: that one again, into a buffer that nobody reads any more, so that the counter of copies in flight means the same at every wait
+    auto slab_at = [&](int t) { return slab_of(min(t, n - 1)); };
+
+#pragma unroll
+    for (int j = 0; j < 4; ++j) {
+      const int slab = slab_at(j);
+      k_dma.copy(k_dst + j * kSlabBytes, kp + slab * k_step, slab);
+    }
+#pragma unroll
+    for (int j = 0; j < 3; ++j) {
+      const int slab = slab_at(j);
+      v_dma.copy(v_dst + j * kSlabBytes, vp + slab * v_step, slab);
+    }
+    wait_vmem<0>();
+    __syncthreads();
+#pragma unroll
+    for (int ks = 0; ks < 8; ++ks) pin(qreg[ks]);
+
+    auto scores = [&](LdsPtr slab) {  // S^T of a slab
+      f32x16 s;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s[r] = 0.f;
+#pragma unroll
+      for (int ks = 0; ks < 8; ++ks) s = Elem<T>::mfma32(read_b128<T>(slab + rm.rd[ks]), qreg[ks], s);
+      return s;
+    };
+    int kind = kind_of(0), kind_before = kNone;
+    f32x16 s_cur;
+#pragma unroll
+    for (int r = 0; r < 16; ++r) s_cur[r] = 0.f;
+    if (kind != kNone) s_cur = scores(k_lds);
+    pin(s_cur);
+    __syncthreads();
+    int owed_k = slab_at(4), owed_v = slab_at(3);  // slabs that the next step requests
+    k_dma.copy(k_dst, kp + owed_k * k_step, owed_k);
+
+    x8 p_prev[2];
+#pragma unroll
+    for (int j = 0; j < 2; ++j)
+#pragma unroll
+      for (int i = 0; i < 8; ++i) p_prev[j][i] = (T)0.f;
+    uint32_t k_into = 0, v_into = 0;
+    bool owed = false;
+
+    // O += P V of the slab in `buf`; the copies that the step owes go between the matrix instructions
+    auto add_pv = [&](LdsPtr buf, auto between) {
+#pragma unroll
+      for (int j = 0; j < 2; ++j)
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb) {
+          const int roff = 16 * j * kRowBytes;
+          acc[mb] = Elem<T>::mfma32(read_tr8<T>(buf + tr.rd[mb][0] + roff, buf + tr.rd[mb][1] + roff), p_prev[j], acc[mb]);
+          between(4 * j + mb);
+        }
+    };
+    // step t (t % 4 == R): O += P_{t-1} V_{t-1} | softmax(S_t) | S_{t+1} = K_{t+1} Q^T
+    auto step = [&](auto ring_c, int t) {
+      constexpr int R = decltype(ring_c)::value;
+      // P_{t-1} was formed against the reference m of step t-1, so it reaches O before step t may raise m
+      if (kind_before != kNone) {
+        add_pv(v_lds + ((R + 3) & 3) * kSlabBytes, [&](int i) {
+          if (i == 0) k_dma.piece(0, k_into, kp + owed_k * k_step, owed_k);
+          if (i == 2) k_dma.piece(1, k_into, kp + owed_k * k_step, owed_k);
+          if (i == 4) v_dma.piece(0, v_into, vp + owed_v * v_step, owed_v);
+          if (i == 6) v_dma.piece(1, v_into, vp + owed_v * v_step, owed_v);
+        });
+      } else if (owed) {
+        k_dma.copy(k_into, kp + owed_k * k_step, owed_k);
+        v_dma.copy(v_into, vp + owed_v * v_step, owed_v);
+      }
+      const int kind_next = kind_of(t + 1);
+      if (kind == kMasked) {
+        const int k0 = slab_of(t) * kSlab + 4 * h, a = lo - k0, z = hi - k0, y = sk - k0;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const int e = 8 * (r >> 2) + (r & 3);
+          s_cur[r] = (e >= a && e <= z) || e < y ? s_cur[r] : -INFINITY;
+        }
+      }
+      if (kind != kNone) {
+        // raise the reference if some row would otherwise see exponents above kLazy
+        float mx = s_cur[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
+        if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kLazy) != 0) {
+          const float m_new = fmaxf(m_run, max_halves(mx));
+          const float alpha = fast_exp2((m_run - m_new) * c);
+          m_run = m_new;
+          l_run *= alpha;
+#pragma unroll
+          for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+            for (int r = 0; r < 16; ++r) acc[mb][r] *= alpha;
+        }
+      }
+      f32x16 s_nxt = s_cur;
+      if (kind_next != kNone) s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
+      if (kind != kNone) {
+        const float mc = m_run * c;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s_cur[r] = fast_exp2(__builtin_fmaf(s_cur[r], c, -mc));
+        const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one
+          p_prev[j] = narrow8<T>(s_cur, j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);
+        }
+      }
+      pin(p_prev[0]);
+      pin(p_prev[1]);
+      s_cur = s_nxt;
+      kind_before = kind;
+      kind = kind_next;
+      // K_{t+2} and V_t must have landed; the copies requested by steps t-2 and t-1 may still fly
+      wait_vmem<8>();
+      __syncthreads();
+      // K_{t+5} into the buffer of K_{t+1}, V_{t+3} into that of V_{t-1}
+      owed_k = slab_at(t + 5);
+      owed_v = slab_at(t + 3);
+      k_into = k_dst + ((R + 1) & 3) * kSlabBytes;
+      v_into = v_dst + ((R + 3) & 3) * kSlabBytes;
+      owed = true;
+    };
+    for (int t = 0;; t += 4) {
+      step(IC<0>{}, t);
+      if (t + 1 >= n) break;
+      step(IC<1>{}, t + 1);
+      if (t + 2 >= n) break;
+      step(IC<2>{}, t + 2);
+      if (t + 3 >= n) break;
+      step(IC<3>{}, t + 3);
+      if (t + 4 >= n) break;
+    }
+    if (kind_before != kNone) add_pv(v_lds + ((n - 1) & 3) * kSlabBytes, [](int) {});
+    wait_vmem<0>();   // no copy may still be writing LDS
+    __syncthreads();  // and everybody is done with the rings
+  }
+
+  const float l = sum_halves(l_run);
+  if (h == 0 && row < p.Sq) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l > 0.f ? m_run * c + __builtin_log2f(l) : INFINITY;
+  store_tile<T>(smem + wave * kSlabBytes, acc, l > 0.f ? 1.f / l : 0.f, p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)wrow0 * p.o.row, p.o.row, lane,
+                p.Sq - wrow0);
+}
+
+hipError_t launch_window_fwd(WindowParams p, bool half, hipStream_t stream) {
+  constexpr int kSmem = 2 * kRing * kSlabBytes;
+  p.tiles = (p.Sq + kWindowTile - 1) / kWindowTile;
+  p.items = p.B * p.Hq * p.tiles;
+  p.chunk = window_chunk(p.items);
+  void (*fn)(const WindowParams) = half ? &window_fwd_kernel<_Float16> : &window_fwd_kernel<__bf16>;
+  hipLaunchKernelGGL(fn, dim3(window_grid(p.items, p.chunk)), dim3(256), kSmem, stream, p);
+  return hipGetLastError();
+}
+
+}  // namespace fba

@@ -36,7 +36,7 @@ extern "C" {
 
 /* Library version: major * 1000 + minor; the minor number goes up whenever an argument list in this header changes, so a
  * binding can refuse a library built from another header (flex_block_attn_amd/_lib.py does). */
-#define FBA_VERSION 2011
+#define FBA_VERSION 2012
 int32_t fba_version(void);
 
 /* Message for the last non-OK return on the calling thread ("" if none). The pointer stays valid until the next
@@ -368,6 +368,36 @@ int32_t fba_ssta_mask_3d(const float* q_mean, const float* k_mean, uint8_t* mask
                          int32_t nW, int32_t half_t, int32_t half_h, int32_t half_w, int32_t topk, int32_t sink, void* hip_stream);
 int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int32_t H, int32_t W, int32_t tile_t,
                          int32_t tile_h, int32_t tile_w, int32_t head_dim, int32_t to_tiles, void* hip_stream);
+
+/*
+ * Attention under a sliding window with sinks, at the granularity of tokens (no counterpart in the reference, whose masks are of blocks).
+ *
+ * Query row i stands at position p = i + Skv - Sq; with `lengths` (int32 [B], Sq = Skv) sequence b has lengths[b] tokens (values outside of [0, Skv]
+ * count as the nearest of the two), its other rows are padding and row i stands at i.  Key j is visible to row i when both are tokens and
+ *   causal != 0:  j <= p and (p - j < window or j < sinks)        causal = 0:  |p - j| < window or j < sinks
+ * o = softmax(q k^T / sqrt(128)) v over the visible keys; rows without any, and padding, are zeros, and so are their gradients.  Padding of q, k, v and d_o
+ * is not read.  A value of v that is no number or infinite reaches the rows that see it, and others of its 32-row neighbourhood.
+ *
+ * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
+ * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [2, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first half (+inf
+ * for rows without a visible key), backward uses the second.
+ * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes, 16-byte aligned, for partial sums of keys with sinks (0 bytes: may be null).
+ * Sq and Skv at most 2^28, B * Hq * Sq and B * Hkv * Skv below 2^29.
+ */
+#define FBA_BF16 0
+#define FBA_FP16 1
+typedef struct {
+  void* ptr;
+  int64_t batch, head, row; /* strides in elements */
+} fba_strided;
+int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, float* stats, const int32_t* lengths, int32_t B,
+                       int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
+                       void* hip_stream);
+int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal);
+int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* d_o, float* stats,
+                       const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
+                       int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
+                       void* hip_stream);
 
 /*
  * Diagnostic, no counterpart in the reference: `work_groups` x 4 waves each issue `iters` x 4 independent
