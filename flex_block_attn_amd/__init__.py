@@ -13,6 +13,7 @@ from .interface import (
     tile_block_mask,
 )
 from . import masks, video
+from .cache import PagedCache, cache_append, cache_attn_func, cache_evict, paged_cache
 from .video import (
     block_mean,
     create_moba_3d_mask,
@@ -49,4 +50,9 @@ __all__ = [
     "untile_tokens",
     "window_attn_func",
     "WindowAttnFunc",
+    "PagedCache",
+    "paged_cache",
+    "cache_append",
+    "cache_attn_func",
+    "cache_evict",
 ]

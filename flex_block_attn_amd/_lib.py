@@ -71,6 +71,11 @@ SIGNATURES = {
     "fba_window_fwd": (_c_i32, [_c_ptr] * 6 + [_c_i32] * 10 + [_c_ptr]),
     "fba_window_workspace_bytes": (_c_i64, [_c_i32] * 8),
     "fba_window_bwd": (_c_i32, [_c_ptr] * 11 + [_c_i64] + [_c_i32] * 10 + [_c_ptr]),
+    "fba_cache_append": (_c_i32, [_c_ptr] * 6 + [_c_i32] + [_c_ptr] * 2),
+    "fba_cache_attn_workspace_bytes": (_c_i64, [_c_ptr] + [_c_i32] * 2),
+    "fba_cache_attn": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 5 + [_c_ptr, _c_i64, _c_ptr]),
+    "fba_cache_evict_workspace_bytes": (_c_i64, [_c_ptr, _c_i32]),
+    "fba_cache_evict": (_c_i32, [_c_ptr] + [_c_i32] * 3 + [_c_ptr] * 2 + [_c_i64, _c_ptr]),
     "fba_bwd_stats": (_c_i32, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr]),
     "fba_bwd_dq": (_c_i32, [_c_ptr] * 8 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),
     "fba_bwd_dkdv": (_c_i32, [_c_ptr] * 9 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),

@@ -7,6 +7,7 @@
 #include <mutex>
 
 #include "../../include/fba.h"
+#include "fba_cache.h"
 #include "fba_kernels.h"
 #include "fba_window.h"
 
@@ -971,6 +972,145 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
   p.parts = (float*)ws;
   hipError_t e = fba::launch_window_bwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window backward launch");
+}
+
+}  // extern "C"
+
+// ---------------------------------------------------------------------------------------------------------------------
+// the paged cache
+// ---------------------------------------------------------------------------------------------------------------------
+namespace {
+
+int take_cache(fba::CacheView& to, const fba_cache* c) {
+  if (c == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  if (int rc = check_ptrs({{"cache k", c->k}, {"cache v", c->v}})) return rc;
+  if (c->batch <= 0 || c->max_pages <= 0 || c->kv_heads <= 0 || c->pages <= 0)
+    return fail(FBA_ERR_INVALID, "pages, kv_heads, batch and max_pages must be positive (got %lld %d %d %d)", (long long)c->pages, c->kv_heads, c->batch, c->max_pages);
+  if (c->page_size < 16 || (c->page_size & (c->page_size - 1))) return fail(FBA_ERR_INVALID, "page_size (%d) must be a power of two, 16 at least", c->page_size);
+  if (c->table == nullptr || c->lengths == nullptr) return fail(FBA_ERR_INVALID, "table or lengths is null");
+  if (c->weights != nullptr && !aligned16(c->weights)) return fail(FBA_ERR_INVALID, "weights is not 16-byte aligned");
+  const int64_t slots = (int64_t)c->max_pages * c->page_size;
+  if (c->pages > 0x7fffffffLL || slots > 1LL << 28 || slots * c->batch > 1LL << 36 || (int64_t)c->batch * c->kv_heads > 1 << 24)
+    return fail(FBA_ERR_UNSUPPORTED, "a sequence may have 2^28 slots at most, all together 2^36, batch * kv_heads 2^24 (got %lld slots, batch %d, kv_heads %d)", (long long)slots,
+                c->batch, c->kv_heads);
+  to.k = (char*)c->k;
+  to.v = (char*)c->v;
+  to.positions = c->positions;
+  to.weights = c->weights;
+  to.table = c->table;
+  to.lengths = c->lengths;
+  to.pages = c->pages;
+  to.kv_heads = c->kv_heads;
+  to.page_log2 = __builtin_ctz((unsigned)c->page_size);
+  to.batch = c->batch;
+  to.max_pages = c->max_pages;
+  return FBA_OK;
+}
+
+int take_attend(fba::AttendParams& p, const fba_cache* cache, int32_t heads, int32_t accumulate) {
+  if (int rc = take_cache(p.cache, cache)) return rc;
+  if (heads <= 0 || heads % cache->kv_heads != 0) return fail(FBA_ERR_INVALID, "heads (%d) must be a multiple of kv_heads (%d)", heads, cache->kv_heads);
+  if (accumulate && cache->weights == nullptr) return fail(FBA_ERR_INVALID, "weights is null");
+  if (heads > 65535) return fail(FBA_ERR_UNSUPPORTED, "heads (%d) may be 65535 at most", heads);
+  p.heads = heads;
+  fba::plan_cache_attend(p, fba::device_compute_units());
+  const int64_t spans = (p.cache.slots() + 1023) / 1024;
+  if ((int64_t)p.slots * heads > 1LL << 30 || (accumulate && spans * cache->kv_heads * cache->batch > 1LL << 30))
+    return fail(FBA_ERR_UNSUPPORTED, "batch (%d) and heads (%d) are too many for one call", cache->batch, heads);
+  return FBA_OK;
+}
+
+int check_ws(const void* ws, int64_t bytes, int64_t need) {
+  if (need > 0 && (ws == nullptr || !aligned16(ws) || bytes < need))
+    return fail(FBA_ERR_INVALID, "ws must be 16-byte aligned and hold %lld bytes, got %lld", (long long)need, (long long)bytes);
+  return FBA_OK;
+}
+
+int take_evict(fba::EvictParams& p, const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks) {
+  if (int rc = take_cache(p.cache, cache)) return rc;
+  if (budget < 1) return fail(FBA_ERR_INVALID, "budget (%d) must be at least 1", budget);
+  if (recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget)
+    return fail(FBA_ERR_INVALID, "recent (%d) and sinks (%d) must not be negative, and fit the budget (%d) together", recent, sinks, budget);
+  if ((int64_t)cache->batch * cache->kv_heads > 65535) return fail(FBA_ERR_UNSUPPORTED, "batch * kv_heads may be 65535 at most");
+  p.budget = budget;
+  p.recent = recent;
+  p.sinks = sinks;
+  return FBA_OK;
+}
+
+}  // namespace
+
+extern "C" {
+
+int32_t fba_cache_append(const fba_cache* cache, const fba_strided* k, const fba_strided* v, const int32_t* counts, const int32_t* first, const float* weights,
+                         int32_t tokens, int32_t* lengths_out, void* hip_stream) {
+  fba::AppendParams p{};
+  if (int rc = take_cache(p.cache, cache)) return rc;
+  if (tokens <= 0 || tokens > 1 << 28) return fail(FBA_ERR_INVALID, "tokens (%d) must be positive, 2^28 at most", tokens);
+  if (int rc = take_strided(p.k, k, "k")) return rc;
+  if (int rc = take_strided(p.v, v, "v")) return rc;
+  if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
+  if (lengths_out == cache->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
+  if ((int64_t)cache->batch * cache->kv_heads > 0x7fffffffLL) return fail(FBA_ERR_UNSUPPORTED, "batch * kv_heads is too large");
+  p.counts = counts;
+  p.first = first;
+  p.weights = weights;
+  p.tokens = tokens;
+  p.lengths_out = lengths_out;
+  hipError_t e = fba::launch_cache_append(p, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache append launch");
+}
+
+int64_t fba_cache_attn_workspace_bytes(const fba_cache* cache, int32_t heads, int32_t accumulate) {
+  fba::AttendParams p{};
+  if (take_attend(p, cache, heads, accumulate)) return -1;
+  return fba::cache_attend_bytes(p, accumulate != 0);
+}
+
+int32_t fba_cache_attn(const fba_cache* cache, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate,
+                       int32_t type, void* ws, int64_t ws_bytes, void* hip_stream) {
+  fba::AttendParams p{};
+  if (int rc = take_attend(p, cache, heads, accumulate)) return rc;
+  if (type != FBA_BF16 && type != FBA_FP16) return fail(FBA_ERR_INVALID, "type must be FBA_BF16 or FBA_FP16, got %d", type);
+  if (int rc = take_strided(p.q, q, "q")) return rc;
+  if (int rc = take_strided(p.o, o, "o")) return rc;
+  if (window < 1) return fail(FBA_ERR_INVALID, "window (%d) must be at least 1", window);
+  if (sinks < 0) return fail(FBA_ERR_INVALID, "sinks (%d) must not be negative", sinks);
+  if (accumulate && window < p.cache.slots()) return fail(FBA_ERR_INVALID, "weights are added up over the whole cache: window (%d) must reach over its %lld slots", window, (long long)p.cache.slots());
+  if (int rc = check_ws(ws, ws_bytes, fba::cache_attend_bytes(p, accumulate != 0))) return rc;
+  p.window = window;
+  p.sinks = sinks;
+  p.scale_log2e = 1.4426950408889634f / 11.313708498984761f;
+  const int64_t parts = (int64_t)p.slots * heads;
+  float* at = (float*)ws;
+  if (accumulate) {
+    p.scores = at;
+    at += (int64_t)cache->batch * heads * p.cache.slots();
+  }
+  p.part = at;
+  p.part_ml = p.part + parts * 128;
+  p.note = (int32_t*)(p.part_ml + parts * 2);
+  hipError_t e = fba::launch_cache_attend(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache attention launch");
+}
+
+int64_t fba_cache_evict_workspace_bytes(const fba_cache* cache, int32_t budget) {
+  fba::EvictParams p{};
+  if (take_evict(p, cache, budget, 0, 0)) return -1;
+  return fba::cache_evict_bytes(p);
+}
+
+int32_t fba_cache_evict(const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream) {
+  fba::EvictParams p{};
+  if (int rc = take_evict(p, cache, budget, recent, sinks)) return rc;
+  if (cache->positions == nullptr || cache->weights == nullptr) return fail(FBA_ERR_INVALID, "positions or weights is null");
+  if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
+  if (lengths_out == cache->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
+  if (int rc = check_ws(ws, ws_bytes, fba::cache_evict_bytes(p))) return rc;
+  p.lengths_out = lengths_out;
+  p.moves = (int32_t*)ws;
+  hipError_t e = fba::launch_cache_evict(p, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache eviction launch");
 }
 
 }  // extern "C"

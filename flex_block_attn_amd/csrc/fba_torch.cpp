@@ -42,7 +42,8 @@ constexpr int64_t kXcds = 8;
 #define FBA_FUNCTIONS(X)                                                                                                \
   X(fba_version) X(fba_last_error) X(fba_split_workspace_bytes) X(fba_lists_cut) X(fba_pair_slots_bounds) X(fba_tile_slots_bounds)        \
   X(fba_fwd) X(fba_fwd_tiled) X(fba_fwd_blocks) X(fba_fwd_blocks_use) X(fba_fwd_mask_copy) X(fba_fwd_takes_mask) X(fba_bwd_mask) X(fba_bwd_takes_mask) X(fba_bwd) X(fba_bwd_handover) X(fba_bwd_tiled_cut) X(fba_bwd_dense) \
-  X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd)
+  X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd) \
+  X(fba_cache_append) X(fba_cache_attn_workspace_bytes) X(fba_cache_attn) X(fba_cache_evict_workspace_bytes) X(fba_cache_evict)
 
 struct Library {
 #define DECLARE(f) decltype(&::f) f = nullptr;
@@ -824,6 +825,116 @@ std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k
   return run_window_backward(q, k, v, o, stats, d_o, window_of(window, sinks, causal, lengths));
 }
 
+// ---------------------------------------------------------------------------------------------------------------------
+// the paged cache
+// ---------------------------------------------------------------------------------------------------------------------
+// Tensors of a call as Python hands them over: nothing where one is no plain tensor.
+bool plain(std::initializer_list<pybind11::handle> objects) {
+  for (pybind11::handle o : objects)
+    if (!o.is_none() && !THPVariable_CheckTypeExact(Py_TYPE(o.ptr()))) return false;
+  return true;
+}
+at::Tensor tensor_of(pybind11::handle o) { return o.is_none() ? at::Tensor() : at::Tensor(THPVariable_Unpack(o.ptr())); }
+
+bool is_ints(const at::Tensor& t, const at::Tensor& like, int64_t n) {
+  return t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
+}
+
+// The cache as the library takes it; false where something does not fit, which Python then reports.
+bool cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& positions, const at::Tensor& weights, const at::Tensor& table, const at::Tensor& lengths,
+              fba_cache* c) {
+  if (!k.defined() || !v.defined() || !table.defined() || !lengths.defined()) return false;
+  if (!k.is_cuda() || k.dim() != 4 || k.size(3) != kHeadDim || !k.is_contiguous() || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf)) return false;
+  if (v.device() != k.device() || v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || !v.is_contiguous()) return false;
+  for (const at::Tensor* t : {&positions, &weights})
+    if (t->defined() && (t->device() != k.device() || t->scalar_type() != (t == &positions ? at::kInt : at::kFloat) || t->sizes() != k.sizes().slice(0, 3) || !t->is_contiguous()))
+      return false;
+  const int64_t page = k.size(2);
+  if (k.numel() == 0 || k.size(0) > 0x7fffffffLL || k.size(1) > 65535 || page < 16 || page > 1 << 28 || (page & (page - 1)) != 0) return false;
+  if (table.device() != k.device() || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || table.numel() == 0) return false;
+  if (table.size(0) > 0x7fffff || table.size(1) * page > 1LL << 28 || !is_ints(lengths, k, table.size(0))) return false;
+  for (const at::Tensor* t : {&k, &v, &weights})
+    if (t->defined() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) != 0) return false;
+  *c = {k.data_ptr(), v.data_ptr(), positions.defined() ? positions.data_ptr<int32_t>() : nullptr, weights.defined() ? weights.data_ptr<float>() : nullptr,
+        table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), k.size(0), (int32_t)k.size(1), (int32_t)page, (int32_t)table.size(0), (int32_t)table.size(1)};
+  return true;
+}
+
+bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
+  if (!at::GradMode::is_enabled()) return false;
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && t->requires_grad()) return true;
+  return false;
+}
+
+// The entry points of cache.py: nothing for arguments that do not fit, which Python then prepares or reports.
+c10::optional<at::Tensor> cache_attention(pybind11::handle q_, pybind11::handle k_, pybind11::handle v_, pybind11::handle weights_, pybind11::handle table_,
+                                          pybind11::handle lengths_, pybind11::handle window_, pybind11::handle sinks_, bool accumulate) {
+  int64_t window, sinks;
+  if (!plain({q_, k_, v_, weights_, table_, lengths_}) || !int32_of(window_, kNoWindow, &window) || !int32_of(sinks_, -1, &sinks) || window < 1 || sinks < 0) return c10::nullopt;
+  const at::Tensor q = tensor_of(q_), k = tensor_of(k_), v = tensor_of(v_), weights = tensor_of(weights_), table = tensor_of(table_), lengths = tensor_of(lengths_);
+  pybind11::gil_scoped_release no_gil;
+  fba_cache cache;
+  if (!cache_of(k, v, at::Tensor(), weights, table, lengths, &cache) || (accumulate && (!weights.defined() || window < kNoWindow))) return c10::nullopt;
+  if (!q.defined() || q.device() != k.device() || q.scalar_type() != k.scalar_type() || !takes_strides(q) || q.size(0) != cache.batch || q.size(2) != 1 || q.numel() == 0 ||
+      q.size(1) % cache.kv_heads != 0 || q.size(1) > 65535)
+    return c10::nullopt;
+  if (transformed({&q, &k, &v}) || wants_grad({&q, &k, &v, &weights})) return c10::nullopt;
+  const c10::DeviceGuard guard(q.device());
+  at::Tensor o = at::empty(q.sizes(), q.options());
+  const int64_t bytes = lib.fba_cache_attn_workspace_bytes(&cache, q.size(1), accumulate);
+  if (bytes < 0) raise_call_error(FBA_ERR_UNSUPPORTED);
+  SplitWorkspace ws(q, bytes);
+  const fba_strided sq = strided(q), so = strided(o);
+  check(lib.fba_cache_attn(&cache, &sq, &so, q.size(1), window, sinks, accumulate, type_of(q), ws.ptr(), bytes, current_stream(q)));
+  return o;
+}
+
+c10::optional<at::Tensor> cache_append(pybind11::handle cache_k_, pybind11::handle cache_v_, pybind11::handle positions_, pybind11::handle weights_, pybind11::handle table_,
+                                       pybind11::handle lengths_, pybind11::handle k_, pybind11::handle v_, pybind11::handle counts_, pybind11::handle first_,
+                                       pybind11::handle given_) {
+  if (!plain({cache_k_, cache_v_, positions_, weights_, table_, lengths_, k_, v_, counts_, first_, given_})) return c10::nullopt;
+  const at::Tensor ck = tensor_of(cache_k_), cv = tensor_of(cache_v_), positions = tensor_of(positions_), weights = tensor_of(weights_), table = tensor_of(table_),
+                   lengths = tensor_of(lengths_), k = tensor_of(k_), v = tensor_of(v_), counts = tensor_of(counts_), first = tensor_of(first_), given = tensor_of(given_);
+  pybind11::gil_scoped_release no_gil;
+  fba_cache cache;
+  if (!cache_of(ck, cv, positions, weights, table, lengths, &cache) || !k.defined() || !v.defined()) return c10::nullopt;
+  for (const at::Tensor* t : {&k, &v})
+    if (t->device() != ck.device() || t->scalar_type() != ck.scalar_type() || !takes_strides(*t) || t->sizes() != k.sizes()) return c10::nullopt;
+  if (k.size(0) != cache.batch || k.size(1) != cache.kv_heads || k.size(2) < 1 || k.size(2) > 1 << 28) return c10::nullopt;
+  if ((counts.defined() && !is_ints(counts, ck, cache.batch)) || (first.defined() && (!positions.defined() || !is_ints(first, ck, cache.batch)))) return c10::nullopt;
+  if (given.defined() && (!weights.defined() || given.device() != ck.device() || given.scalar_type() != at::kFloat || given.sizes() != k.sizes().slice(0, 3) || !given.is_contiguous()))
+    return c10::nullopt;
+  if (transformed({&ck, &cv, &k, &v}) || wants_grad({&ck, &cv, &weights, &k, &v, &given})) return c10::nullopt;
+  const c10::DeviceGuard guard(ck.device());
+  at::Tensor out = at::empty_like(lengths);
+  const fba_strided sk = strided(k), sv = strided(v);
+  auto ints_of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; };
+  check(lib.fba_cache_append(&cache, &sk, &sv, ints_of(counts), ints_of(first), given.defined() ? given.data_ptr<float>() : nullptr, k.size(2), out.data_ptr<int32_t>(),
+                             current_stream(ck)));
+  return out;
+}
+
+c10::optional<at::Tensor> cache_evict(pybind11::handle k_, pybind11::handle v_, pybind11::handle positions_, pybind11::handle weights_, pybind11::handle table_,
+                                      pybind11::handle lengths_, pybind11::handle budget_, pybind11::handle recent_, pybind11::handle sinks_) {
+  int64_t budget, recent, sinks;
+  if (!plain({k_, v_, positions_, weights_, table_, lengths_}) || !int32_of(budget_, -1, &budget) || !int32_of(recent_, -1, &recent) || !int32_of(sinks_, -1, &sinks) || budget < 1 ||
+      recent < 0 || sinks < 0 || recent + sinks > budget)
+    return c10::nullopt;
+  const at::Tensor k = tensor_of(k_), v = tensor_of(v_), positions = tensor_of(positions_), weights = tensor_of(weights_), table = tensor_of(table_), lengths = tensor_of(lengths_);
+  pybind11::gil_scoped_release no_gil;
+  fba_cache cache;
+  if (!positions.defined() || !weights.defined() || !cache_of(k, v, positions, weights, table, lengths, &cache)) return c10::nullopt;
+  if (transformed({&k, &v}) || wants_grad({&k, &v, &weights})) return c10::nullopt;
+  const c10::DeviceGuard guard(k.device());
+  const int64_t bytes = lib.fba_cache_evict_workspace_bytes(&cache, budget);
+  if (bytes < 0) raise_call_error(FBA_ERR_UNSUPPORTED);
+  SplitWorkspace ws(k, bytes);
+  at::Tensor out = at::empty_like(lengths);
+  check(lib.fba_cache_evict(&cache, budget, recent, sinks, out.data_ptr<int32_t>(), ws.ptr(), bytes, current_stream(k)));
+  return out;
+}
+
 }  // namespace
 
 PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
@@ -836,6 +947,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("forward_on_mask", &forward_on_mask, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("backward_takes_mask", &backward_takes_mask_of);
   m.def("backward_on_mask", &backward_on_mask, pybind11::call_guard<pybind11::gil_scoped_release>());
+  m.def("cache_attention", &cache_attention);
+  m.def("cache_append", &cache_append);
+  m.def("cache_evict", &cache_evict);
   m.def("window_attention", &window_attention);
   m.def("window_forward", &window_forward, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("window_backward", &window_backward, pybind11::call_guard<pybind11::gil_scoped_release>());

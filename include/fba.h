@@ -400,6 +400,45 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
                        void* hip_stream);
 
 /*
+ * A paged cache of keys and values, and attention of single new tokens over it (no counterpart in the reference).
+ *
+ * k, v: a pool [pages, kv_heads, page_size, 128] of 16-bit values; positions (int32) and weights (fp32) [pages, kv_heads, page_size] go with its slots.  page_size is a
+ * power of two, 16 at least.  Slot s of sequence b is slot s % page_size of page table[b, s / page_size] (table [batch, max_pages]); its first lengths[b] slots are
+ * filled.  table and lengths are read on the device.  A length below 0 or beyond the table, or a page that is none of the pool's among those that a call needs,
+ * cannot be reported by the return code: nothing is read or written outside of the pool, and the call answers for that sequence as stated with each.  A page that a call
+ * writes to may be in one place of the table only.
+ *
+ * fba_cache_append: tokens 0 .. counts[b] - 1 (null: all `tokens`) of k, v [batch, kv_heads, tokens, 128] go to the slots from lengths[b] on; positions, if there are
+ *   any, become first[b] (null: lengths[b]) and so on, weights those given [batch, kv_heads, tokens] (null: 0).  lengths_out[b] = lengths[b] + counts[b].  Where
+ *   lengths or counts make no sense or there is no room nothing is written, for a page outside of the pool not its rows, and lengths_out[b] = -1.
+ * fba_cache_attn: o[b, h] = softmax(q[b, h] k^T / sqrt(128)) v over the slots s < lengths[b] with s >= lengths[b] - window or s < sinks; zeros where there are none,
+ *   NaN for a sequence with a wrong length or page.  q, o [batch, heads, 1, 128].  accumulate != 0: weights[slot] += the sum over the query heads of a kv head
+ *   of what softmax gives the slot (window must then reach over all slots); a sequence whose o is NaN adds nothing.
+ * fba_cache_evict: brings every sequence of more than `budget` slots down to that, head by head: kept are the slots whose position is below `sinks` or among the last
+ *   `recent` ones (above the largest position - recent), then those with the largest weights, of equal ones the lower slot.  The i-th slot below `budget` that is freed
+ *   receives the i-th kept one from `budget` on: row, position and weight; all other slots stay as they are.  lengths_out[b] = min(lengths[b], budget); -1, and nothing
+ *   moved, for a wrong length or page.  NaN is the lowest weight.  recent + sinks <= budget.
+ * Workspaces: as many bytes as the function of that name says, 16-byte aligned.  fba_cache_attn needs a multiple of the cache's scores with accumulate, little without.
+ */
+typedef struct {
+  void* k;
+  void* v;
+  int32_t* positions; /* may be null, but for fba_cache_evict */
+  float* weights;     /* may be null, but for fba_cache_evict and accumulate */
+  const int32_t* table;
+  const int32_t* lengths;
+  int64_t pages;
+  int32_t kv_heads, page_size, batch, max_pages;
+} fba_cache;
+int32_t fba_cache_append(const fba_cache* cache, const fba_strided* k, const fba_strided* v, const int32_t* counts, const int32_t* first, const float* weights,
+                         int32_t tokens, int32_t* lengths_out, void* hip_stream);
+int64_t fba_cache_attn_workspace_bytes(const fba_cache* cache, int32_t heads, int32_t accumulate);
+int32_t fba_cache_attn(const fba_cache* cache, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate,
+                       int32_t type, void* ws, int64_t ws_bytes, void* hip_stream);
+int64_t fba_cache_evict_workspace_bytes(const fba_cache* cache, int32_t budget);
+int32_t fba_cache_evict(const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream);
+
+/*
  * Diagnostic, no counterpart in the reference: `work_groups` x 4 waves each issue `iters` x 4 independent
  * v_mfma_f32_32x32x16_bf16 on register operands taken from src (1024 floats in device memory; null: all-zero operands)
  * and write a checksum per thread to sink (work_groups * 256 floats).  The launch executes
