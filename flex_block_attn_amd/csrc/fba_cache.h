@@ -49,10 +49,10 @@ struct AttendParams {
   Strided q, o;              // [batch, heads, 1, 128]
   int heads, window, sinks;
   float scale_log2e;
-  int target;                // chunks of all sequences together, for a kv head
-  int head_tiles;            // work-groups that share a chunk of a kv head
-  int slots;                 // chunks there may be
-  // workspace: sums of the chunks [slots, heads, 128], their references and denominators [slots, heads, 2], first chunk and number of chunks of a sequence
+  int target;                // shares that the tiles of all sequences are cut into, at most
+  int head_tiles;            // work-groups that share a share of a kv head
+  int slots;                 // places for parts of sequences
+  // workspace: sums of the parts [slots, heads, 128], their references and denominators [slots, heads, 2], first place and number of parts of a sequence
   // [batch, 2], scores [batch, heads, cache.slots()] (null: weights are not added up)
   float* part;
   float* part_ml;
