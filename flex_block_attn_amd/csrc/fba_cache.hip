@@ -53,24 +53,65 @@ hipError_t launch_cache_append(AppendParams p, hipStream_t stream) {
   return hipGetLastError();
 }
 
-// Eviction, first kernel: which slots of a (sequence, kv head) stay.  A work-group of 1024 threads finds the budget-th largest key, 8 bits at a time by counting,
-// and lists the freed slots below the budget and the kept slots behind it, in order.
+// Eviction, first kernel: which slots of a (sequence, kv head) stay.  A work-group of 1024 threads reads weights and positions once, finds the budget-th largest key by
+// counting (11, 11 and 10 bits of it at a time), and lists the freed slots below the budget and the kept slots behind it, in order.  A wave has consecutive slots, 256 at a
+// time, four to a lane, so that loads are dense, ballots number the slots inside of a wave and one scan over the waves does the rest.  Bound by latency: the loads, and
+// some twenty barriers.
 //
 // A slot's key orders as its weight does (NaN below everything, the two zeros alike); the slots that are held are above all of them.
 namespace {
-constexpr int kSelectThreads = 1024;
+constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 2048;
 FBA_DEVICE uint32_t weight_key(float w) {
   if (w != w) return 0;
   uint32_t bits = __builtin_bit_cast(uint32_t, w);
   if (bits == 0x80000000u) bits = 0;
   return bits & 0x80000000u ? ~bits : bits | 0x80000000u;
 }
+
+// Sum over the waves in front of this one, and over all of them, of a number that a wave's lanes have alike.  `of`: kSelectWaves ints that nobody else uses at the time.
+FBA_DEVICE int waves_before(int x, int* of, int* total) {
+  const int wave = threadIdx.x >> 6;
+  if ((threadIdx.x & 63) == 0) of[wave] = x;
+  __syncthreads();
+  int before = 0, all = 0;
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) {
+    const int n = of[i];
+    before += i < wave ? n : 0;
+    all += n;
+  }
+  *total = all;
+  return before;
+}
+
+// Places of the set ones of 256 slots, four to a lane, in order.
+struct Ranks {
+  int at[4], n;  // set ones in front of each of this lane's four, and of all
+  FBA_DEVICE Ranks(const bool (&on)[4], int lane) {
+    const unsigned long long below = (1ull << lane) - 1;
+    int before = 0, all = 0;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      const unsigned long long ballot = __builtin_amdgcn_ballot_w64(on[e]);
+      before += __builtin_popcountll(ballot & below);
+      all += __builtin_popcountll(ballot);
+    }
+    n = all;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      at[e] = before;
+      before += on[e];
+    }
+  }
+};
 }  // namespace
 
+// kGroups: keys of up to kGroups times 4096 slots stay in registers (kGroups <= 8); 0: any number of slots, read again in every pass.
+template <int kGroups>
 __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const EvictParams p) {
   const CacheView& cache = p.cache;
-  __shared__ int counts[256], wave_sums[3][kSelectThreads / 64], found[2], newest_of[kSelectThreads / 64];
-  const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+  __shared__ int bins[kBins], sums[6][kSelectWaves], found[2];
+  const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hkv = blockIdx.x % cache.kv_heads, b = blockIdx.x / cache.kv_heads;
   int32_t* const moves = p.moves + (int64_t)blockIdx.x * (1 + 2 * (int64_t)p.most);
   const int len = cache.lengths[b];
@@ -83,89 +124,180 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
     if (tid == 0) moves[0] = 0;
     return;
   }
-  auto row_of = [&](int slot) { return cache.row_of(cache.page_of(b, slot), hkv, slot); };
+  typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
+  auto row_of = [&](int slot) { return cache.row_of(cache.page_of(b, slot), hkv, slot); };  // of four slots, which are on one page
+  const int per = (len + 4 * kSelectThreads - 1) / (4 * kSelectThreads);  // groups of 256 slots that a wave has
+  auto slot_of = [&](int j) { return (wave * per + j) * 256 + 4 * lane; };
 
+  // the largest position
   int newest = -0x7fffffff - 1;
-  for (int s = tid; s < len; s += kSelectThreads) newest = max(newest, cache.positions[row_of(s)]);
+  constexpr int kHeld = kGroups > 0 ? kGroups : 1;
+  f32x4 weight[kHeld];
+  i32x4 at[kHeld];
+  if constexpr (kGroups > 0) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+      if (j < per && slot_of(j) < len) {
+        const int64_t row = row_of(slot_of(j));
+        weight[j] = *reinterpret_cast<const f32x4*>(cache.weights + row);
+        at[j] = *reinterpret_cast<const i32x4*>(cache.positions + row);
+      }
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (j < per && slot_of(j) + e < len) newest = max(newest, at[j][e]);
+  } else {
+    for (int s = tid; s < len; s += kSelectThreads) newest = max(newest, cache.positions[row_of(s)]);
+  }
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) newest = max(newest, __shfl_xor(newest, x));
-  if (lane == 0) newest_of[wave] = newest;
+  if (lane == 0) sums[0][wave] = newest;
+  for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
   __syncthreads();
-  for (int i = 0; i < kSelectThreads / 64; ++i) newest = max(newest, newest_of[i]);
-  auto key_of = [&](int slot) -> uint32_t {
-    const int64_t row = row_of(slot);
-    const int at = cache.positions[row];
-    return at < p.sinks || (int64_t)at > (int64_t)newest - p.recent ? 0xffffffffu : weight_key(cache.weights[row]);
+#pragma unroll
+  for (int i = 0; i < kSelectWaves; ++i) newest = max(newest, sums[0][i]);
+  auto key_of = [&](int position, float w) -> uint32_t {
+    return position < p.sinks || (int64_t)position > (int64_t)newest - p.recent ? 0xffffffffu : weight_key(w);
+  };
+  uint32_t key[kHeld][4];
+  if constexpr (kGroups > 0) {
+#pragma unroll
+    for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+      for (int e = 0; e < 4; ++e) key[j][e] = slot_of(j) + e < len ? key_of(at[j][e], weight[j][e]) : 0;
+  }
+  // f(group, this lane's four keys) for the wave's groups, in order.  Slots behind the last one have the lowest key: they are never reached, since more slots are there than stay.
+  auto each = [&](auto f) {
+    if constexpr (kGroups > 0) {
+#pragma unroll
+      for (int j = 0; j < kHeld; ++j)
+        if (j < per && (wave * per + j) * 256 < len) f(j, key[j]);
+    } else {
+      for (int j = 0; j < per && (wave * per + j) * 256 < len; ++j) {
+        uint32_t k[4] = {0, 0, 0, 0};
+        if (slot_of(j) < len) {
+          const int64_t row = row_of(slot_of(j));
+          const f32x4 w = *reinterpret_cast<const f32x4*>(cache.weights + row);
+          const i32x4 q = *reinterpret_cast<const i32x4*>(cache.positions + row);
+#pragma unroll
+          for (int e = 0; e < 4; ++e) k[e] = slot_of(j) + e < len ? key_of(q[e], w[e]) : 0;
+        }
+        f(j, k);
+      }
+    }
   };
 
-  // the key of rank `budget` from above, and how many keys equal to it stay
+  // The key of rank `budget` from above, and how many keys equal to it stay.
   uint32_t prefix = 0;
   int need = p.budget;
-  for (int shift = 24; shift >= 0; shift -= 8) {
-    for (int i = tid; i < 256; i += kSelectThreads) counts[i] = 0;
-    __syncthreads();
-    for (int s = tid; s < len; s += kSelectThreads) {
-      const uint32_t key = key_of(s);
-      if (shift == 24 || key >> (shift + 8) == prefix >> (shift + 8)) atomicAdd(&counts[key >> shift & 255], 1);
-    }
-    __syncthreads();
-    if (wave == 0) {  // from the largest digit down: a lane has four
-      int mine[4], sum = 0;
 #pragma unroll
-      for (int i = 0; i < 4; ++i) sum += mine[i] = counts[255 - 4 * lane - i];
-      int upto = sum;
+  for (int digit = 0; digit < 3; ++digit) {
+    const int shift = digit == 0 ? 21 : digit == 1 ? 10 : 0, width = digit == 2 ? 10 : 11;
+    each([&](int, const uint32_t(&k)[4]) {
 #pragma unroll
-      for (int d = 1; d < 64; d *= 2) {
-        const int other = __shfl_up(upto, d);
-        if (lane >= d) upto += other;
-      }
-      int above = upto - sum;
-#pragma unroll
-      for (int i = 0; i < 4; ++i) {
-        if (above < need && above + mine[i] >= need) {
-          found[0] = 255 - 4 * lane - i;
-          found[1] = need - above;
+      for (int e = 0; e < 4; ++e) {
+        const bool on = digit == 0 || (k[e] >> (shift + width)) == (prefix >> (shift + width));
+        const unsigned long long ballot = __builtin_amdgcn_ballot_w64(on);
+        if (ballot == 0) continue;
+        const int bin = k[e] >> shift & ((1 << width) - 1), some = __builtin_amdgcn_readlane(bin, __builtin_ctzll(ballot));
+        if (__builtin_amdgcn_ballot_w64(on && bin != some) == 0) {  // all in one (slots without a weight, held ones): 64 lanes would wait for each other
+          if (lane == 0) atomicAdd(&bins[some], __builtin_popcountll(ballot));
+        } else if (on) {
+          atomicAdd(&bins[bin], 1);
         }
-        above += mine[i];
       }
+    });
+    __syncthreads();
+    // from the largest digit down: a thread has two
+    const int d0 = kBins - 1 - 2 * tid, n0 = bins[d0], n1 = bins[d0 - 1];
+    int upto = n0 + n1, all;
+#pragma unroll
+    for (int d = 1; d < 64; d *= 2) {
+      const int other = __shfl_up(upto, d);
+      if (lane >= d) upto += other;
+    }
+    const int before = upto - n0 - n1 + waves_before(__builtin_amdgcn_readlane(upto, 63), sums[1 + digit], &all);
+    bins[d0] = 0;
+    bins[d0 - 1] = 0;
+    if (before < need && before + n0 >= need) {
+      found[0] = d0;
+      found[1] = need - before;
+    } else if (before + n0 < need && before + n0 + n1 >= need) {
+      found[0] = d0 - 1;
+      found[1] = need - before - n0;
     }
     __syncthreads();
     prefix |= (uint32_t)found[0] << shift;
     need = found[1];
-    __syncthreads();
+    __syncthreads();  // found is read
   }
 
-  // slots in order, 1024 at a time: equal keys stay while there is need, then freed slots and kept ones are numbered
-  int equal_before = 0, freed_before = 0, late_before = 0;
-  for (int s0 = 0; s0 < len; s0 += kSelectThreads) {
-    const int s = s0 + tid;
-    const uint32_t key = s < len ? key_of(s) : 0;
-    auto rank = [&](bool on, int which, int* total) {  // of the threads with it in front of this one
-      const unsigned long long ballot = __builtin_amdgcn_ballot_w64(on);
-      if (lane == 0) wave_sums[which][wave] = __builtin_popcountll(ballot);
-      __syncthreads();
-      int before = 0, all = 0;
-      for (int i = 0; i < kSelectThreads / 64; ++i) {
-        before += i < wave ? wave_sums[which][i] : 0;
-        all += wave_sums[which][i];
-      }
-      *total = all;
-      return before + __builtin_popcountll(ballot & ((1ull << lane) - 1));
-    };
-    int n_equal, n_freed, n_late;
-    const bool equal = s < len && key == prefix;
-    const int at = rank(equal, 0, &n_equal);
-    const bool kept = s < len && (key > prefix || (equal && equal_before + at < need));
-    const bool freed = s < len && !kept && s < p.budget, late = kept && s >= p.budget;
-    const int at_freed = rank(freed, 1, &n_freed), at_late = rank(late, 2, &n_late);
-    if (freed) moves[1 + freed_before + at_freed] = s;
-    if (late) moves[1 + p.most + late_before + at_late] = s;
-    equal_before += n_equal;
-    freed_before += n_freed;
-    late_before += n_late;
-    __syncthreads();
-  }
-  if (tid == 0) moves[0] = freed_before;  // as many as late_before: budget slots stay
+  // of the keys equal to it the first `need` stay
+  int equal = 0, all;
+  each([&](int, const uint32_t(&k)[4]) {
+#pragma unroll
+    for (int e = 0; e < 4; ++e) equal += __builtin_popcountll(__builtin_amdgcn_ballot_w64(k[e] == prefix));
+  });
+  const int equal_before = waves_before(equal, sums[4], &all);
+  auto staying = [&](const uint32_t(&k)[4], int* equals, bool (&stays)[4]) {  // whether this lane's four stay
+    const bool same[4] = {k[0] == prefix, k[1] == prefix, k[2] == prefix, k[3] == prefix};
+#pragma unroll
+    for (int e = 0; e < 4; ++e) stays[e] = k[e] > prefix;
+    if (__builtin_amdgcn_ballot_w64(same[0] || same[1] || same[2] || same[3]) == 0) return;
+    const Ranks r(same, lane);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) stays[e] = stays[e] || (same[e] && *equals + r.at[e] < need);
+    *equals += r.n;
+  };
+  // Freed ones of slots below the budget, kept ones of those behind it: a group is on either side, or, one of them, on both.
+  int freed = 0, late = 0, equals = equal_before;
+  uint32_t kept = 0;  // four bits for each group
+  each([&](int j, const uint32_t(&k)[4]) {
+    bool stays[4];
+    staying(k, &equals, stays);
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if constexpr (kGroups > 0) kept |= (uint32_t)stays[e] << (4 * j + e);
+      const bool below = slot_of(j) + e < p.budget;
+      freed += __builtin_popcountll(__builtin_amdgcn_ballot_w64(!stays[e] && below));
+      late += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stays[e] && !below));
+    }
+  });
+  int n_freed, n_late;
+  int to = waves_before(freed, sums[5], &n_freed), from = waves_before(late, sums[0], &n_late);
+  equals = equal_before;
+  each([&](int j, const uint32_t(&k)[4]) {
+    bool stays[4];
+    if constexpr (kGroups > 0) {
+#pragma unroll
+      for (int e = 0; e < 4; ++e) stays[e] = kept >> (4 * j + e) & 1;
+    } else {
+      staying(k, &equals, stays);
+    }
+    const int s0 = (wave * per + j) * 256;
+    if (s0 < p.budget) {
+      bool frees[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) frees[e] = !stays[e] && slot_of(j) + e < p.budget;
+      const Ranks r(frees, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (frees[e]) moves[1 + to + r.at[e]] = slot_of(j) + e;
+      to += r.n;
+    }
+    if (s0 + 256 > p.budget) {
+      bool lates[4];
+#pragma unroll
+      for (int e = 0; e < 4; ++e) lates[e] = stays[e] && slot_of(j) + e >= p.budget;
+      const Ranks r(lates, lane);
+#pragma unroll
+      for (int e = 0; e < 4; ++e)
+        if (lates[e]) moves[1 + p.most + from + r.at[e]] = slot_of(j) + e;
+      from += r.n;
+    }
+  });
+  if (tid == 0) moves[0] = n_freed;  // as many as n_late: budget slots stay
 }
 
 // Second kernel: the i-th freed slot gets the i-th kept one from behind the budget, row, position and weight.
@@ -193,7 +325,9 @@ int64_t cache_evict_bytes(EvictParams& p) {
 
 hipError_t launch_cache_evict(EvictParams p, hipStream_t stream) {
   const int items = p.cache.batch * p.cache.kv_heads;
-  hipLaunchKernelGGL(cache_select_kernel, dim3(items), dim3(kSelectThreads), 0, stream, p);
+  const int64_t groups = (p.cache.slots() + 4 * kSelectThreads - 1) / (4 * kSelectThreads);  // for the longest sequence there may be
+  void (*select)(const EvictParams) = groups <= 2 ? &cache_select_kernel<2> : groups <= 8 ? &cache_select_kernel<8> : &cache_select_kernel<0>;
+  hipLaunchKernelGGL(select, dim3(items), dim3(kSelectThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
   if (e != hipSuccess || p.most == 0) return e;
   // about 4096 work-groups, none without a row to move if all are moved
