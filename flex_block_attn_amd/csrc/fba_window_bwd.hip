@@ -130,30 +130,48 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) { pin(qreg[ks]); pin(doreg[ks]); }
 
-      uint32_t into = 0;
-      int owed_slab = 0;
-      // step t (t % 4 == R): S_t, dP_t | dS_t | dQ += K_t^T dS_t.  The copies that a step requests (slab t+4 into the buffer of slab t) are issued by the
-      // following one, between its first matrix instructions.
+      // dS^T of a slab from S^T and dP^T - delta, and what it adds to dQ.  dS is rounded to T as the matrix instruction takes it; the factor 1 / sqrt(128) comes at the end.
+      auto add_dq = [&](LdsPtr pair, const f32x16& s) {
+        x8 ds[2];
+#pragma unroll
+        for (int j = 0; j < 2; ++j) ds[j] = narrow8<T>(s, j);
+#pragma unroll
+        for (int j = 0; j < 2; ++j)
+#pragma unroll
+          for (int mb = 0; mb < 4; ++mb) {
+            const int roff = 16 * j * kRowBytes;
+            acc[mb] = Elem<T>::mfma32(read_tr8<T>(pair + tr.rd[mb][0] + roff, pair + tr.rd[mb][1] + roff), ds[j], acc[mb]);
+          }
+      };
+      auto form_ds = [&](LdsPtr pair, auto between) {
+        f32x16 s, d;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) { s[r] = 0.f; d[r] = neg_delta; }
+#pragma unroll
+        for (int ks = 0; ks < 8; ++ks) {
+          s = Elem<T>::mfma32(read_b128<T>(pair + rm.rd[ks]), qreg[ks], s);
+          d = Elem<T>::mfma32(read_b128<T>(pair + kSlabBytes + rm.rd[ks]), doreg[ks], d);
+          between(ks);
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -lse2)) * d[r];
+        return s;
+      };
+      // Step t (t % 4 == R): S_t, dP_t | dS_t | dQ += K_t^T dS_t.  Slab t+3 is requested into the buffer of slab t-1, between the first matrix instructions; behind the step
+      // slab t+1 must have landed (and has, as slab t+2): what step t requested may still fly.
       auto step = [&](auto ring_c, int t) {
         constexpr int R = decltype(ring_c)::value;
-        const int kind = kind_of(t);
+        const int kind = kind_of(t), slab = slab_at(t + 3);
         const LdsPtr pair = lds + R * kPairBytes;
-        auto owed = [&](int i) {
-          if (i < 2) k_dma.piece(i, into, kp + owed_slab * k_step, owed_slab);
-          else v_dma.piece(i - 2, into + kSlabBytes, vp + owed_slab * v_step, owed_slab);
+        const uint32_t into = dst + ((R + 3) & 3) * kPairBytes;
+        auto request = [&](int i) {
+          if (i < 2) k_dma.piece(i, into, kp + slab * k_step, slab);
+          else v_dma.piece(i - 2, into + kSlabBytes, vp + slab * v_step, slab);
         };
         if (kind != kNone) {
-          f32x16 s, d;
-#pragma unroll
-          for (int r = 0; r < 16; ++r) { s[r] = 0.f; d[r] = neg_delta; }
-#pragma unroll
-          for (int ks = 0; ks < 8; ++ks) {
-            s = Elem<T>::mfma32(read_b128<T>(pair + rm.rd[ks]), qreg[ks], s);
-            d = Elem<T>::mfma32(read_b128<T>(pair + kSlabBytes + rm.rd[ks]), doreg[ks], d);
-            if (ks < 4 && t > 0) owed(ks);
-          }
-#pragma unroll
-          for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -lse2)) * d[r];
+          f32x16 s = form_ds(pair, [&](int ks) {
+            if (ks < 4 && t > 0) request(ks);
+          });
           if (kind == kMasked) {
             const int k0 = slab_of(t) * kSlab + 4 * h, a = lo - k0, z = hi - k0, y = sk - k0;
 #pragma unroll
@@ -162,36 +180,53 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
               s[r] = (e >= a && e <= z) || e < y ? s[r] : 0.f;
             }
           }
-          // dS is rounded to T as the matrix instruction takes it; the factor 1 / sqrt(128) comes at the end
-          x8 ds[2];
-#pragma unroll
-          for (int j = 0; j < 2; ++j) ds[j] = narrow8<T>(s, j);
-#pragma unroll
-          for (int j = 0; j < 2; ++j)
-#pragma unroll
-            for (int mb = 0; mb < 4; ++mb) {
-              const int roff = 16 * j * kRowBytes;
-              acc[mb] = Elem<T>::mfma32(read_tr8<T>(pair + tr.rd[mb][0] + roff, pair + tr.rd[mb][1] + roff), ds[j], acc[mb]);
-            }
+          add_dq(pair, s);
         } else if (t > 0) {
 #pragma unroll
-          for (int i = 0; i < 4; ++i) owed(i);
+          for (int i = 0; i < 4; ++i) request(i);
         }
-        // slab t+1 must have landed, as must slab t+2 one step on: the four copies of slab t+3 may still fly
         wait_vmem<4>();
         __syncthreads();
-        owed_slab = slab_at(t + 4);
-        into = dst + R * kPairBytes;
       };
-      for (int t = 0;; t += 4) {
+      // The same where all rows of the tile see slab t whole and slab t+3 is not the last one.
+      const char *k_src = kp, *v_src = vp;
+      auto whole_step = [&](auto ring_c) {
+        constexpr int R = decltype(ring_c)::value;
+        const LdsPtr pair = lds + R * kPairBytes;
+        const uint32_t into = dst + ((R + 3) & 3) * kPairBytes + k_dma.wave_dst;
+        const f32x16 s = form_ds(pair, [&](int ks) {
+          if (ks == 0) dma16(into, k_src, k_dma.off[0]);
+          if (ks == 1) dma16(into + 4 * kRowBytes, k_src, k_dma.off[1]);
+          if (ks == 2) dma16(into + kSlabBytes, v_src, v_dma.off[0]);
+          if (ks == 3) dma16(into + kSlabBytes + 4 * kRowBytes, v_src, v_dma.off[1]);
+        });
+        add_dq(pair, s);
+        wait_vmem<4>();
+        __syncthreads();
+        k_src += k_step;
+        v_src += v_step;
+      };
+      const int whole_lo = max(0, last_row + shift - p.window + 1), whole_hi = min(len - 1, row0 + shift + ahead);
+      const int from = n_sink + max(0, (whole_lo + kSlab - 1) / kSlab - first);
+      const int to = row0 + kWindowTile <= rows ? n_sink + (whole_hi + 1) / kSlab - first : 0;
+      const int whole_end = min(to, n - 4);  // of the steps that whole_step takes
+      for (int t = 0; t < n;) {
+        if (t > 0 && t >= from && t + 4 <= whole_end) {
+          k_src = kp + slab_of(t + 3) * k_step;
+          v_src = vp + slab_of(t + 3) * v_step;
+          do {
+            whole_step(IC<0>{});
+            whole_step(IC<1>{});
+            whole_step(IC<2>{});
+            whole_step(IC<3>{});
+            t += 4;
+          } while (t + 4 <= whole_end);
+        }
         step(IC<0>{}, t);
-        if (t + 1 >= n) break;
-        step(IC<1>{}, t + 1);
-        if (t + 2 >= n) break;
-        step(IC<2>{}, t + 2);
-        if (t + 3 >= n) break;
-        step(IC<3>{}, t + 3);
-        if (t + 4 >= n) break;
+        if (t + 1 < n) step(IC<1>{}, t + 1);
+        if (t + 2 < n) step(IC<2>{}, t + 2);
+        if (t + 3 < n) step(IC<3>{}, t + 3);
+        t += 4;
       }
       wait_vmem<0>();
       __syncthreads();

@@ -132,25 +132,20 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       for (int ks = 0; ks < 8; ++ks) s = Elem<T>::mfma32(read_b128<T>(slab + rm.rd[ks]), qreg[ks], s);
       return s;
     };
-    int kind = kind_of(0), kind_before = kNone;
     f32x16 s_cur;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_cur[r] = 0.f;
-    if (kind != kNone) s_cur = scores(k_lds);
+    if (kind_of(0) != kNone) s_cur = scores(k_lds);
     pin(s_cur);
     __syncthreads();
-    int owed_k = slab_at(4), owed_v = slab_at(3);  // slabs that the next step requests
-    k_dma.copy(k_dst, kp + owed_k * k_step, owed_k);
 
     x8 p_prev[2];
 #pragma unroll
     for (int j = 0; j < 2; ++j)
 #pragma unroll
       for (int i = 0; i < 8; ++i) p_prev[j][i] = (T)0.f;
-    uint32_t k_into = 0, v_into = 0;
-    bool owed = false;
 
-    // O += P V of the slab in `buf`; the copies that the step owes go between the matrix instructions
+    // O += P V of the slab in `buf`; `between` runs behind the matrix instructions
     auto add_pv = [&](LdsPtr buf, auto between) {
 #pragma unroll
       for (int j = 0; j < 2; ++j)
@@ -161,22 +156,55 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           between(4 * j + mb);
         }
     };
-    // step t (t % 4 == R): O += P_{t-1} V_{t-1} | softmax(S_t) | S_{t+1} = K_{t+1} Q^T
+    auto raise = [&]() {  // the reference, if some row would otherwise see exponents above kLazy
+      float mx = s_cur[0];
+#pragma unroll
+      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
+      if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kLazy) != 0) {
+        const float m_new = fmaxf(m_run, max_halves(mx));
+        const float alpha = fast_exp2((m_run - m_new) * c);
+        m_run = m_new;
+        l_run *= alpha;
+#pragma unroll
+        for (int mb = 0; mb < 4; ++mb)
+#pragma unroll
+          for (int r = 0; r < 16; ++r) acc[mb][r] *= alpha;
+      }
+    };
+    auto weights = [&]() {  // p_prev := P_t
+      const float mc = m_run * c;
+#pragma unroll
+      for (int r = 0; r < 16; ++r) s_cur[r] = fast_exp2(__builtin_fmaf(s_cur[r], c, -mc));
+      const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
+#pragma unroll
+      for (int j = 0; j < 2; ++j) {
+        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one
+        p_prev[j] = narrow8<T>(s_cur, j);
+#pragma unroll
+        for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);
+      }
+      pin(p_prev[0]);
+      pin(p_prev[1]);
+    };
+    // Step t (t % 4 == R): O += P_{t-1} V_{t-1} | softmax(S_t) | S_{t+1} = K_{t+1} Q^T.  P_{t-1} was formed against the reference m of step t-1, so it reaches O before
+    // step t may raise m.  The copies that a step owes, K_{t+4} into the buffer of K_t and V_{t+2} into that of V_{t-2}, go between its first matrix instructions.
+    // Behind it K_{t+2} and V_t must have landed; what steps t-1 and t requested may still fly.
     auto step = [&](auto ring_c, int t) {
       constexpr int R = decltype(ring_c)::value;
-      // P_{t-1} was formed against the reference m of step t-1, so it reaches O before step t may raise m
+      const int kind_before = t > 0 ? kind_of(t - 1) : (int)kNone, kind = kind_of(t), kind_next = kind_of(t + 1);
+      const int k_slab = slab_at(t + 4), v_slab = slab_at(t + 2);
+      const uint32_t k_into = k_dst + R * kSlabBytes, v_into = v_dst + ((R + 2) & 3) * kSlabBytes;
       if (kind_before != kNone) {
         add_pv(v_lds + ((R + 3) & 3) * kSlabBytes, [&](int i) {
-          if (i == 0) k_dma.piece(0, k_into, kp + owed_k * k_step, owed_k);
-          if (i == 2) k_dma.piece(1, k_into, kp + owed_k * k_step, owed_k);
-          if (i == 4) v_dma.piece(0, v_into, vp + owed_v * v_step, owed_v);
-          if (i == 6) v_dma.piece(1, v_into, vp + owed_v * v_step, owed_v);
+          if (i == 0) k_dma.piece(0, k_into, kp + k_slab * k_step, k_slab);
+          if (i == 2) k_dma.piece(1, k_into, kp + k_slab * k_step, k_slab);
+          if (i == 4) v_dma.piece(0, v_into, vp + v_slab * v_step, v_slab);
+          if (i == 6) v_dma.piece(1, v_into, vp + v_slab * v_step, v_slab);
         });
-      } else if (owed) {
-        k_dma.copy(k_into, kp + owed_k * k_step, owed_k);
-        v_dma.copy(v_into, vp + owed_v * v_step, owed_v);
+      } else {
+        k_dma.copy(k_into, kp + k_slab * k_step, k_slab);
+        if (t > 0) v_dma.copy(v_into, vp + v_slab * v_step, v_slab);  // (the first three V slabs are there)
       }
-      const int kind_next = kind_of(t + 1);
       if (kind == kMasked) {
         const int k0 = slab_of(t) * kSlab + 4 * h, a = lo - k0, z = hi - k0, y = sk - k0;
 #pragma unroll
@@ -185,62 +213,58 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           s_cur[r] = (e >= a && e <= z) || e < y ? s_cur[r] : -INFINITY;
         }
       }
-      if (kind != kNone) {
-        // raise the reference if some row would otherwise see exponents above kLazy
-        float mx = s_cur[0];
-#pragma unroll
-        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
-        if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kLazy) != 0) {
-          const float m_new = fmaxf(m_run, max_halves(mx));
-          const float alpha = fast_exp2((m_run - m_new) * c);
-          m_run = m_new;
-          l_run *= alpha;
-#pragma unroll
-          for (int mb = 0; mb < 4; ++mb)
-#pragma unroll
-            for (int r = 0; r < 16; ++r) acc[mb][r] *= alpha;
-        }
-      }
+      if (kind != kNone) raise();
       f32x16 s_nxt = s_cur;
       if (kind_next != kNone) s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
-      if (kind != kNone) {
-        const float mc = m_run * c;
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s_cur[r] = fast_exp2(__builtin_fmaf(s_cur[r], c, -mc));
-        const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
-#pragma unroll
-        for (int j = 0; j < 2; ++j) {
-          // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one
-          p_prev[j] = narrow8<T>(s_cur, j);
-#pragma unroll
-          for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);
-        }
-      }
-      pin(p_prev[0]);
-      pin(p_prev[1]);
+      if (kind != kNone) weights();
       s_cur = s_nxt;
-      kind_before = kind;
-      kind = kind_next;
-      // K_{t+2} and V_t must have landed; the copies requested by steps t-2 and t-1 may still fly
       wait_vmem<8>();
       __syncthreads();
-      // K_{t+5} into the buffer of K_{t+1}, V_{t+3} into that of V_{t-1}
-      owed_k = slab_at(t + 5);
-      owed_v = slab_at(t + 3);
-      k_into = k_dst + ((R + 1) & 3) * kSlabBytes;
-      v_into = v_dst + ((R + 3) & 3) * kSlabBytes;
-      owed = true;
     };
-    for (int t = 0;; t += 4) {
+    // The same where all rows of the tile see slabs t-1, t and t+1 whole, and no slab that is requested is the last one.
+    const char *k_src = kp, *v_src = vp;
+    auto whole_step = [&](auto ring_c) {
+      constexpr int R = decltype(ring_c)::value;
+      const uint32_t k_into = k_dst + R * kSlabBytes, v_into = v_dst + ((R + 2) & 3) * kSlabBytes;
+      add_pv(v_lds + ((R + 3) & 3) * kSlabBytes, [&](int i) {
+        if (i == 0) dma16(k_into + k_dma.wave_dst, k_src, k_dma.off[0]);
+        if (i == 2) dma16(k_into + k_dma.wave_dst + 4 * kRowBytes, k_src, k_dma.off[1]);
+        if (i == 4) dma16(v_into + v_dma.wave_dst, v_src, v_dma.off[0]);
+        if (i == 6) dma16(v_into + v_dma.wave_dst + 4 * kRowBytes, v_src, v_dma.off[1]);
+      });
+      raise();
+      const f32x16 s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
+      weights();
+      s_cur = s_nxt;
+      wait_vmem<8>();
+      __syncthreads();
+      k_src += k_step;
+      v_src += v_step;
+    };
+    // steps [from, to) of the window's slabs that are whole for all rows of the tile
+    const int whole_lo = max(0, last_row + shift - p.window + 1), whole_hi = min(len - 1, row0 + shift + ahead);
+    const int from = n_sink + max(0, (whole_lo + kSlab - 1) / kSlab - first);
+    const int to = row0 + kWindowTile <= rows ? n_sink + (whole_hi + 1) / kSlab - first : 0;
+    const int whole_end = min(to - 1, n - 5);  // of the steps that whole_step takes
+    for (int t = 0; t < n;) {
+      if (t > from && t + 4 <= whole_end) {
+        k_src = kp + slab_of(t + 4) * k_step;
+        v_src = vp + slab_of(t + 2) * v_step;
+        do {
+          whole_step(IC<0>{});
+          whole_step(IC<1>{});
+          whole_step(IC<2>{});
+          whole_step(IC<3>{});
+          t += 4;
+        } while (t + 4 <= whole_end);
+      }
       step(IC<0>{}, t);
-      if (t + 1 >= n) break;
-      step(IC<1>{}, t + 1);
-      if (t + 2 >= n) break;
-      step(IC<2>{}, t + 2);
-      if (t + 3 >= n) break;
-      step(IC<3>{}, t + 3);
-      if (t + 4 >= n) break;
+      if (t + 1 < n) step(IC<1>{}, t + 1);
+      if (t + 2 < n) step(IC<2>{}, t + 2);
+      if (t + 3 < n) step(IC<3>{}, t + 3);
+      t += 4;
     }
+    const int kind_before = kind_of(n - 1);
     if (kind_before != kNone) add_pv(v_lds + ((n - 1) & 3) * kSlabBytes, [](int) {});
     wait_vmem<0>();   // no copy may still be writing LDS
     __syncthreads();  // and everybody is done with the rings
