@@ -16,7 +16,7 @@ import sysconfig
 CSRC = os.path.join(os.path.dirname(os.path.abspath(__file__)), "csrc")
 LIB_NAME = "libfba_gfx950.so"
 LIB_PATH = os.path.join(CSRC, LIB_NAME)
-SOURCES = ["fba_api.hip", "fba_mask_compact.hip", "fba_ssta_mask.hip", "fba_fwd.hip", "fba_bwd_dq.hip", "fba_bwd_dq_ds.hip", "fba_bwd_dkdv.hip", "fba_bwd_dkdv64.hip", "fba_bwd_dkdv_slab.hip", "fba_bwd_mask.hip", "fba_probe.hip", "fba_split.hip", "fba_window_fwd.hip", "fba_window_bwd.hip", "fba_cache.hip", "fba_cache_attend.hip"]
+SOURCES = ["fba_api.hip", "fba_mask_compact.hip", "fba_ssta_mask.hip", "fba_fwd.hip", "fba_bwd_dq.hip", "fba_bwd_dq_ds.hip", "fba_bwd_dkdv.hip", "fba_bwd_dkdv64.hip", "fba_bwd_dkdv_slab.hip", "fba_bwd_mask.hip", "fba_probe.hip", "fba_split.hip", "fba_window_fwd.hip", "fba_window_dq.hip", "fba_window_dkdv.hip", "fba_window_few.hip", "fba_cache.hip", "fba_cache_attend.hip"]
 
 # Per-file extras.  --amdgpu-mfma-vgpr-form keeps MFMA accumulators in ordinary VGPRs, so the softmax arithmetic on
 # them needs no accumulator-register copies; it pays off where the whole working set fits 256 registers.
@@ -27,7 +27,9 @@ EXTRA_FLAGS = {
     "fba_bwd_mask.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
     "fba_bwd_dkdv64.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
     "fba_window_fwd.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
-    "fba_window_bwd.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+    "fba_window_dq.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+    "fba_window_dkdv.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
+    "fba_window_few.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
     "fba_cache_attend.hip": ["-mllvm", "--amdgpu-mfma-vgpr-form"],
 }
 

@@ -940,16 +940,17 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.k, k, "k")) return rc;
   if (int rc = take_strided(p.v, v, "v")) return rc;
   if (int rc = take_strided(p.o, o, "o")) return rc;
-  hipError_t e = fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  const bool few = fba::window_takes_few(p, fba::device_compute_units());
+  hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, false, (hipStream_t)hip_stream) : fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window forward launch");
 }
 
-int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal) {
+int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal) {
   fba::WindowParams p{};
   float stats;
   const int32_t lengths = 0;
-  if (fill_window(p, &stats, has_lengths ? &lengths : nullptr, B, Hkv, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
-  return fba::plan_window_bwd(p);
+  if (fill_window(p, &stats, has_lengths ? &lengths : nullptr, B, Hq, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
+  return fba::plan_window_dkdv(p, fba::device_compute_units());
 }
 
 int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* d_o, float* stats,
@@ -966,12 +967,16 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.dq, dq, "dq")) return rc;
   if (int rc = take_strided(p.dk, dk, "dk")) return rc;
   if (int rc = take_strided(p.dv, dv, "dv")) return rc;
-  const int64_t need = fba::plan_window_bwd(p);
+  if (p.d_o.row != p.q.row) return fail(FBA_ERR_UNSUPPORTED, "q and d_o must have the same row stride");
+  const int64_t need = fba::plan_window_dkdv(p, fba::device_compute_units());
   if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need))
     return fail(FBA_ERR_INVALID, "ws must be 16-byte aligned and hold %lld bytes (fba_window_workspace_bytes), got %lld", (long long)need, (long long)ws_bytes);
   p.parts = (float*)ws;
-  hipError_t e = fba::launch_window_bwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
-  return e == hipSuccess ? FBA_OK : hip_fail(e, "window backward launch");
+  const bool few = fba::window_takes_few(p, fba::device_compute_units());
+  hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, true, (hipStream_t)hip_stream) : fba::launch_window_dq(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  if (e != hipSuccess) return hip_fail(e, "window dq launch");
+  e = fba::launch_window_dkdv(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "window dkdv launch");
 }
 
 }  // extern "C"

@@ -717,11 +717,12 @@ std::pair<at::Tensor, at::Tensor> run_window_forward(const at::Tensor& q, const 
   return {o, stats};
 }
 
-std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
+std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
                                             at::Tensor d_o, const Window& w) {
-  const c10::DeviceGuard guard(q.device());
+  const c10::DeviceGuard guard(given_q.device());
+  at::Tensor q = given_q;
   std::vector<at::Tensor> grads;
-  for (const at::Tensor* t : {&q, &k, &v}) {
+  for (const at::Tensor* t : {&given_q, &k, &v}) {
     grads.push_back(at::empty_like(*t));
     if (!takes_strides(grads.back())) grads.back() = at::empty(t->sizes(), t->options());
   }
@@ -730,8 +731,14 @@ std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tenso
     return grads;
   }
   d_o = d_o.to(q.scalar_type());
-  if (!takes_strides(d_o)) d_o = d_o.clone(at::MemoryFormat::Contiguous);
-  const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
+  // dK and dV take dO with the row stride of q
+  auto same_rows = [](const at::Tensor& a, const at::Tensor& b) { return a.size(2) <= 1 || a.stride(2) == b.stride(2); };
+  if (!takes_strides(d_o) || !same_rows(d_o, q)) d_o = at::empty_like(q).copy_(d_o);
+  if (!takes_strides(d_o) || !same_rows(d_o, q)) {  // a q that repeats rows
+    d_o = d_o.contiguous();
+    q = q.contiguous();
+  }
+  const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
   SplitWorkspace ws(q, bytes);
   const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
                     dv = strided(grads[2]);

@@ -21,21 +21,27 @@ struct WindowParams {
   float* lse;              // [B, Hq, Sq], in log2 units; +inf for a row that sees nothing
   float* neg_delta;        // [B, Hq, Sq], -rowsum(dO o O)
   const int32_t* lengths;  // null, or [B]
-  float* parts;            // fp32 partial sums of dK and dV of key tiles with sinks
+  float* parts;            // fp32 partial sums of dK and dV of key tiles with several items
   int B, Hq, Hkv, Sq, Skv, window, sinks, causal;
   float scale, scale_log2e;  // 1 / sqrt(128), and times log2(e)
   int tiles, items, chunk;   // tiles of a head, work items, consecutive items that one XCD gets together
-  // dK/dV: tiles with sinks of a (batch, kv head), and the parts that the rows outside of the window are cut into (0: there are none)
-  int sink_tiles, sink_parts, sink_items;
+  // dK/dV: keys of a tile; parts that the rows inside of a tile's window are cut into; tiles with sinks of a (batch, kv head), and the parts of the rows outside (0: there are none)
+  int key_tile, band_parts, sink_tiles, sink_parts, sink_items;
 };
 
 constexpr int kWindowTile = 128;
-constexpr int kPartFloats = 2 * kWindowTile * 128;  // dV tile, dK tile
+inline __host__ __device__ int64_t part_floats(const WindowParams& p) { return 2 * 128 * p.key_tile; }  // dV tile, dK tile
 
+// Few query rows: forward, or dQ and neg_delta.  Few key tiles: dK and dV.
+bool window_takes_few(const WindowParams& p, int compute_units);
+bool window_keys_few(const WindowParams& p, int compute_units);
+hipError_t launch_window_few_dkdv(WindowParams p, bool half, hipStream_t stream);
+hipError_t launch_window_few(WindowParams p, bool half, bool backward, hipStream_t stream);
 hipError_t launch_window_fwd(WindowParams p, bool half, hipStream_t stream);
-hipError_t launch_window_bwd(WindowParams p, bool half, hipStream_t stream);
-// Sets sink_tiles and sink_parts; returns the bytes of `parts` that backward needs.
-int64_t plan_window_bwd(WindowParams& p);
+hipError_t launch_window_dq(WindowParams p, bool half, hipStream_t stream);    // before dK and dV: works neg_delta out
+hipError_t launch_window_dkdv(WindowParams p, bool half, hipStream_t stream);  // d_o has q's row stride
+// Decides on key_tile, band_parts, sink_tiles and sink_parts; returns the bytes of `parts` that dK and dV need.
+int64_t plan_window_dkdv(WindowParams& p, int compute_units);
 
 // Work-group id -> item: consecutive items, which read the same keys, go to one XCD `chunk` at a time, so that they meet in its L2, and the XCDs take turns, so
 // that each gets short and long items alike.

@@ -46,7 +46,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
   item /= p.tiles;
   const int hkv = item % p.Hkv, b = item / p.Hkv, hq = hkv * group + g;
 
-  const int len = p.lengths != nullptr ? min(max(p.lengths[b], 0), p.Skv) : p.Skv;
+  const int len = p.lengths != nullptr ? min(max(const_idx(p.lengths)[b], 0), p.Skv) : p.Skv;
   const int rows = p.lengths != nullptr ? len : p.Sq;  // that are not padding
   const int shift = p.lengths != nullptr ? 0 : p.Skv - p.Sq;
   const int row0 = tile * kWindowTile, ahead = p.causal ? 0 : p.window - 1;
@@ -135,7 +135,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     f32x16 s_cur;
 #pragma unroll
     for (int r = 0; r < 16; ++r) s_cur[r] = 0.f;
-    if (kind_of(0) != kNone) s_cur = scores(k_lds);
+    int kind = kind_of(0), kind_before = kNone;  // of the step's slab and the one before
+    if (kind != kNone) s_cur = scores(k_lds);
     pin(s_cur);
     __syncthreads();
 
@@ -191,7 +192,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     // Behind it K_{t+2} and V_t must have landed; what steps t-1 and t requested may still fly.
     auto step = [&](auto ring_c, int t) {
       constexpr int R = decltype(ring_c)::value;
-      const int kind_before = t > 0 ? kind_of(t - 1) : (int)kNone, kind = kind_of(t), kind_next = kind_of(t + 1);
+      const int kind_next = kind_of(t + 1);
       const int k_slab = slab_at(t + 4), v_slab = slab_at(t + 2);
       const uint32_t k_into = k_dst + R * kSlabBytes, v_into = v_dst + ((R + 2) & 3) * kSlabBytes;
       if (kind_before != kNone) {
@@ -218,6 +219,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       if (kind_next != kNone) s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
       if (kind != kNone) weights();
       s_cur = s_nxt;
+      kind_before = kind;
+      kind = kind_next;
       wait_vmem<8>();
       __syncthreads();
     };
@@ -257,6 +260,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           whole_step(IC<3>{});
           t += 4;
         } while (t + 4 <= whole_end);
+        kind_before = kind = kFull;
       }
       step(IC<0>{}, t);
       if (t + 1 < n) step(IC<1>{}, t + 1);
@@ -264,7 +268,6 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       if (t + 3 < n) step(IC<3>{}, t + 3);
       t += 4;
     }
-    const int kind_before = kind_of(n - 1);
     if (kind_before != kNone) add_pv(v_lds + ((n - 1) & 3) * kSlabBytes, [](int) {});
     wait_vmem<0>();   // no copy may still be writing LDS
     __syncthreads();  // and everybody is done with the rings

@@ -381,7 +381,8 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
  * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [2, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first half (+inf
  * for rows without a visible key), backward uses the second.
- * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes, 16-byte aligned, for partial sums of keys with sinks (0 bytes: may be null).
+ * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes on the same GPU, 16-byte aligned, for partial sums of dk and dv (0 bytes: may be null), and d_o with the row
+ * stride of q (FBA_ERR_UNSUPPORTED otherwise).
  * Sq and Skv at most 2^28, B * Hq * Sq and B * Hkv * Skv below 2^29.
  */
 #define FBA_BF16 0
@@ -393,7 +394,7 @@ typedef struct {
 int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, float* stats, const int32_t* lengths, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream);
-int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal);
+int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal);
 int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* d_o, float* stats,
                        const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,

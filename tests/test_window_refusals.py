@@ -40,17 +40,20 @@ def test_c_entry_refuses(change, code, text):
 
 def test_workspace_is_asked_for_and_checked():
     lib = _lib().load()
-    assert lib.fba_window_workspace_bytes(0, 1, 1, 64, 64, 64, 8, 1) == 0  # the window reaches over everything
-    assert lib.fba_window_workspace_bytes(0, 1, 1, 64, 64, 8, 0, 1) == 0   # no sinks
-    n = lib.fba_window_workspace_bytes(0, 2, 3, 1000, 1000, 8, 130, 1)
-    assert n > 0 and n % (2 * 3 * 2 * 2 * 128 * 128 * 4) == 0  # batch, kv heads, tiles with sinks, dV and dK
-    assert lib.fba_window_workspace_bytes(0, 1, 1, 64, 64, 0, 0, 1) == -1
+    assert lib.fba_window_workspace_bytes(0, 1, 1, 1, 64, 64, 64, 8, 1) == 0  # the window reaches over everything
+    assert lib.fba_window_workspace_bytes(0, 1, 1, 1, 64, 64, 8, 0, 1) == 0   # no sinks
+    n = lib.fba_window_workspace_bytes(0, 2, 3, 3, 1000, 1000, 8, 130, 1)
+    assert n > 0 and n % (2 * 3 * 2 * 32 * 128 * 4) == 0  # batch, kv heads, dV and dK, 32 keys
+    assert lib.fba_window_workspace_bytes(0, 1, 1, 1, 64, 64, 0, 0, 1) == -1
     t = ctypes.byref(Strided(0x1000, 1000 * 128, 1000 * 128, 128))
     f = ctypes.c_void_p(0x1000)
     args = (1, 1, 1, 1000, 1000, 128, 8, 4, 1, 0, None)
     assert lib.fba_window_bwd(t, t, t, t, t, f, None, t, t, t, None, 0, *args) == 1
     assert "ws must" in lib.fba_last_error().decode()
     assert lib.fba_window_bwd(t, t, t, t, t, f, None, t, t, t, f, 1000, *args) == 1
+    other = ctypes.byref(Strided(0x1000, 1000 * 256, 1000 * 256, 256))
+    assert lib.fba_window_bwd(t, t, t, t, other, f, None, t, t, t, f, 1 << 40, *args) == 2
+    assert "row stride" in lib.fba_last_error().decode()
 
 
 def test_python_refuses():
