@@ -68,9 +68,9 @@ SIGNATURES = {
     "fba_ssta_mask_3d": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 11 + [_c_ptr]),
     "fba_fwd_tiled": (_c_i32, [_c_ptr] * 7 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),
     "fba_bwd_tiled": (_c_i32, [_c_ptr] * 14 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),
-    "fba_window_fwd": (_c_i32, [_c_ptr] * 6 + [_c_i32] * 10 + [_c_ptr]),
+    "fba_window_fwd": (_c_i32, [_c_ptr] * 7 + [_c_i32] * 10 + [_c_ptr]),
     "fba_window_workspace_bytes": (_c_i64, [_c_i32] * 9),
-    "fba_window_bwd": (_c_i32, [_c_ptr] * 11 + [_c_i64] + [_c_i32] * 10 + [_c_ptr]),
+    "fba_window_bwd": (_c_i32, [_c_ptr] * 12 + [_c_i64] + [_c_i32] * 10 + [_c_ptr]),
     "fba_cache_append": (_c_i32, [_c_ptr] * 6 + [_c_i32] + [_c_ptr] * 2),
     "fba_cache_attn_workspace_bytes": (_c_i64, [_c_ptr] + [_c_i32] * 2),
     "fba_cache_attn": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 5 + [_c_ptr, _c_i64, _c_ptr]),

@@ -931,7 +931,7 @@ int fill_window(fba::WindowParams& p, float* stats, const int32_t* lengths, int3
 
 extern "C" {
 
-int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, float* stats, const int32_t* lengths, int32_t B,
+int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* o_low, float* stats, const int32_t* lengths, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream) {
   fba::WindowParams p{};
@@ -940,6 +940,8 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.k, k, "k")) return rc;
   if (int rc = take_strided(p.v, v, "v")) return rc;
   if (int rc = take_strided(p.o, o, "o")) return rc;
+  if (o_low != nullptr)
+    if (int rc = take_strided(p.o_low, o_low, "o_low")) return rc;
   const bool few = fba::window_takes_few(p, fba::device_compute_units());
   hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, false, (hipStream_t)hip_stream) : fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window forward launch");
@@ -953,7 +955,7 @@ int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hq, i
   return fba::plan_window_dkdv(p, fba::device_compute_units());
 }
 
-int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* d_o, float* stats,
+int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* o_low, const fba_strided* d_o, float* stats,
                        const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream) {
@@ -963,6 +965,8 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.k, k, "k")) return rc;
   if (int rc = take_strided(p.v, v, "v")) return rc;
   if (int rc = take_strided(p.o, o, "o")) return rc;
+  if (o_low != nullptr)
+    if (int rc = take_strided(p.o_low, o_low, "o_low")) return rc;
   if (int rc = take_strided(p.d_o, d_o, "d_o")) return rc;
   if (int rc = take_strided(p.dq, dq, "dq")) return rc;
   if (int rc = take_strided(p.dk, dk, "dk")) return rc;

@@ -700,25 +700,25 @@ struct Window : torch::CustomClassHolder {
 };
 int32_t type_of(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FBA_FP16 : FBA_BF16; }
 
-// -> o, and statistics with room for those of backward
-std::pair<at::Tensor, at::Tensor> run_window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Window& w) {
+// -> o, statistics with room for those of backward and, where backward may come, what rounding o has left
+std::tuple<at::Tensor, at::Tensor, at::Tensor> run_window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Window& w, bool backward) {
   const c10::DeviceGuard guard(q.device());
   at::Tensor o = at::empty_like(q);
   if (!takes_strides(o)) o = at::empty(q.sizes(), q.options());
-  at::Tensor stats = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-  if (q.numel() == 0) return {o, stats};
+  at::Tensor low = backward ? at::empty_like(o) : at::Tensor(), stats = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {o, stats, low};
   if (k.numel() == 0) {  // there is nothing to see
     o.zero_();
-    return {o, stats};
+    return {o, stats, low};
   }
-  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o);
-  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, stats.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
+  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = backward ? strided(low) : so;
+  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, backward ? &sl : nullptr, stats.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
                            w.sinks, w.causal, type_of(q), current_stream(q)));
-  return {o, stats};
+  return {o, stats, low};
 }
 
-std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
-                                            at::Tensor d_o, const Window& w) {
+std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
+                                            const at::Tensor& stats, at::Tensor d_o, const Window& w) {
   const c10::DeviceGuard guard(given_q.device());
   at::Tensor q = given_q;
   std::vector<at::Tensor> grads;
@@ -740,9 +740,9 @@ std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at:
   }
   const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
   SplitWorkspace ws(q, bytes);
-  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
+  const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = strided(low), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
                     dv = strided(grads[2]);
-  check(lib.fba_window_bwd(&sq, &sk, &sv, &so, &sd, stats.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
+  check(lib.fba_window_bwd(&sq, &sk, &sv, &so, &sl, &sd, stats.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
                            q.size(2), k.size(2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
   return grads;
 }
@@ -750,8 +750,8 @@ std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at:
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, c10::intrusive_ptr<Window> w) {
     if (w->lengths.defined()) w->lengths = w->lengths.clone();  // the caller may write to theirs before backward comes
-    auto [o, stats] = run_window_forward(q, k, v, *w);
-    ctx->save_for_backward({q, k, v, o, stats});
+    auto [o, stats, low] = run_window_forward(q, k, v, *w, true);
+    ctx->save_for_backward({q, k, v, o, low, stats});
     ctx->saved_data["w"] = c10::IValue::make_capsule(std::move(w));
     return o;
   }
@@ -760,18 +760,18 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const auto capsule = ctx->saved_data["w"].toCapsule();
     const Window& w = *static_cast<Window*>(capsule.get());
     // What a saved-tensor hook hands back is read by raw pointer.
-    for (int i = 0; i < 5; ++i) {
+    for (int i = 0; i < 6; ++i) {
       const at::Tensor& t = saved[i];
       TORCH_CHECK_VALUE(t.defined() && t.device() == grads[0].device(), "saved tensors must come back on ", grads[0].device());
-      TORCH_CHECK_TYPE(t.scalar_type() == (i < 4 ? saved[0].scalar_type() : at::kFloat) && (i == 4 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
+      TORCH_CHECK_TYPE(t.scalar_type() == (i < 5 ? saved[0].scalar_type() : at::kFloat) && (i == 5 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
                        "saved tensors must come back in their types");
-      TORCH_CHECK_VALUE(i == 4 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
+      TORCH_CHECK_VALUE(i == 5 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
     }
-    TORCH_CHECK_VALUE(saved[0].sizes() == grads[0].sizes() && saved[3].sizes() == grads[0].sizes() && saved[1].sizes() == saved[2].sizes() &&
-                          saved[4].numel() == 2 * saved[0].size(0) * saved[0].size(1) * saved[0].size(2) && saved[1].size(0) == saved[0].size(0) &&
+    TORCH_CHECK_VALUE(saved[0].sizes() == grads[0].sizes() && saved[3].sizes() == grads[0].sizes() && saved[4].sizes() == grads[0].sizes() &&
+                          saved[1].sizes() == saved[2].sizes() && saved[5].numel() == 2 * saved[0].size(0) * saved[0].size(1) * saved[0].size(2) && saved[1].size(0) == saved[0].size(0) &&
                           saved[1].size(1) > 0 == saved[1].numel() > 0 && (saved[1].numel() == 0 || saved[0].size(1) % saved[1].size(1) == 0),
                       "saved tensors must come back in their shapes");
-    const auto g = run_window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], grads[0], w);
+    const auto g = run_window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], grads[0], w);
     return {g[0], g[1], g[2], at::Tensor()};
   }
 };
@@ -811,7 +811,7 @@ c10::optional<at::Tensor> window_attention(pybind11::handle q_, pybind11::handle
                                !w->lengths.is_contiguous() || q.size(2) != k.size(2)))
     return c10::nullopt;
   if (at::GradMode::is_enabled() && (q.requires_grad() || k.requires_grad() || v.requires_grad())) return WindowAttention::apply(q, k, v, std::move(w));
-  return run_window_forward(q, k, v, *w).first;
+  return std::get<0>(run_window_forward(q, k, v, *w, false));
 }
 
 // The two passes for the Python autograd function; arguments have been checked and prepared.
@@ -823,13 +823,13 @@ Window window_of(int64_t window, int64_t sinks, bool causal, const c10::optional
   if (lengths) w.lengths = *lengths;
   return w;
 }
-std::pair<at::Tensor, at::Tensor> window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks, bool causal,
-                                                 const c10::optional<at::Tensor>& lengths) {
-  return run_window_forward(q, k, v, window_of(window, sinks, causal, lengths));
+std::tuple<at::Tensor, at::Tensor, at::Tensor> window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, int64_t window, int64_t sinks,
+                                                              bool causal, const c10::optional<at::Tensor>& lengths) {
+  return run_window_forward(q, k, v, window_of(window, sinks, causal, lengths), true);
 }
-std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& stats,
-                                        const at::Tensor& d_o, int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
-  return run_window_backward(q, k, v, o, stats, d_o, window_of(window, sinks, causal, lengths));
+std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
+                                        const at::Tensor& stats, const at::Tensor& d_o, int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
+  return run_window_backward(q, k, v, o, low, stats, d_o, window_of(window, sinks, causal, lengths));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

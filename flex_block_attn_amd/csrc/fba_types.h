@@ -88,16 +88,19 @@ struct RowDma {
   }
 };
 
-// store_tile_bf16 by type, to rows `stride` bytes apart; `rows` of the 32 are stored.
-template <typename T>
+// store_tile_bf16 by type, to rows `stride` bytes apart; `rows` of the 32 are stored.  kLow: what rounding leaves, rounded, instead.
+template <typename T, bool kLow = false>
 FBA_DEVICE void store_tile(char* buf, const f32x16 (&acc)[4], float scale, char* out, uint32_t stride, int lane, int rows) {
   const int l32 = lane & 31, h = lane >> 5;
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
-    for (int g = 0; g < 4; ++g)
-      *reinterpret_cast<x4_of<T>*>(buf + tile_off(l32, 4 * mb + g) + 8 * h) =
-          narrow4<T>(acc[mb][4 * g + 0] * scale, acc[mb][4 * g + 1] * scale, acc[mb][4 * g + 2] * scale, acc[mb][4 * g + 3] * scale);
+    for (int g = 0; g < 4; ++g) {
+      const float v[4] = {acc[mb][4 * g + 0] * scale, acc[mb][4 * g + 1] * scale, acc[mb][4 * g + 2] * scale, acc[mb][4 * g + 3] * scale};
+      x4_of<T> value = narrow4<T>(v[0], v[1], v[2], v[3]);
+      if constexpr (kLow) value = narrow4<T>(v[0] - (float)value[0], v[1] - (float)value[1], v[2] - (float)value[2], v[3] - (float)value[3]);
+      *reinterpret_cast<x4_of<T>*>(buf + tile_off(l32, 4 * mb + g) + 8 * h) = value;
+    }
 #pragma unroll
   for (int i = 0; i < 8; ++i) {
     const int row = 4 * i + (lane >> 4);

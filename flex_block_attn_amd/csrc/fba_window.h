@@ -18,6 +18,7 @@ struct Strided {  // a (batch, heads, rows, 128) tensor of 16-bit values; stride
 
 struct WindowParams {
   Strided q, k, v, o, d_o, dq, dk, dv;
+  Strided o_low;           // what rounding o has left; ptr null: not wanted
   float* lse;              // [B, Hq, Sq], in log2 units; +inf for a row that sees nothing
   float* neg_delta;        // [B, Hq, Sq], -rowsum(dO o O)
   const int32_t* lengths;  // null, or [B]

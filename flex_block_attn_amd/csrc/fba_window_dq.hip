@@ -86,6 +86,9 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     const char* const qp = p.q.ptr + b * p.q.batch + hq * p.q.head + (int64_t)from * p.q.row + 16 * h;
     const char* const dp = p.d_o.ptr + b * p.d_o.batch + hq * p.d_o.head + (int64_t)from * p.d_o.row + 16 * h;
     const char* const op = p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)from * p.o.row + 16 * h;
+    // delta: with what rounding o has left, where that is there (a row's error in it goes into all of its dS)
+    const char* const lp = p.o_low.ptr == nullptr ? op : p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)from * p.o_low.row + 16 * h;
+    const float low = p.o_low.ptr == nullptr ? 0.f : 1.f;
     const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Sq + from;
     float lse2 = p.lse[stat];
     float sum = 0.f;
@@ -93,9 +96,9 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     for (int ks = 0; ks < 8; ++ks) {
       qreg[ks] = *reinterpret_cast<const x8*>(qp + 32 * ks);
       doreg[ks] = *reinterpret_cast<const x8*>(dp + 32 * ks);
-      const x8 o8 = *reinterpret_cast<const x8*>(op + 32 * ks);
+      const x8 o8 = *reinterpret_cast<const x8*>(op + 32 * ks), l8 = *reinterpret_cast<const x8*>(lp + 32 * ks);
 #pragma unroll
-      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)doreg[ks][i], (float)o8[i], sum);
+      for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)doreg[ks][i], __builtin_fmaf(low, (float)l8[i], (float)o8[i]), sum);
     }
     const float neg_delta = -sum_halves(sum);
     if (h == 0 && there) p.neg_delta[stat] = neg_delta;

@@ -100,15 +100,17 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
     if constexpr (kBackward) {
       const char* const dp = p.d_o.ptr + b * p.d_o.batch + hq * p.d_o.head + (int64_t)from * p.d_o.row + 16 * h;
       const char* const op = p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)from * p.o.row + 16 * h;
+      const char* const lp = p.o_low.ptr == nullptr ? op : p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)from * p.o_low.row + 16 * h;
+      const float low = p.o_low.ptr == nullptr ? 0.f : 1.f;
       const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Sq + from;
       lse2 = p.lse[stat];
       float sum = 0.f;
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
         doreg[ks] = *reinterpret_cast<const x8*>(dp + 32 * ks);
-        const x8 o8 = *reinterpret_cast<const x8*>(op + 32 * ks);
+        const x8 o8 = *reinterpret_cast<const x8*>(op + 32 * ks), l8 = *reinterpret_cast<const x8*>(lp + 32 * ks);
 #pragma unroll
-        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)doreg[ks][i], (float)o8[i], sum);
+        for (int i = 0; i < 8; ++i) sum = __builtin_fmaf((float)doreg[ks][i], __builtin_fmaf(low, (float)l8[i], (float)o8[i]), sum);
       }
       neg_delta = -sum_halves(sum);
       if (wave == 0 && h == 0 && there) p.neg_delta[stat] = neg_delta;
@@ -242,7 +244,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
     f32x4 sum = {0.f, 0.f, 0.f, 0.f};
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) sum += factor[w] * *reinterpret_cast<const f32x4*>(smem + w * 2 * kSlabBytes + r * 512 + ((chunk ^ r) << 4));
-    *reinterpret_cast<x4_of<T>*>(to + chunk * 8) = narrow4<T>(sum[0] * scale, sum[1] * scale, sum[2] * scale, sum[3] * scale);
+    sum *= scale;
+    const x4_of<T> value = narrow4<T>(sum[0], sum[1], sum[2], sum[3]);
+    *reinterpret_cast<x4_of<T>*>(to + chunk * 8) = value;
+    if (!kBackward && p.o_low.ptr != nullptr)
+      *reinterpret_cast<x4_of<T>*>(p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)(row0 + r) * p.o_low.row + chunk * 8) =
+          narrow4<T>(sum[0] - (float)value[0], sum[1] - (float)value[1], sum[2] - (float)value[2], sum[3] - (float)value[3]);
   }
 }
 

@@ -275,8 +275,10 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 
   const float l = sum_halves(l_run);
   if (h == 0 && row < p.Sq) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l > 0.f ? m_run * c + __builtin_log2f(l) : INFINITY;
-  store_tile<T>(smem + wave * kSlabBytes, acc, l > 0.f ? 1.f / l : 0.f, p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)wrow0 * p.o.row, p.o.row, lane,
-                p.Sq - wrow0);
+  const float scale = l > 0.f ? 1.f / l : 0.f;
+  store_tile<T>(smem + wave * kSlabBytes, acc, scale, p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)wrow0 * p.o.row, p.o.row, lane, p.Sq - wrow0);
+  if (p.o_low.ptr != nullptr)  // for backward
+    store_tile<T, true>(smem + wave * kSlabBytes, acc, scale, p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)wrow0 * p.o_low.row, p.o_low.row, lane, p.Sq - wrow0);
 }
 
 hipError_t launch_window_fwd(WindowParams p, bool half, hipStream_t stream) {

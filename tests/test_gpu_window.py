@@ -298,10 +298,10 @@ def test_writes_nothing_beside_its_outputs(gpu):
     stats = torch.full((2 * B * H * S + 64,), 7.0, device=gpu)
     of = lambda t: ctypes.byref(Strided(t.data_ptr(), *t.stride()[:3]))
     sizes = (B, H, Hk, S, S, 128, 40, 5, 1, 0)
-    _lib.call("fba_window_fwd", of(q), of(k), of(v), of(inner[0]), ctypes.c_void_p(stats.data_ptr()), None, *sizes, _stream())
+    _lib.call("fba_window_fwd", of(q), of(k), of(v), of(inner[0]), None, ctypes.c_void_p(stats.data_ptr()), None, *sizes, _stream())
     n = _lib.load().fba_window_workspace_bytes(0, B, H, Hk, S, S, 40, 5, 1)
     ws = torch.full((n + 64,), 7, dtype=torch.uint8, device=gpu)
-    _lib.call("fba_window_bwd", of(q), of(k), of(v), of(inner[0]), of(do), ctypes.c_void_p(stats.data_ptr()), None, of(inner[1]), of(inner[2]), of(inner[3]),
+    _lib.call("fba_window_bwd", of(q), of(k), of(v), of(inner[0]), None, of(do), ctypes.c_void_p(stats.data_ptr()), None, of(inner[1]), of(inner[2]), of(inner[3]),
               ctypes.c_void_p(ws.data_ptr()), n, *sizes, _stream())
     want, off = reference(q, k, v, do, 40, 5, True, None)
     for t, x, y, z in zip(around, inner, want, off):

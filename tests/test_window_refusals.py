@@ -21,7 +21,7 @@ GOOD = dict(B=1, Hq=2, Hkv=1, Sq=64, Skv=64, D=128, window=8, sinks=1, causal=1,
 def _fwd(q=(0x1000, 128 * 64 * 2, 128 * 64, 128), lengths=None, stats=0x1000, **change):
     a = dict(GOOD, **change)
     t = [ctypes.byref(Strided(*x)) if x is not None else None for x in (q, *[(0x1000, 8192, 8192, 128)] * 3)]
-    return _lib().load().fba_window_fwd(*t, ctypes.c_void_p(stats), ctypes.c_void_p(lengths), a["B"], a["Hq"], a["Hkv"], a["Sq"], a["Skv"], a["D"], a["window"], a["sinks"],
+    return _lib().load().fba_window_fwd(*t, None, ctypes.c_void_p(stats), ctypes.c_void_p(lengths), a["B"], a["Hq"], a["Hkv"], a["Sq"], a["Skv"], a["D"], a["window"], a["sinks"],
                                         a["causal"], a["type"], None)
 
 
@@ -48,11 +48,11 @@ def test_workspace_is_asked_for_and_checked():
     t = ctypes.byref(Strided(0x1000, 1000 * 128, 1000 * 128, 128))
     f = ctypes.c_void_p(0x1000)
     args = (1, 1, 1, 1000, 1000, 128, 8, 4, 1, 0, None)
-    assert lib.fba_window_bwd(t, t, t, t, t, f, None, t, t, t, None, 0, *args) == 1
+    assert lib.fba_window_bwd(t, t, t, t, None, t, f, None, t, t, t, None, 0, *args) == 1
     assert "ws must" in lib.fba_last_error().decode()
-    assert lib.fba_window_bwd(t, t, t, t, t, f, None, t, t, t, f, 1000, *args) == 1
+    assert lib.fba_window_bwd(t, t, t, t, None, t, f, None, t, t, t, f, 1000, *args) == 1
     other = ctypes.byref(Strided(0x1000, 1000 * 256, 1000 * 256, 256))
-    assert lib.fba_window_bwd(t, t, t, t, other, f, None, t, t, t, f, 1 << 40, *args) == 2
+    assert lib.fba_window_bwd(t, t, t, t, None, other, f, None, t, t, t, f, 1 << 40, *args) == 2
     assert "row stride" in lib.fba_last_error().decode()
 
 
