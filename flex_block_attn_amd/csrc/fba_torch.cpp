@@ -20,6 +20,8 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
+#include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/custom_class.h>
@@ -717,9 +719,45 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> run_window_forward(const at::Tens
   return {o, stats, low};
 }
 
+// What a saved-tensor hook hands back is read by raw pointer.
+void check_window_saved(std::initializer_list<at::Tensor> tensors, const at::Tensor& d_o, const Window& w) {
+  const at::Tensor *saved = tensors.begin(), &q = saved[0], &k = saved[1];
+  for (int i = 0; i < 6; ++i) {
+    const at::Tensor& t = saved[i];
+    TORCH_CHECK_VALUE(t.defined() && t.device() == d_o.device(), "saved tensors must come back on ", d_o.device());
+    TORCH_CHECK_TYPE(i == 5 ? t.scalar_type() == at::kFloat : t.scalar_type() == q.scalar_type() && (t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
+                     "saved tensors must come back in their types");
+    TORCH_CHECK_VALUE(i == 5 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
+  }
+  TORCH_CHECK_VALUE(q.sizes() == d_o.sizes() && saved[3].sizes() == d_o.sizes() && saved[4].sizes() == d_o.sizes() && k.sizes() == saved[2].sizes() &&
+                        saved[5].numel() == 2 * q.size(0) * q.size(1) * q.size(2) && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+                        (!w.lengths.defined() || (w.lengths.size(0) == q.size(0) && q.size(2) == k.size(2))),
+                    "saved tensors must come back in their shapes");
+}
+
+// A leaf's place in autograd's graph keeps the stream on which it was first used for as long as a graph with it lives.  While backward is captured, autograd would make
+// that stream, which has no part in the capture, wait for the capturing one: that breaks the capture and ends the process.
+void refuse_foreign_leaves(const at::Tensor& q) {
+  const auto node = torch::autograd::get_current_node();
+  if (!node) return;
+  const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(q.device().index());
+  bool foreign = false;
+  for (const torch::autograd::Edge& edge : node->next_edges())
+    if (edge.function != nullptr && dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) != nullptr) {
+      const auto stream = edge.function->stream();
+      foreign = foreign || (stream.has_value() && (stream->device_index() != here.device_index() || stream->id() != here.id()));
+    }
+  if (!foreign) return;
+  pybind11::gil_scoped_acquire gil;
+  const bool capturing = pybind11::module_::import("torch").attr("cuda").attr("is_current_stream_capturing")().cast<bool>();
+  TORCH_CHECK(!capturing, "backward is captured on another stream than that of an earlier graph of the same leaves: drop what holds that graph before the capture");
+}
+
 std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
                                             const at::Tensor& stats, at::Tensor d_o, const Window& w) {
+  check_window_saved({given_q, k, v, o, low, stats}, d_o, w);
   const c10::DeviceGuard guard(given_q.device());
+  refuse_foreign_leaves(given_q);
   at::Tensor q = given_q;
   std::vector<at::Tensor> grads;
   for (const at::Tensor* t : {&given_q, &k, &v}) {
@@ -759,18 +797,6 @@ struct WindowAttention : torch::autograd::Function<WindowAttention> {
     const auto saved = ctx->get_saved_variables();
     const auto capsule = ctx->saved_data["w"].toCapsule();
     const Window& w = *static_cast<Window*>(capsule.get());
-    // What a saved-tensor hook hands back is read by raw pointer.
-    for (int i = 0; i < 6; ++i) {
-      const at::Tensor& t = saved[i];
-      TORCH_CHECK_VALUE(t.defined() && t.device() == grads[0].device(), "saved tensors must come back on ", grads[0].device());
-      TORCH_CHECK_TYPE(t.scalar_type() == (i < 5 ? saved[0].scalar_type() : at::kFloat) && (i == 5 || t.scalar_type() == at::kHalf || t.scalar_type() == at::kBFloat16),
-                       "saved tensors must come back in their types");
-      TORCH_CHECK_VALUE(i == 5 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
-    }
-    TORCH_CHECK_VALUE(saved[0].sizes() == grads[0].sizes() && saved[3].sizes() == grads[0].sizes() && saved[4].sizes() == grads[0].sizes() &&
-                          saved[1].sizes() == saved[2].sizes() && saved[5].numel() == 2 * saved[0].size(0) * saved[0].size(1) * saved[0].size(2) && saved[1].size(0) == saved[0].size(0) &&
-                          saved[1].size(1) > 0 == saved[1].numel() > 0 && (saved[1].numel() == 0 || saved[0].size(1) % saved[1].size(1) == 0),
-                      "saved tensors must come back in their shapes");
     const auto g = run_window_backward(saved[0], saved[1], saved[2], saved[3], saved[4], saved[5], grads[0], w);
     return {g[0], g[1], g[2], at::Tensor()};
   }

@@ -271,10 +271,10 @@ __global__ __launch_bounds__(256) void window_sum_kernel(const WindowParams p) {
   *reinterpret_cast<x4_of<T>*>(out.ptr + b * out.batch + hkv * out.head + (int64_t)key * out.row + c4 * 2) = narrow4<T>(acc[0] * s, acc[1] * s, acc[2] * s, acc[3] * s);
 }
 
-// How the rows of a key tile are cut into items.  Two work-groups are on a compute unit at a time.
-//   Inside of the window: into several where the tiles alone leave half of the compute units idle and more, so that all places are taken, with 16 slabs to an item at least.
-//   dQ, dK and dV, one item / several: B2 H8/2 S3136 window 384 (100 tiles) 118 / 100 us; B1 H8 S4096 window 1024, where there are 256 tiles, 121 / 133.
-//   Outside (tiles with sinks): into as many as are about as long as the items inside, for the longest sequence there may be.
+// How the rows of a key tile are cut into items.
+//   Inside of the window: into several where there are so few tiles (of 32 keys then) that half of the compute units and more would idle, so that two items come to each, with
+//   8 slabs to an item at least.  dQ, dK and dV, one item / several, H4/1 S2048 window 1024 (64 tiles): 95 / 56 us, H8/2 S1024 window 512: 67 / 47, B2 H8/1 S1024, 400 to either side: 136 / 70.
+//   Outside (tiles with sinks): into as many as are about as long as the items inside, for the longest sequence there may be, of 16 slabs (tiles of 32 keys: 8) at least.
 constexpr int kLeastSlabs = 16, kLeastSlabsFew = 8;
 int64_t plan_window_dkdv(WindowParams& p, int compute_units) {
   p.key_tile = window_keys_few(p, compute_units) ? 32 : kWindowTile;

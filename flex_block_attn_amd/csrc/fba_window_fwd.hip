@@ -179,7 +179,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one
+        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one (lse, of
+        // that sum, is off by half a step of T at most for it, and P of backward with it; P is rounded by as much again there)
         p_prev[j] = narrow8<T>(s_cur, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);

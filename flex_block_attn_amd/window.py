@@ -1,6 +1,6 @@
 """Attention under a sliding window with sinks, at the granularity of tokens: what a block mask (`masks.swa_block_mask`, the sliding tiles and sink blocks of
-`video`) cannot say, a border inside a block, and causality.  The kernels are csrc/fba_window_fwd.hip and csrc/fba_window_bwd.hip; what they compute is stated
-in include/fba.h."""
+`video`) cannot say, a border inside a block, and causality.  The kernels are csrc/fba_window_fwd.hip, fba_window_dq.hip, fba_window_dkdv.hip and, for small
+calls, fba_window_few.hip; what they compute is stated in include/fba.h."""
 import numbers
 
 import torch
@@ -89,7 +89,10 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     i + kv_seq_len - q_seq_len.  `window` None: no limit.  `lengths`, int32 (batch,) on the GPU: sequence b has lengths[b] tokens, the rows behind them are
     padding (not read, zeros in o and in the gradients); q and k then have one length.  A row that sees no key is zeros.
 
-    Returns o, shaped like q.  Differentiable in q, k and v, once.  Gradients in fp16 need the usual scaling of the loss."""
+    Scores of keys that a row does not see may be anything; v has to be finite there (a weight of zero times infinity is no number), padding excepted.
+
+    Returns o, shaped like q.  Differentiable in q, k and v, once.  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
+    graph of the same leaves may be alive then (backward raises)."""
     o = _lib.host().window_attention(q, k, v, window, sinks, bool(causal), lengths)
     if o is not None:
         return o

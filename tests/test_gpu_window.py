@@ -3,9 +3,12 @@
 Tolerances.  u = eps / 2 of the type: what one rounding is off by.  e: what P is off by, relatively, from fp32 sums: 128 products added in fp32, 130 * 2^-24 of
 the sum of their sizes at most, and a few 2^-24 for exp2 and the denominator.
   o   P is rounded once (and its sum with it, u each) and o once:            (2u + 2e) P|v| + u|o|
-  dv  P and dv are rounded:                                                  (u + 2e) P^T|do| + u|dv|
-  ds  rounded once; delta comes from the rounded o, dP from fp32 sums:       (u + 2e) |ds| + P (|do| E_o + 260 * 2^-24 |do||v|)
+  dv  P and dv are rounded:                                                  (2u + 2e) P^T|do| + u|dv|
+  ds  rounded once; delta comes from the rounded o, dP from fp32 sums:       (2u + 2e) |ds| + P (|do| E_o + 260 * 2^-24 |do||v|)
   dq, dk  the sum of that and a rounding.
+P of backward is exp2(S - lse), and lse is that of the rounded P's sum, whose rounding errors are u of it together at most, with one P that decides it: P is off by u before it
+is rounded (once: 2u), or what it makes is.  What is rounded has its own error E by then: a rounding of x + E is off by u (|x| + E) at most, not by u |x|.  Likewise two factors
+of 1 + u, and (1 + u) / (1 - u), are off from 1 by 2u + 4u^2 at most.
 """
 import math
 
@@ -49,18 +52,19 @@ def reference(q, k, v, do, window, sinks, causal, lengths):
             p = torch.softmax(s, -1).nan_to_num(0.0) if n else s
             e = 130 * f * (torch.where(seen, qd.abs() @ kd.abs().T, torch.zeros_like(s)).max().item() if s.numel() else 0.0) * SCALE + 16 * f
             o = p @ vd
-            eo = (2 * u + 2 * e) * (p @ vd.abs()) + u * o.abs()
+            eo = (2 * u + 4 * u * u + 2 * e) * (p @ vd.abs())
+            eo = eo + u * (o.abs() + eo)
             delta = (o * dod).sum(-1, keepdim=True)
             ds = p * (dod @ vd.T - delta)
-            eds = (u + 2 * e) * ds.abs() + p * ((eo * dod.abs()).sum(-1, keepdim=True) + 260 * f * (dod.abs() @ vd.abs().T))
+            eds = (2 * u + 4 * u * u + 2 * e) * ds.abs() + p * ((eo * dod.abs()).sum(-1, keepdim=True) + 260 * f * (dod.abs() @ vd.abs().T))
             out[0][b, h, :r], off[0][b, h, :r] = o, eo
             out[1][b, h, :r], off[1][b, h, :r] = ds @ kd * SCALE, eds @ kd.abs() * SCALE
             out[2][b, h // G, :n] += ds.T @ qd * SCALE
             off[2][b, h // G, :n] += eds.T @ qd.abs() * SCALE
             out[3][b, h // G, :n] += p.T @ dod
-            off[3][b, h // G, :n] += (u + 2 * e) * (p.T @ dod.abs())
+            off[3][b, h // G, :n] += (2 * u + 4 * u * u + 2 * e) * (p.T @ dod.abs())
     for x, y in list(zip(out, off))[1:]:
-        y += u * x.abs()
+        y += u * (x.abs() + y)
     return out, [y + torch.finfo(q.dtype).smallest_normal for y in off]  # (below that fp16 has fixed steps)
 
 
@@ -309,3 +313,106 @@ def test_writes_nothing_beside_its_outputs(gpu):
         x.fill_(7.0)
         assert bool((t == 7.0).all())
     assert bool((stats[-64:] == 7.0).all()) and bool((ws[n:] == 7).all())
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("B,H,Hk,Sq,Skv,window,sinks", [
+    (3, 48, 48, 70, 70, 20, 4), (2, 36, 36, 257, 257, 31, 128), (1, 48, 48, 400, 400, 100, 130), (1, 27, 27, 640, 640, 33, 4), (2, 24, 24, 300, 411, None, 0), (2, 48, 48, 300, 120, 40, 4),
+    (1, 44, 44, 513, 513, 512, 600), (150, 1, 1, 33, 33, 7, 2), (2, 96, 24, 130, 130, 64, 9), (1, 64, 8, 1100, 1100, 129, 31), (1, 24, 24, 777, 777, 1, 97),
+])
+def test_many_rows_and_keys(gpu, dtype, causal, B, H, Hk, Sq, Skv, window, sinks):
+    """More than 128 tiles of 128 rows: tiles of 128, and from 128 tiles of keys on, there too.  (What comes before has tiles of 32 rows and keys.)"""
+    check(gpu, *inputs(gpu, B, H, Hk, Sq, Skv, dtype, Sq + H), window, sinks, causal)
+
+
+@pytest.mark.parametrize("causal", [True, False])
+@pytest.mark.parametrize("window,sinks", [(60, 4), (200, 140), (None, 0), (1, 31)])
+def test_many_rows_and_keys_in_padded_batches(gpu, causal, window, sinks):
+    S, lengths = 415, torch.tensor([415, 0, 1, 32, 129, 300, 1000, -3, 257], dtype=torch.int32, device=gpu)
+    q, k, v, do = inputs(gpu, len(lengths), 8, 4, S, S, torch.bfloat16, 5)
+    for b, n in enumerate(lengths.tolist()):
+        for t in (q, k, v, do):
+            t[b, :, max(0, n):] = math.nan
+    got = check(gpu, q, k, v, do, window, sinks, causal, lengths)
+    for x in got:
+        for b, n in enumerate(lengths.tolist()):
+            assert int(x[b, :, max(0, n):].count_nonzero()) == 0
+
+
+@pytest.mark.parametrize("B,H,Hk,S,window,sinks,causal", [(1, 4, 1, 2048, 1024, 0, True), (1, 8, 2, 1024, 512, 40, True), (2, 8, 1, 700, 300, 5, False), (1, 1, 1, 1536, 700, 64, False)])
+def test_few_keys_with_many_rows_each(gpu, B, H, Hk, S, window, sinks, causal):
+    """A tile's rows are cut into several items."""
+    check(gpu, *inputs(gpu, B, H, Hk, S, S, torch.bfloat16, S), window, sinks, causal)
+
+
+def test_many_rows_in_other_layouts(gpu):
+    """As contiguous copies, bit for bit, where tiles have 128 rows."""
+    import flex_block_attn_amd as fba
+
+    g = torch.Generator(device="cpu").manual_seed(3)
+    packed = torch.randn((2, 300, 3, 48, 128), generator=g).to(torch.bfloat16).to(gpu)
+    a, b, c = (packed[:, :, i].transpose(1, 2) for i in range(3))
+    do = torch.randn((2, 300, 48, 128), generator=g).to(torch.bfloat16).to(gpu).transpose(1, 2)
+    results = []
+    for prepare in (lambda t: t, lambda t: t.contiguous()):
+        leaves = [prepare(t).detach().requires_grad_(True) for t in (a, b, c)]
+        o = fba.window_attn_func(*leaves, 70, sinks=9)
+        results.append((o.detach(), *torch.autograd.grad(o, leaves, prepare(do))))
+    for x, y in zip(*results):
+        assert torch.equal(x, y)
+
+
+def _both_paths():
+    import flex_block_attn_amd as fba
+
+    return fba.window_attn_func, lambda q, k, v, window, sinks: fba.WindowAttnFunc.apply(q, k, v, window, sinks, True, None)
+
+
+def test_saved_tensors_that_come_back_changed(gpu):
+    """From the host and back is the same step; what comes back in another type, shape or place is refused before a kernel reads it."""
+    q, k, v, do = inputs(gpu, 1, 4, 2, 100, 100, torch.bfloat16, 3)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for f in _both_paths():
+        want = torch.autograd.grad(f(*leaves, 30, sinks=3), leaves, do)
+        with torch.autograd.graph.save_on_cpu():
+            o = f(*leaves, 30, sinks=3)
+        for x, y in zip(torch.autograd.grad(o, leaves, do), want):
+            assert torch.equal(x, y)
+        for change, error in ((lambda t: t.cpu(), ValueError), (lambda t: t.double(), TypeError), (lambda t: t[:, :, :50].contiguous(), ValueError), (lambda t: t[..., :64], ValueError)):
+            with torch.autograd.graph.saved_tensors_hooks(lambda t: t, change):
+                o = f(*leaves, 30, sinks=3)
+            with pytest.raises((error, RuntimeError)):
+                torch.autograd.grad(o, leaves, do)
+        o = f(*leaves, 30, sinks=3)
+        with torch.no_grad():
+            k.add_(1)
+        with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+            torch.autograd.grad(o, leaves, do)
+
+
+def test_capture_beside_an_earlier_graph_of_the_same_leaves(gpu):
+    """Refused by backward, before autograd would make the leaves' stream part of the capture; once the earlier graph is gone the step can be captured."""
+    q, k, v, do = inputs(gpu, 1, 4, 2, 100, 100, torch.bfloat16, 3)
+    leaves = [t.requires_grad_(True) for t in (q, k, v)]
+    for f in _both_paths():
+        earlier = f(*leaves, 30, sinks=3)
+        want = (earlier.detach().clone(), *torch.autograd.grad(earlier, leaves, do, retain_graph=True))
+        torch.cuda.synchronize()
+        with pytest.raises(RuntimeError, match="earlier graph"):
+            with torch.cuda.graph(torch.cuda.CUDAGraph()):
+                torch.autograd.grad(f(*leaves, 30, sinks=3), leaves, do)
+        for x, y in zip(torch.autograd.grad(earlier, leaves, do), want[1:]):
+            assert torch.equal(x, y)
+        del earlier
+        graph = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(graph):
+            o = f(*leaves, 30, sinks=3)
+            out = (o.detach(), *torch.autograd.grad(o, leaves, do))
+        del o
+        for x in out:
+            x.fill_(math.nan)
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
