@@ -6,8 +6,9 @@ the sum of their sizes at most, and a few 2^-24 for exp2 and the denominator.
   dv  P and dv are rounded:                                                  (2u + 2e) P^T|do| + u|dv|
   ds  rounded once; delta comes from the rounded o, dP from fp32 sums:       (2u + 2e) |ds| + P (|do| E_o + 260 * 2^-24 |do||v|)
   dq, dk  the sum of that and a rounding.
-P of backward is exp2(S - lse), and lse is that of the rounded P's sum, whose rounding errors are u of it together at most, with one P that decides it: P is off by u before it
-is rounded (once: 2u), or what it makes is.  What is rounded has its own error E by then: a rounding of x + E is off by u (|x| + E) at most, not by u |x|.  Likewise two factors
+P of backward is exp2(S - lse).  With lse of the rounded P's sum, as forward leaves it without o_low, it is off by u before it is rounded (all errors of a row are u of the sum
+together at most); with lse of the sum before that, not: the bound covers both.
+What is rounded has its own error E by then: a rounding of x + E is off by u (|x| + E) at most, not by u |x|.  Likewise two factors
 of 1 + u, and (1 + u) / (1 - u), are off from 1 by 2u + 4u^2 at most.
 """
 import math
