@@ -942,7 +942,7 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.o, o, "o")) return rc;
   if (o_low != nullptr)
     if (int rc = take_strided(p.o_low, o_low, "o_low")) return rc;
-  const bool few = fba::window_takes_few(p, fba::device_compute_units());
+  const bool few = fba::window_takes_few(p, fba::device_compute_units(), false);
   hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, false, (hipStream_t)hip_stream) : fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window forward launch");
 }
@@ -976,7 +976,7 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need))
     return fail(FBA_ERR_INVALID, "ws must be 16-byte aligned and hold %lld bytes (fba_window_workspace_bytes), got %lld", (long long)need, (long long)ws_bytes);
   p.parts = (float*)ws;
-  const bool few = fba::window_takes_few(p, fba::device_compute_units());
+  const bool few = fba::window_takes_few(p, fba::device_compute_units(), true);
   hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, true, (hipStream_t)hip_stream) : fba::launch_window_dq(p, type == FBA_FP16, (hipStream_t)hip_stream);
   if (e != hipSuccess) return hip_fail(e, "window dq launch");
   e = fba::launch_window_dkdv(p, type == FBA_FP16, (hipStream_t)hip_stream);

@@ -34,7 +34,7 @@ constexpr int kWindowTile = 128;
 inline __host__ __device__ int64_t part_floats(const WindowParams& p) { return 2 * 128 * p.key_tile; }  // dV tile, dK tile
 
 // Few query rows: forward, or dQ and neg_delta.  Few key tiles: dK and dV.
-bool window_takes_few(const WindowParams& p, int compute_units);
+bool window_takes_few(const WindowParams& p, int compute_units, bool backward);
 bool window_keys_few(const WindowParams& p, int compute_units);
 hipError_t launch_window_few_dkdv(WindowParams p, bool half, hipStream_t stream);
 hipError_t launch_window_few(WindowParams p, bool half, bool backward, hipStream_t stream);

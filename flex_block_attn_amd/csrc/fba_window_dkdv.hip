@@ -272,8 +272,9 @@ __global__ __launch_bounds__(256) void window_sum_kernel(const WindowParams p) {
 }
 
 // How the rows of a key tile are cut into items.
-//   Inside of the window: into several where there are so few tiles (of 32 keys then) that half of the compute units and more would idle, so that two items come to each, with
-//   8 slabs to an item at least.  dQ, dK and dV, one item / several, H4/1 S2048 window 1024 (64 tiles): 95 / 56 us, H8/2 S1024 window 512: 67 / 47, B2 H8/1 S1024, 400 to either side: 136 / 70.
+//   Inside of the window: into several where the tiles alone leave half of the compute units idle and more, so that two items come to each, with 16 slabs (tiles of 32 keys: 8)
+//   to an item at least.  dQ, dK and dV, one item / several, H4/1 S2048 window 1024 (64 tiles of 32): 95 / 56 us, H8/2 S1024 window 512: 67 / 47, B2 H8/1 S1024, 400 to either
+//   side: 136 / 70.
 //   Outside (tiles with sinks): into as many as are about as long as the items inside, for the longest sequence there may be, of 16 slabs (tiles of 32 keys: 8) at least.
 constexpr int kLeastSlabs = 16, kLeastSlabsFew = 8;
 int64_t plan_window_dkdv(WindowParams& p, int compute_units) {

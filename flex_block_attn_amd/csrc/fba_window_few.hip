@@ -415,18 +415,35 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   finish(acc_k, 1, p.dk, p.scale);
 }
 
-// Which launches: those that leave half of the compute units without a 128-row (128-key) tile and more.  Forward, and dQ, dK and dV, with 128-row tiles / here:
-//   6 tiles (H1 S768 window 128)           17.1 / 7.1 us    55.9 / 32.9
-//   32 (H4 S1024 window 256)               20.8 / 8.3       53.9 / 32.0
-//   128 rows, 32 keys (H8/2 S2000, 384)    26.5 / 12.4      68.0 / 53.3
-//   384, 96 (H16/4 S3000, 512)             39.2 / 33.0     127.4 / 110.3
-//   256, 256 (H8 S4096, 256)               22.3 / 19.0      72.6 / 84.2
-//   256, 256 (H8 S4096, 2048)              47.7 / 55.2     175.8 / 182.7
-bool window_takes_few(const WindowParams& p, int compute_units) {
-  return (int64_t)p.B * p.Hq * ((p.Sq + kWindowTile - 1) / kWindowTile) <= compute_units / 2;
+// Which launches.  Rows: dQ where tiles of 128 rows leave half of the compute units idle and more; forward, which reads less, up to three quarters of them, and up to one and a
+// half tiles to each as long as the keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
+// Tiles of 128 / of 32, in us:
+//   forward    window      64          256         1024        2048         4096        dQ, dK, dV    64         256        1024
+//     32 tiles (H1 S4096)    17 / 7      24 / 9      36 / 14                  73 / 33                 35 / 27    42 / 31    74 / 51
+//    100 (B2 H2 S3136)       18 / 9      25 / 11     45 / 19                                          41 / 37    52 / 45    87 / 70
+//    128 (B4 H4 S1024)       18 / 9      25 / 12     31 / 17                                          50 / 46    65 / 58    70 / 56
+//    200 (B2 H4 S3136)       20 / 15     27 / 20     48 / 33     81 / 40                              59 / 63    64 / 68   104 / 106
+//    256 (H4 S8192)          21 / 15     30 / 20     40 / 38     57 / 61      89 / 108                66 / 69    75 / 78   120 / 126
+//    384 (H6 S8192)          27 / 20     39 / 29     61 / 54
+//    400 (B2 H8 S3136)       28 / 23     38 / 33     64 / 52    107 / 76
+//    512 (H8 S8192)          30 / 27     41 / 38     61 / 69     89 / 116
+//   keys, dQ, dK, dV  window 128         512         2048
+//     16 tiles (H4/1 S2048)  46 / 33     53 / 50    110 / 110
+//     32 (H4/1 S4096)        63 / 50     85 / 86    159 / 203
+//    100 (B2 H8/2 S3136)     86 / 68    133 / 117   223 / 272
+bool window_takes_few(const WindowParams& p, int compute_units, bool backward) {
+  const int64_t tiles = (int64_t)p.B * p.Hq * ((p.Sq + kWindowTile - 1) / kWindowTile);
+  if (2 * tiles <= compute_units) return true;
+  if (backward) return false;
+  const int window = p.causal ? p.window : 2 * p.window - 1, keys = (window < p.Skv ? window : p.Skv) + p.sinks;
+  return 4 * tiles <= 3 * compute_units || (2 * tiles <= 3 * compute_units && keys <= 2048);
 }
 bool window_keys_few(const WindowParams& p, int compute_units) {
-  return (int64_t)p.B * p.Hkv * ((p.Skv + kWindowTile - 1) / kWindowTile) <= compute_units / 2;
+  const int64_t tiles = (int64_t)p.B * p.Hkv * ((p.Skv + kWindowTile - 1) / kWindowTile);
+  if (8 * tiles <= compute_units) return true;
+  const int window = p.causal ? p.window : 2 * p.window - 1;
+  const int64_t rows = (int64_t)(p.Hq / p.Hkv) * (window < p.Sq ? window : p.Sq);
+  return 2 * tiles <= compute_units && rows <= 4096;
 }
 
 hipError_t launch_window_few_dkdv(WindowParams p, bool half, hipStream_t stream) {

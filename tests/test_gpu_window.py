@@ -321,9 +321,11 @@ def test_writes_nothing_beside_its_outputs(gpu):
 @pytest.mark.parametrize("B,H,Hk,Sq,Skv,window,sinks", [
     (3, 48, 48, 70, 70, 20, 4), (2, 36, 36, 257, 257, 31, 128), (1, 48, 48, 400, 400, 100, 130), (1, 27, 27, 640, 640, 33, 4), (2, 24, 24, 300, 411, None, 0), (2, 48, 48, 300, 120, 40, 4),
     (1, 44, 44, 513, 513, 512, 600), (150, 1, 1, 33, 33, 7, 2), (2, 96, 24, 130, 130, 64, 9), (1, 64, 8, 1100, 1100, 129, 31), (1, 24, 24, 777, 777, 1, 97),
+    (4, 100, 100, 70, 70, 20, 4), (2, 66, 33, 257, 257, 31, 128), (1, 98, 49, 400, 400, 100, 130), (1, 78, 6, 640, 640, 33, 4), (2, 66, 66, 300, 411, None, 0), (2, 66, 33, 300, 120, 40, 4),
+    (1, 78, 78, 513, 513, 512, 600), (400, 1, 1, 33, 33, 7, 2), (2, 100, 20, 130, 130, 64, 9), (1, 56, 7, 777, 777, 1, 97), (1, 13, 13, 2100, 2100, None, 5),
 ])
 def test_many_rows_and_keys(gpu, dtype, causal, B, H, Hk, Sq, Skv, window, sinks):
-    """More than 128 tiles of 128 rows: tiles of 128, and from 128 tiles of keys on, there too.  (What comes before has tiles of 32 rows and keys.)"""
+    """More than 128 tiles of 128: so are those of dQ, dK and dV, from 384 on (192, where a row has more than 2048 keys) those of forward.  (What comes before has tiles of 32.)"""
     check(gpu, *inputs(gpu, B, H, Hk, Sq, Skv, dtype, Sq + H), window, sinks, causal)
 
 
@@ -331,7 +333,7 @@ def test_many_rows_and_keys(gpu, dtype, causal, B, H, Hk, Sq, Skv, window, sinks
 @pytest.mark.parametrize("window,sinks", [(60, 4), (200, 140), (None, 0), (1, 31)])
 def test_many_rows_and_keys_in_padded_batches(gpu, causal, window, sinks):
     S, lengths = 415, torch.tensor([415, 0, 1, 32, 129, 300, 1000, -3, 257], dtype=torch.int32, device=gpu)
-    q, k, v, do = inputs(gpu, len(lengths), 8, 4, S, S, torch.bfloat16, 5)
+    q, k, v, do = inputs(gpu, len(lengths), 16, 4, S, S, torch.bfloat16, 5)
     for b, n in enumerate(lengths.tolist()):
         for t in (q, k, v, do):
             t[b, :, max(0, n):] = math.nan
@@ -352,9 +354,9 @@ def test_many_rows_in_other_layouts(gpu):
     import flex_block_attn_amd as fba
 
     g = torch.Generator(device="cpu").manual_seed(3)
-    packed = torch.randn((2, 300, 3, 48, 128), generator=g).to(torch.bfloat16).to(gpu)
+    packed = torch.randn((2, 300, 3, 70, 128), generator=g).to(torch.bfloat16).to(gpu)
     a, b, c = (packed[:, :, i].transpose(1, 2) for i in range(3))
-    do = torch.randn((2, 300, 48, 128), generator=g).to(torch.bfloat16).to(gpu).transpose(1, 2)
+    do = torch.randn((2, 300, 70, 128), generator=g).to(torch.bfloat16).to(gpu).transpose(1, 2)
     results = []
     for prepare in (lambda t: t, lambda t: t.contiguous()):
         leaves = [prepare(t).detach().requires_grad_(True) for t in (a, b, c)]
