@@ -61,6 +61,9 @@ hipError_t launch_cache_append(AppendParams p, hipStream_t stream) {
 // A slot's key orders as its weight does (NaN below everything, the two zeros alike); the slots that are held are above all of them.
 namespace {
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 2048;
+// Minima one after the other / the search, both kernels, 32 x 6 heads of 4096 slots and 1, 2, 4, 8 more: 8.5 / 13.5, 9.4 / 13.6, 10.7 / 14.1, 13.4 / 14.6 us; 4 x 6 of 16384: 13.8 / 22.8,
+// 14.9 / 22.9, 17.3 / 23.4, 21.8 / 23.9; 8 of 1024: 7.8 / 11.2, 8.5 / 11.2, 10.1 / 11.4, 12.9 / 11.7.
+constexpr int kFewDropped = 6;
 FBA_DEVICE uint32_t weight_key(float w) {
   if (w != w) return 0;
   uint32_t bits = __builtin_bit_cast(uint32_t, w);
@@ -166,6 +169,71 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
     for (int j = 0; j < kHeld; ++j)
 #pragma unroll
       for (int e = 0; e < 4; ++e) key[j][e] = slot_of(j) + e < len ? key_of(at[j][e], weight[j][e]) : 0;
+  }
+  // A few over the budget, as after single tokens: as many minima of (key, slot from behind) in place of the search, and the rows move at once.
+  if constexpr (kGroups > 0) {
+    if (const int drop = len - p.budget; drop <= kFewDropped) {
+      __shared__ unsigned long long lowest[kFewDropped];
+      __shared__ int dropped[kFewDropped];
+      if (tid < kFewDropped) lowest[tid] = ~0ull;
+      __syncthreads();
+      unsigned long long own = 0;  // this thread's lowest that is still there
+      auto next = [&]() __attribute__((always_inline)) {
+        unsigned long long low = ~0ull;
+#pragma unroll
+        for (int j = 0; j < kHeld; ++j)
+#pragma unroll
+          for (int e = 0; e < 4; ++e) {
+            const unsigned long long of = (unsigned long long)key[j][e] << 32 | (uint32_t)~(slot_of(j) + e);
+            if (j < per && slot_of(j) + e < len && of > own) low = min(low, of);
+          }
+        own = low;
+      };
+      next();  // (a slot's complement is above zero)
+      for (int r = 0; r < drop; ++r) {
+        uint32_t low = own >> 32;
+#pragma unroll
+        for (int x = 1; x < 64; x *= 2) low = min(low, (uint32_t)__shfl_xor((int)low, x));
+        const bool mine = own >> 32 == low;
+        unsigned long long some = __builtin_amdgcn_ballot_w64(mine);
+        if (some & (some - 1)) {  // equal ones: the highest slot
+          uint32_t slot = mine ? (uint32_t)own : ~0u;
+#pragma unroll
+          for (int x = 1; x < 64; x *= 2) slot = min(slot, (uint32_t)__shfl_xor((int)slot, x));
+          some = __builtin_amdgcn_ballot_w64(mine && (uint32_t)own == slot);
+        }
+        if (lane == __builtin_ctzll(some)) atomicMin(&lowest[r], own);
+        __syncthreads();
+        const unsigned long long gone = lowest[r];
+        if (tid == 0) dropped[r] = (int)~(uint32_t)gone;
+        if (own == gone) next();
+      }
+      __syncthreads();
+      // lane i: the i-th dropped slot, and the i-th one behind the budget
+      const int gone = lane < drop ? dropped[lane] : 0;
+      const bool frees = lane < drop && gone < p.budget;
+      bool late = lane < drop;
+      int rank = 0;
+      for (int i = 0; i < drop; ++i) {
+        late = late && dropped[i] != p.budget + lane;
+        rank += dropped[i] < gone;
+      }
+      const unsigned long long lates = __builtin_amdgcn_ballot_w64(late);
+      const int late_rank = __builtin_popcountll(lates & ((1ull << lane) - 1)), n = __builtin_popcountll(lates);
+      for (int i = wave; i < n; i += kSelectWaves) {
+        const int to_slot = __builtin_amdgcn_readlane(gone, __builtin_ctzll(__builtin_amdgcn_ballot_w64(frees && rank == i)));
+        const int from_slot = p.budget + __builtin_ctzll(__builtin_amdgcn_ballot_w64(late && late_rank == i));
+        const int64_t to = row_of(to_slot), from = row_of(from_slot);
+        if (lane < 32) {
+          char* const rows = (lane < 16 ? cache.k : cache.v) + (lane & 15) * 16;
+          *reinterpret_cast<u32x4*>(rows + to * kRowBytes) = *reinterpret_cast<const u32x4*>(rows + from * kRowBytes);
+        }
+        if (lane == 32) cache.positions[to] = cache.positions[from];
+        if (lane == 33) cache.weights[to] = cache.weights[from];
+      }
+      if (tid == 0) moves[0] = 0;
+      return;
+    }
   }
   // f(group, this lane's four keys) for the wave's groups, in order.  Slots behind the last one have the lowest key: they are never reached, since more slots are there than stay.
   auto each = [&](auto f) {

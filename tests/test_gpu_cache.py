@@ -285,6 +285,7 @@ def evict_reference(cache, table, lengths, budget, recent, sinks):
 @pytest.mark.parametrize("lengths,budget,recent,sinks,page", [
     ([1, 2, 0], 1, 0, 0, 16), ([33, 32, 31], 32, 4, 2, 16), ([100, 300, 64], 64, 64, 0, 16), ([1025, 1024, 2000], 1000, 30, 4, 64), ([3000, 2048], 1, 1, 0, 128),
     ([5000, 4097], 4096, 256, 4, 32), ([2500, 10], 700, 0, 700, 256), ([40000], 9000, 100, 10, 256),
+    (list(range(40, 50)), 40, 5, 2, 16), (list(range(1020, 1032)), 1022, 1000, 22, 64), ([1, 2, 3, 4, 5, 6, 7, 8], 1, 0, 0, 16), ([12293, 12290, 12289], 12288, 64, 4, 128),
 ])
 def test_evict(gpu, kind, lengths, budget, recent, sinks, page):
     import flex_block_attn_amd as fba
