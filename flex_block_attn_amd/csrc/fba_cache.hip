@@ -55,11 +55,15 @@ hipError_t launch_cache_append(AppendParams p, hipStream_t stream) {
 
 // Eviction, first kernel: which slots of a (sequence, kv head) stay.  A work-group of 1024 threads reads weights and positions once, finds the budget-th largest key by
 // counting (11, 11 and 10 bits of it at a time), and lists the freed slots below the budget and the kept slots behind it, in order.  A wave has consecutive slots, 256 at a
-// time, four to a lane, so that loads are dense, ballots number the slots inside of a wave and one scan over the waves does the rest.  Bound by latency: the loads, and
-// some twenty barriers.
+// time, four to a lane, so that loads are dense, ballots number the slots inside of a wave and one scan over the waves does the rest.  Bound by latency, of the loads and
+// some twenty barriers, and, where a sequence is long, by the arithmetic for each slot on the one compute unit that its head has (24 heads of 30720: 28 us; what moves the rows, 19 us for
+// 102 MB).
 //
 // A slot's key orders as its weight does (NaN below everything, the two zeros alike); the slots that are held are above all of them.
 namespace {
+// Counters of a digit, lanes apart: weights have few exponents, and lanes that add to one counter wait for each other (4 x 6 heads of 32768 slots to 16384: 44 / 40 us with one /
+// four of each; eight, whose sum takes longer, 43, and 24 instead of 20 for 32 x 6 of 8192).
+constexpr int kCopies = 4;
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 2048;
 // Minima one after the other / the search, both kernels, 32 x 6 heads of 4096 slots and 1, 2, 4, 8 more: 8.5 / 13.5, 9.4 / 13.6, 10.7 / 14.1, 13.4 / 14.6 us; 4 x 6 of 16384: 13.8 / 22.8,
 // 14.9 / 22.9, 17.3 / 23.4, 21.8 / 23.9; 8 of 1024: 7.8 / 11.2, 8.5 / 11.2, 10.1 / 11.4, 12.9 / 11.7.
@@ -113,7 +117,8 @@ struct Ranks {
 template <int kGroups>
 __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const EvictParams p) {
   const CacheView& cache = p.cache;
-  __shared__ int bins[kBins], sums[6][kSelectWaves], found[2];
+  __shared__ __attribute__((aligned(16))) int bins[kBins * kCopies];
+  __shared__ int sums[6][kSelectWaves], found[2];
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hkv = blockIdx.x % cache.kv_heads, b = blockIdx.x / cache.kv_heads;
   int32_t* const moves = p.moves + (int64_t)blockIdx.x * (1 + 2 * (int64_t)p.most);
@@ -156,12 +161,14 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
 #pragma unroll
   for (int x = 1; x < 64; x *= 2) newest = max(newest, __shfl_xor(newest, x));
   if (lane == 0) sums[0][wave] = newest;
-  for (int i = tid; i < kBins; i += kSelectThreads) bins[i] = 0;
+  i32x4* const own_bins = reinterpret_cast<i32x4*>(bins + (kBins - 2 - 2 * tid) * kCopies);  // of this thread's two digits
+#pragma unroll
+  for (int i = 0; i < kCopies / 2; ++i) own_bins[i] = (i32x4){0, 0, 0, 0};
   __syncthreads();
 #pragma unroll
   for (int i = 0; i < kSelectWaves; ++i) newest = max(newest, sums[0][i]);
-  auto key_of = [&](int position, float w) -> uint32_t {
-    return position < p.sinks || (int64_t)position > (int64_t)newest - p.recent ? 0xffffffffu : weight_key(w);
+  auto key_of = [&](int position, float w) -> uint32_t {  // (no position is behind the newest: the difference fits)
+    return position < p.sinks || (uint32_t)newest - (uint32_t)position < (uint32_t)p.recent ? 0xffffffffu : weight_key(w);
   };
   uint32_t key[kHeld][4];
   if constexpr (kGroups > 0) {
@@ -265,20 +272,20 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
     each([&](int, const uint32_t(&k)[4]) {
 #pragma unroll
       for (int e = 0; e < 4; ++e) {
-        const bool on = digit == 0 || (k[e] >> (shift + width)) == (prefix >> (shift + width));
-        const unsigned long long ballot = __builtin_amdgcn_ballot_w64(on);
-        if (ballot == 0) continue;
-        const int bin = k[e] >> shift & ((1 << width) - 1), some = __builtin_amdgcn_readlane(bin, __builtin_ctzll(ballot));
-        if (__builtin_amdgcn_ballot_w64(on && bin != some) == 0) {  // all in one (slots without a weight, held ones): 64 lanes would wait for each other
-          if (lane == 0) atomicAdd(&bins[some], __builtin_popcountll(ballot));
-        } else if (on) {
-          atomicAdd(&bins[bin], 1);
-        }
+        if (digit == 0 || (k[e] >> (shift + width)) == (prefix >> (shift + width)))
+          atomicAdd(&bins[(k[e] >> shift & ((1 << width) - 1)) * kCopies + (lane & (kCopies - 1))], 1);
       }
     });
     __syncthreads();
     // from the largest digit down: a thread has two
-    const int d0 = kBins - 1 - 2 * tid, n0 = bins[d0], n1 = bins[d0 - 1];
+    const int d0 = kBins - 1 - 2 * tid;
+    int n0 = 0, n1 = 0;
+#pragma unroll
+    for (int i = 0; i < kCopies / 4; ++i) {
+      const i32x4 low = own_bins[i], high = own_bins[kCopies / 4 + i];
+      n1 += low[0] + low[1] + low[2] + low[3];
+      n0 += high[0] + high[1] + high[2] + high[3];
+    }
     int upto = n0 + n1, all;
 #pragma unroll
     for (int d = 1; d < 64; d *= 2) {
@@ -286,8 +293,8 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
       if (lane >= d) upto += other;
     }
     const int before = upto - n0 - n1 + waves_before(__builtin_amdgcn_readlane(upto, 63), sums[1 + digit], &all);
-    bins[d0] = 0;
-    bins[d0 - 1] = 0;
+#pragma unroll
+    for (int i = 0; i < kCopies / 2; ++i) own_bins[i] = (i32x4){0, 0, 0, 0};
     if (before < need && before + n0 >= need) {
       found[0] = d0;
       found[1] = need - before;
@@ -327,9 +334,13 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
 #pragma unroll
     for (int e = 0; e < 4; ++e) {
       if constexpr (kGroups > 0) kept |= (uint32_t)stays[e] << (4 * j + e);
-      const bool below = slot_of(j) + e < p.budget;
-      freed += __builtin_popcountll(__builtin_amdgcn_ballot_w64(!stays[e] && below));
-      late += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stays[e] && !below));
+    }
+    // (the group with the budget inside is on both sides)
+    const int s0 = (wave * per + j) * 256, inside = p.budget - s0 - 4 * lane;
+#pragma unroll
+    for (int e = 0; e < 4; ++e) {
+      if (s0 < p.budget) freed += __builtin_popcountll(__builtin_amdgcn_ballot_w64(!stays[e] && e < inside));
+      if (s0 + 256 > p.budget) late += __builtin_popcountll(__builtin_amdgcn_ballot_w64(stays[e] && e >= inside));
     }
   });
   int n_freed, n_late;
