@@ -999,8 +999,8 @@ int take_cache(fba::CacheView& to, const fba_cache* c) {
   if (c->table == nullptr || c->lengths == nullptr) return fail(FBA_ERR_INVALID, "table or lengths is null");
   if (c->weights != nullptr && !aligned16(c->weights)) return fail(FBA_ERR_INVALID, "weights is not 16-byte aligned");
   const int64_t slots = (int64_t)c->max_pages * c->page_size;
-  if (c->pages > 0x7fffffffLL || slots > 1LL << 28 || slots * c->batch > 1LL << 36 || (int64_t)c->batch * c->kv_heads > 1 << 24)
-    return fail(FBA_ERR_UNSUPPORTED, "a sequence may have 2^28 slots at most, all together 2^36, batch * kv_heads 2^24 (got %lld slots, batch %d, kv_heads %d)", (long long)slots,
+  if (c->pages > 0x7fffffffLL || slots > 1LL << 28 || slots * c->batch > 1LL << 35 || (int64_t)c->batch * c->kv_heads > 1 << 24)
+    return fail(FBA_ERR_UNSUPPORTED, "a sequence may have 2^28 slots at most, all together 2^35, batch * kv_heads 2^24 (got %lld slots, batch %d, kv_heads %d)", (long long)slots,
                 c->batch, c->kv_heads);
   to.k = (char*)c->k;
   to.v = (char*)c->v;
