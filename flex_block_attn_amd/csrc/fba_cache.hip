@@ -65,9 +65,12 @@ namespace {
 // four of each; eight, whose sum takes longer, 43, and 24 instead of 20 for 32 x 6 of 8192).
 constexpr int kCopies = 4;
 constexpr int kSelectThreads = 1024, kSelectWaves = kSelectThreads / 64, kBins = 2048;
-// Minima one after the other / the search, both kernels, 32 x 6 heads of 4096 slots and 1, 2, 4, 8 more: 8.5 / 13.5, 9.4 / 13.6, 10.7 / 14.1, 13.4 / 14.6 us; 4 x 6 of 16384: 13.8 / 22.8,
-// 14.9 / 22.9, 17.3 / 23.4, 21.8 / 23.9; 8 of 1024: 7.8 / 11.2, 8.5 / 11.2, 10.1 / 11.4, 12.9 / 11.7.
+// Minima one after the other / the search, 32 x 6 heads of 4096 slots and 1, 2, 4, 8 more (with the launch of the second kernel): 8.5 / 13.5, 9.4 / 13.6, 10.7 / 14.1, 13.4 / 14.6 us;
+// 4 x 6 of 16384: 13.8 / 22.8, 14.9 / 22.9, 17.3 / 23.4, 21.8 / 23.9; 8 of 1024: 7.8 / 11.2, 8.5 / 11.2, 10.1 / 11.4, 12.9 / 11.7.
 constexpr int kFewDropped = 6;
+// Rows that one head may have to move, by the table's size, up to which the first kernel moves them.  A second one / the first, 1, 64 and 256 slots over the budget: 32 x 6 heads of
+// 4096 slots 8.6 / 7.2, 16.6 / 14.1, 21.5 / 17.0 us; 4 x 6 of 16384: 13.9 / 12.5, 25.0 / 23.4, 27.1 / 28.1, and with 1024 29.6 / 34.1.
+constexpr int kFewMoved = 256;
 FBA_DEVICE uint32_t weight_key(float w) {
   if (w != w) return 0;
   uint32_t bits = __builtin_bit_cast(uint32_t, w);
@@ -111,6 +114,19 @@ struct Ranks {
     }
   }
 };
+
+// The i-th freed slot gets the i-th kept one from behind the budget, row, position and weight: 16 lanes to a row, i = first, first + step, ...
+FBA_DEVICE void move_rows(const CacheView& cache, const int32_t* moves, int most, int b, int hkv, int c, int first, int step, int n) {
+  for (int i = first; i < n; i += step) {
+    const int to_slot = moves[1 + i], from_slot = moves[1 + most + i];
+    const int64_t to = cache.row_of(cache.page_of(b, to_slot), hkv, to_slot), from = cache.row_of(cache.page_of(b, from_slot), hkv, from_slot);
+    const u32x4 kr = *reinterpret_cast<const u32x4*>(cache.k + from * kRowBytes + c * 16), vr = *reinterpret_cast<const u32x4*>(cache.v + from * kRowBytes + c * 16);
+    *reinterpret_cast<u32x4*>(cache.k + to * kRowBytes + c * 16) = kr;
+    *reinterpret_cast<u32x4*>(cache.v + to * kRowBytes + c * 16) = vr;
+    if (c == 0) cache.positions[to] = cache.positions[from];
+    if (c == 1) cache.weights[to] = cache.weights[from];
+  }
+}
 }  // namespace
 
 // kGroups: keys of up to kGroups times 4096 slots stay in registers (kGroups <= 8); 0: any number of slots, read again in every pass.
@@ -376,24 +392,20 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
       from += r.n;
     }
   });
-  if (tid == 0) moves[0] = n_freed;  // as many as n_late: budget slots stay
+  // (as many as n_late: budget slots stay)
+  if (p.most > kFewMoved) {
+    if (tid == 0) moves[0] = n_freed;
+  } else {
+    __syncthreads();
+    move_rows(cache, moves, p.most, b, hkv, tid & 15, tid >> 4, kSelectThreads / 16, n_freed);
+  }
 }
 
-// Second kernel: the i-th freed slot gets the i-th kept one from behind the budget, row, position and weight.
+// Second kernel, where rows are many.
 __global__ __launch_bounds__(256) void cache_move_kernel(const EvictParams p) {
-  const CacheView& cache = p.cache;
-  const int tid = threadIdx.x, c = tid & 15, item = blockIdx.y, hkv = item % cache.kv_heads, b = item / cache.kv_heads;
+  const int tid = threadIdx.x, item = blockIdx.y;
   const int32_t* const moves = p.moves + (int64_t)item * (1 + 2 * (int64_t)p.most);
-  const int n = moves[0];
-  for (int i = blockIdx.x * 16 + (tid >> 4); i < n; i += gridDim.x * 16) {
-    const int to_slot = moves[1 + i], from_slot = moves[1 + p.most + i];
-    const int64_t to = cache.row_of(cache.page_of(b, to_slot), hkv, to_slot), from = cache.row_of(cache.page_of(b, from_slot), hkv, from_slot);
-    const u32x4 kr = *reinterpret_cast<const u32x4*>(cache.k + from * kRowBytes + c * 16), vr = *reinterpret_cast<const u32x4*>(cache.v + from * kRowBytes + c * 16);
-    *reinterpret_cast<u32x4*>(cache.k + to * kRowBytes + c * 16) = kr;
-    *reinterpret_cast<u32x4*>(cache.v + to * kRowBytes + c * 16) = vr;
-    if (c == 0) cache.positions[to] = cache.positions[from];
-    if (c == 1) cache.weights[to] = cache.weights[from];
-  }
+  move_rows(p.cache, moves, p.most, item / p.cache.kv_heads, item % p.cache.kv_heads, tid & 15, blockIdx.x * 16 + (tid >> 4), gridDim.x * 16, moves[0]);
 }
 
 int64_t cache_evict_bytes(EvictParams& p) {
@@ -408,7 +420,7 @@ hipError_t launch_cache_evict(EvictParams p, hipStream_t stream) {
   void (*select)(const EvictParams) = groups <= 2 ? &cache_select_kernel<2> : groups <= 8 ? &cache_select_kernel<8> : &cache_select_kernel<0>;
   hipLaunchKernelGGL(select, dim3(items), dim3(kSelectThreads), 0, stream, p);
   hipError_t e = hipGetLastError();
-  if (e != hipSuccess || p.most == 0) return e;
+  if (e != hipSuccess || p.most <= kFewMoved) return e;
   // about 4096 work-groups, none without a row to move if all are moved
   int wgs = (p.most + 15) / 16, few = 4096 / items;
   if (few < 1) few = 1;
