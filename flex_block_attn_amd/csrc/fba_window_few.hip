@@ -416,7 +416,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
 }
 
 // Which launches.  Rows: dQ where tiles of 128 rows leave half of the compute units idle and more; forward, which reads less, up to three quarters of them, and up to one and a
-// half tiles to each as long as the keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
+// half tiles to each (three of a padded batch, where some are empty: two sequences of up to 3136 tokens, 8 heads, window 384, 43 / 37 us) as long as the keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
 // Tiles of 128 / of 32, in us:
 //   forward    window      64          256         1024        2048         4096        dQ, dK, dV    64         256        1024
 //     32 tiles (H1 S4096)    17 / 7      24 / 9      36 / 14                  73 / 33                 35 / 27    42 / 31    74 / 51
@@ -436,7 +436,8 @@ bool window_takes_few(const WindowParams& p, int compute_units, bool backward) {
   if (2 * tiles <= compute_units) return true;
   if (backward) return false;
   const int window = p.causal ? p.window : 2 * p.window - 1, keys = (window < p.Skv ? window : p.Skv) + p.sinks;
-  return 4 * tiles <= 3 * compute_units || (2 * tiles <= 3 * compute_units && keys <= 2048);
+  const int real = p.lengths != nullptr ? 1 : 2;  // of two tiles
+  return 4 * tiles <= 3 * compute_units || (real * tiles <= 3 * compute_units && keys <= 2048);
 }
 bool window_keys_few(const WindowParams& p, int compute_units) {
   const int64_t tiles = (int64_t)p.B * p.Hkv * ((p.Skv + kWindowTile - 1) / kWindowTile);
