@@ -916,7 +916,8 @@ int fill_window(fba::WindowParams& p, float* stats, const int32_t* lengths, int3
   if (int rc = check_window(lengths != nullptr, B, Hq, Hkv, Sq, Skv, window, sinks)) return rc;
   if (stats == nullptr) return fail(FBA_ERR_INVALID, "stats is null");
   p.lse = stats;
-  p.neg_delta = stats + (int64_t)B * Hq * Sq;
+  p.lse_exact = stats + (int64_t)B * Hq * Sq;
+  p.neg_delta = p.lse_exact + (int64_t)B * Hq * Sq;
   p.lengths = lengths;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
   p.window = window < (Sq > Skv ? Sq : Skv) ? window : (Sq > Skv ? Sq : Skv);  // no two positions are further apart
@@ -979,6 +980,7 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
   const bool few = fba::window_takes_few(p, fba::device_compute_units(), true);
   hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, true, (hipStream_t)hip_stream) : fba::launch_window_dq(p, type == FBA_FP16, (hipStream_t)hip_stream);
   if (e != hipSuccess) return hip_fail(e, "window dq launch");
+  p.lse = p.lse_exact;
   e = fba::launch_window_dkdv(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window dkdv launch");
 }

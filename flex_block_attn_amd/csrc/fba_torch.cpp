@@ -707,7 +707,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> run_window_forward(const at::Tens
   const c10::DeviceGuard guard(q.device());
   at::Tensor o = at::empty_like(q);
   if (!takes_strides(o)) o = at::empty(q.sizes(), q.options());
-  at::Tensor low = backward ? at::empty_like(o) : at::Tensor(), stats = at::empty({2, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  at::Tensor low = backward ? at::empty_like(o) : at::Tensor(), stats = at::empty({backward ? 3 : 1, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
   if (q.numel() == 0) return {o, stats, low};
   if (k.numel() == 0) {  // there is nothing to see
     o.zero_();
@@ -730,7 +730,7 @@ void check_window_saved(std::initializer_list<at::Tensor> tensors, const at::Ten
     TORCH_CHECK_VALUE(i == 5 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
   }
   TORCH_CHECK_VALUE(q.sizes() == d_o.sizes() && saved[3].sizes() == d_o.sizes() && saved[4].sizes() == d_o.sizes() && k.sizes() == saved[2].sizes() &&
-                        saved[5].numel() == 2 * q.size(0) * q.size(1) * q.size(2) && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+                        saved[5].numel() == 3 * q.size(0) * q.size(1) * q.size(2) && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
                         (!w.lengths.defined() || (w.lengths.size(0) == q.size(0) && q.size(2) == k.size(2))),
                     "saved tensors must come back in their shapes");
 }

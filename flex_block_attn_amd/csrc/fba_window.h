@@ -20,6 +20,7 @@ struct WindowParams {
   Strided q, k, v, o, d_o, dq, dk, dv;
   Strided o_low;           // what rounding o has left; ptr null: not wanted
   float* lse;              // [B, Hq, Sq], in log2 units; +inf for a row that sees nothing
+  float* lse_exact;        // [B, Hq, Sq], of P before rounding, found by dQ for dK and dV
   float* neg_delta;        // [B, Hq, Sq], -rowsum(dO o O)
   const int32_t* lengths;  // null, or [B]
   float* parts;            // fp32 partial sums of dK and dV of key tiles with several items
@@ -39,8 +40,8 @@ bool window_keys_few(const WindowParams& p, int compute_units);
 hipError_t launch_window_few_dkdv(WindowParams p, bool half, hipStream_t stream);
 hipError_t launch_window_few(WindowParams p, bool half, bool backward, hipStream_t stream);
 hipError_t launch_window_fwd(WindowParams p, bool half, hipStream_t stream);
-hipError_t launch_window_dq(WindowParams p, bool half, hipStream_t stream);    // before dK and dV: works neg_delta out
-hipError_t launch_window_dkdv(WindowParams p, bool half, hipStream_t stream);  // d_o has q's row stride
+hipError_t launch_window_dq(WindowParams p, bool half, hipStream_t stream);    // before dK and dV: works lse_exact and neg_delta out
+hipError_t launch_window_dkdv(WindowParams p, bool half, hipStream_t stream);  // lse: the exact one; d_o has q's row stride
 // Decides on key_tile, band_parts, sink_tiles and sink_parts; returns the bytes of `parts` that dK and dV need.
 int64_t plan_window_dkdv(WindowParams& p, int compute_units);
 

@@ -79,6 +79,10 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[mb][r] = 0.f;
 
+  // The sum of a row's P as they are formed here: one, but for what forward's rounding of P has left in lse.  dQ is divided by it, and dK and dV get an lse that has it.  (Half of
+  // that error is a row's own: without this dq of 150 to 600 keys in fp16 is off by 1.5 times what rounding it alone does, with it by 1.45.)
+  float of_p[2] = {0.f, 0.f}, lse2 = INFINITY;
+  const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Sq + min(row, rows - 1);
   if (last_row >= row0) {
     // Q and dO as B operands: lane holds row l32, d = 16 ks + 8 h .. +7 (rows behind the last: that one)
     x8 qreg[8], doreg[8];
@@ -89,8 +93,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     // delta: with what rounding o has left, where that is there (a row's error in it goes into all of its dS)
     const char* const lp = p.o_low.ptr == nullptr ? op : p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)from * p.o_low.row + 16 * h;
     const float low = p.o_low.ptr == nullptr ? 0.f : 1.f;
-    const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Sq + from;
-    float lse2 = p.lse[stat];
+    lse2 = p.lse[stat];
     float sum = 0.f;
 #pragma unroll
     for (int ks = 0; ks < 8; ++ks) {
@@ -142,7 +145,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
             acc[mb] = Elem<T>::mfma32(read_tr8<T>(pair + tr.rd[mb][0] + roff, pair + tr.rd[mb][1] + roff), ds[j], acc[mb]);
           }
       };
-      auto form_ds = [&](LdsPtr pair, auto between) {
+      auto form_ds = [&](LdsPtr pair, auto between, auto sees) __attribute__((always_inline)) {
         f32x16 s, d;
 #pragma unroll
         for (int r = 0; r < 16; ++r) { s[r] = 0.f; d[r] = neg_delta; }
@@ -152,9 +155,16 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           d = Elem<T>::mfma32(read_b128<T>(pair + kSlabBytes + rm.rd[ks]), doreg[ks], d);
           between(ks);
         }
-#pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -lse2)) * d[r];
+        sees(s, d);
         return s;
+      };
+      auto unmasked = [&](f32x16& s, const f32x16& d) __attribute__((always_inline)) {  // dS from S and dP - delta
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+          const float pv = fast_exp2(__builtin_fmaf(s[r], c, -lse2));
+          of_p[r & 1] += pv;
+          s[r] = pv * d[r];
+        }
       };
       // Step t (t % 4 == R): S_t, dP_t | dS_t | dQ += K_t^T dS_t.  Slab t+3 is requested into the buffer of slab t-1, between the first matrix instructions; behind the step
       // slab t+1 must have landed (and has, as slab t+2): what step t requested may still fly.
@@ -168,18 +178,21 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           else v_dma.piece(i - 2, into + kSlabBytes, vp + slab * v_step, slab);
         };
         if (kind != kNone) {
-          f32x16 s = form_ds(pair, [&](int ks) {
+          const f32x16 ds = form_ds(pair, [&](int ks) {
             if (ks < 4 && t > 0) request(ks);
-          });
-          if (kind == kMasked) {
+          }, [&](f32x16& s, const f32x16& d) __attribute__((always_inline)) {
+            if (kind != kMasked) return unmasked(s, d);
             const int k0 = slab_of(t) * kSlab + 4 * h, a = lo - k0, z = hi - k0, y = sk - k0;
 #pragma unroll
             for (int r = 0; r < 16; ++r) {
               const int e = 8 * (r >> 2) + (r & 3);
-              s[r] = (e >= a && e <= z) || e < y ? s[r] : 0.f;
+              const bool sees = (e >= a && e <= z) || e < y;
+              const float pv = sees ? fast_exp2(__builtin_fmaf(s[r], c, -lse2)) : 0.f;
+              of_p[r & 1] += pv;
+              s[r] = sees ? pv * d[r] : 0.f;
             }
-          }
-          add_dq(pair, s);
+          });
+          add_dq(pair, ds);
         } else if (t > 0) {
 #pragma unroll
           for (int i = 0; i < 4; ++i) request(i);
@@ -198,7 +211,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           if (ks == 1) dma16(into + 4 * kRowBytes, k_src, k_dma.off[1]);
           if (ks == 2) dma16(into + kSlabBytes, v_src, v_dma.off[0]);
           if (ks == 3) dma16(into + kSlabBytes + 4 * kRowBytes, v_src, v_dma.off[1]);
-        });
+        }, unmasked);
         add_dq(pair, s);
         wait_vmem<4>();
         __syncthreads();
@@ -231,7 +244,9 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       __syncthreads();
     }
   }
-  store_tile<T>(smem + wave * kSlabBytes, acc, p.scale, p.dq.ptr + b * p.dq.batch + hq * p.dq.head + (int64_t)wrow0 * p.dq.row, p.dq.row, lane, p.Sq - wrow0);
+  const float sum_p = sum_halves(of_p[0] + of_p[1]);
+  if (h == 0 && there) p.lse_exact[stat] = sum_p > 0.f ? lse2 + __builtin_log2f(sum_p) : lse2;
+  store_tile<T>(smem + wave * kSlabBytes, acc, sum_p > 0.f ? p.scale / sum_p : p.scale, p.dq.ptr + b * p.dq.batch + hq * p.dq.head + (int64_t)wrow0 * p.dq.row, p.dq.row, lane, p.Sq - wrow0);
 }
 
 hipError_t launch_window_dq(WindowParams p, bool half, hipStream_t stream) {

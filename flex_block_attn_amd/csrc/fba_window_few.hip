@@ -30,7 +30,7 @@ FBA_DEVICE void wait_fetches() { asm volatile("s_waitcnt lgkmcnt(0)" : : : "memo
 template <typename T, bool kBackward>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves), amdgpu_waves_per_eu(2, 2))) void window_few_kernel(const WindowParams p) {
   __shared__ __attribute__((aligned(16))) char smem[kWaves * 2 * kSlabBytes];  // [wave][K slab | V slab]; at the end [wave][32 rows][128] floats
-  __shared__ float ml[3][kWaves][kRows];
+  __shared__ float ml[2][kWaves][kRows];
   using x8 = x8_of<T>;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -69,7 +69,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
     for (int r = 0; r < 16; ++r) acc[mb][r] = 0.f;
-  float m_run = kNoReference, l_run = 0.f, l_exact = 0.f;
+  float m_run = kNoReference, l_run = 0.f;
   const float c = p.scale_log2e;
 
   if (last_row >= row0) {
@@ -156,6 +156,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
           const float pv = fast_exp2(__builtin_fmaf(s[r], c, -lse2));
+          l_run += pv;
           s[r] = s[r] == -INFINITY ? 0.f : pv * d[r];
         }
       } else {
@@ -166,7 +167,6 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
           const float m_new = fmaxf(m_run, max_halves(mx)), alpha = fast_exp2((m_run - m_new) * c);
           m_run = m_new;
           l_run *= alpha;
-          l_exact *= alpha;
 #pragma unroll
           for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
@@ -175,10 +175,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
         const float mc = m_run * c;
 #pragma unroll
         for (int r = 0; r < 16; ++r) s[r] = fast_exp2(__builtin_fmaf(s[r], c, -mc));
-#pragma unroll
-        for (int r = 0; r < 16; ++r) l_exact += s[r];
       }
-      // rounded to T as the matrix instruction takes it (P: o's denominator sums the rounded values; lse is of the sum before)
+      // rounded to T as the matrix instruction takes it (P: the denominator sums the rounded values)
 #pragma unroll
       for (int j = 0; j < 2; ++j) pk[j] = narrow8<T>(s, j);
       if constexpr (!kBackward) {
@@ -214,11 +212,10 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
 #pragma unroll
       for (int i = 0; i < 4; ++i)
         *reinterpret_cast<f32x4*>(own + l32 * 512 + (((8 * mb + 2 * i + h) ^ l32) << 4)) = (f32x4){acc[mb][4 * i + 0], acc[mb][4 * i + 1], acc[mb][4 * i + 2], acc[mb][4 * i + 3]};
-    const float l = sum_halves(l_run), le = sum_halves(l_exact);
+    const float l = sum_halves(l_run);  // (backward: the sum of P)
     if (h == 0) {
       ml[0][wave][l32] = m_run;
       ml[1][wave][l32] = l;
-      ml[2][wave][l32] = le;
     }
   }
   __syncthreads();
@@ -228,18 +225,23 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   if constexpr (kBackward) {
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) factor[w] = 1.f;
+    const float l = ml[1][0][r] + ml[1][1][r] + ml[1][2][r] + ml[1][3][r];  // as in fba_window_dq.hip
+    if (l > 0.f) scale /= l;
+    if ((tid & 7) == 0 && row0 + r < rows) {
+      const int64_t stat = ((int64_t)b * p.Hq + hq) * p.Sq + row0 + r;
+      p.lse_exact[stat] = p.lse[stat] + (l > 0.f ? __builtin_log2f(l) : 0.f);
+    }
   } else {
-    float m = kNoReference, l = 0.f, le = 0.f;
+    float m = kNoReference, l = 0.f;
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[0][w][r]);
 #pragma unroll
     for (int w = 0; w < kWaves; ++w) {
       factor[w] = fast_exp2((ml[0][w][r] - m) * c);
       l += factor[w] * ml[1][w][r];
-      le += factor[w] * ml[2][w][r];
     }
     scale = l > 0.f ? 1.f / l : 0.f;
-    if ((tid & 7) == 0) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row0 + r] = l > 0.f ? m * c + __builtin_log2f(le) : INFINITY;
+    if ((tid & 7) == 0) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row0 + r] = l > 0.f ? m * c + __builtin_log2f(l) : INFINITY;
   }
   const Strided& out = kBackward ? p.dq : p.o;
   char* const to = out.ptr + b * out.batch + hq * out.head + (int64_t)(row0 + r) * out.row;

@@ -30,8 +30,7 @@ enum Kind { kNone, kFull, kMasked };
 
 }  // namespace
 
-// kLearns: backward will come, and what it needs exactly is left to it
-template <typename T, bool kLearns>
+template <typename T>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(2, 2))) void window_fwd_kernel(const WindowParams p) {
   extern __shared__ __attribute__((aligned(16))) char smem[];  // K ring [4][8 KiB] | V ring [4][8 KiB]
   using x8 = x8_of<T>;
@@ -85,7 +84,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
   const int64_t k_step = (int64_t)p.k.row * kSlab, v_step = (int64_t)p.v.row * kSlab;
 
   f32x16 acc[4];
-  float l_run = 0.f, l_exact = 0.f, m_run = kNoReference;
+  float l_run = 0.f, m_run = kNoReference;
   const float c = p.scale_log2e;
 #pragma unroll
   for (int mb = 0; mb < 4; ++mb)
@@ -167,7 +166,6 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         const float alpha = fast_exp2((m_run - m_new) * c);
         m_run = m_new;
         l_run *= alpha;
-        l_exact *= alpha;
 #pragma unroll
         for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
@@ -181,18 +179,11 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
 #pragma unroll
       for (int j = 0; j < 2; ++j) {
-        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one.  For backward lse is of the sum
-        // before: with that of the rounded ones all P of a row are off by what is left of their errors (dq of 150 to 600 keys in fp16, against 64 bits: 1.5 times the error of
-        // rounding it, instead of 1.45; H24 S30720, 1152 to either side: forward with it 1200 us, without 1100, of a step of 4.6 ms).
+        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one (lse, of
+        // that sum, is off by half a step of T at most for it; backward finds the sum before rounding, where there is more time for sixteen additions: 25 us against 130)
         p_prev[j] = narrow8<T>(s_cur, j);
 #pragma unroll
         for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);
-      }
-      if constexpr (kLearns) {
-        float sum[2] = {0.f, 0.f};
-#pragma unroll
-        for (int r = 0; r < 16; ++r) sum[r & 1] += s_cur[r];
-        l_exact += sum[0] + sum[1];
       }
       pin(p_prev[0]);
       pin(p_prev[1]);
@@ -284,11 +275,10 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
   }
 
   const float l = sum_halves(l_run);
-  const float of_lse = kLearns ? sum_halves(l_exact) : l;
-  if (h == 0 && row < p.Sq) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l > 0.f ? m_run * c + __builtin_log2f(of_lse) : INFINITY;
+  if (h == 0 && row < p.Sq) p.lse[((int64_t)b * p.Hq + hq) * p.Sq + row] = l > 0.f ? m_run * c + __builtin_log2f(l) : INFINITY;
   const float scale = l > 0.f ? 1.f / l : 0.f;
   store_tile<T>(smem + wave * kSlabBytes, acc, scale, p.o.ptr + b * p.o.batch + hq * p.o.head + (int64_t)wrow0 * p.o.row, p.o.row, lane, p.Sq - wrow0);
-  if constexpr (kLearns)
+  if (p.o_low.ptr != nullptr)  // for backward
     store_tile<T, true>(smem + wave * kSlabBytes, acc, scale, p.o_low.ptr + b * p.o_low.batch + hq * p.o_low.head + (int64_t)wrow0 * p.o_low.row, p.o_low.row, lane, p.Sq - wrow0);
 }
 
@@ -297,8 +287,7 @@ hipError_t launch_window_fwd(WindowParams p, bool half, hipStream_t stream) {
   p.tiles = (p.Sq + kWindowTile - 1) / kWindowTile;
   p.items = p.B * p.Hq * p.tiles;
   p.chunk = window_chunk(p.items);
-  const bool learns = p.o_low.ptr != nullptr;
-  void (*fn)(const WindowParams) = half ? (learns ? &window_fwd_kernel<_Float16, true> : &window_fwd_kernel<_Float16, false>) : learns ? &window_fwd_kernel<__bf16, true> : &window_fwd_kernel<__bf16, false>;
+  void (*fn)(const WindowParams) = half ? &window_fwd_kernel<_Float16> : &window_fwd_kernel<__bf16>;
   hipLaunchKernelGGL(fn, dim3(window_grid(p.items, p.chunk)), dim3(256), kSmem, stream, p);
   return hipGetLastError();
 }

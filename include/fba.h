@@ -379,11 +379,10 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  * is not read.  A value of v that is no number or infinite reaches the rows that see it, and others of its 32-row neighbourhood.
  *
  * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
- * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [2, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first half (+inf
- * for rows without a visible key), backward uses the second.
- * o_low, shaped like o, may be null: what rounding o has left, rounded.  Backward subtracts rowsum(d_o o) from every row, and takes o + o_low for it; where o_low is asked for,
- * stats comes from the weights before they are rounded for the second product, too (dq of a window of 350 keys: off by 0.0024 of its size instead of 0.0027, of which 0.0017
- * are its own rounding).
+ * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [3, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first
+ * third (+inf for rows without a visible key), backward uses the others.
+ * o_low, shaped like o, may be null: what rounding o has left, rounded.  Backward subtracts rowsum(d_o o) from every row, and takes o + o_low for it where it is there (dq of
+ * a window of 350 keys: off by 0.0024 of its size instead of 0.0027, of which 0.0017 are its own rounding).
  * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes on the same GPU, 16-byte aligned, for partial sums of dk and dv (0 bytes: may be null), and d_o with the row
  * stride of q (FBA_ERR_UNSUPPORTED otherwise).
  * Sq and Skv at most 2^28, B * Hq * Sq and B * Hkv * Skv below 2^29.

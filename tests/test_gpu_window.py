@@ -6,8 +6,8 @@ the sum of their sizes at most, and a few 2^-24 for exp2 and the denominator.
   dv  P and dv are rounded:                                                  (2u + 2e) P^T|do| + u|dv|
   ds  rounded once; delta comes from the rounded o, dP from fp32 sums:       (2u + 2e) |ds| + P (|do| E_o + 260 * 2^-24 |do||v|)
   dq, dk  the sum of that and a rounding.
-P of backward is exp2(S - lse).  With lse of the rounded P's sum, as forward leaves it without o_low, it is off by u before it is rounded (all errors of a row are u of the sum
-together at most); with lse of the sum before that, not: the bound covers both.
+P of backward is exp2(S - lse).  With lse of the rounded P's sum, as forward leaves it, it is off by u before it is rounded (all errors of a row are u of the sum together at
+most); with that of the sum before, not: the bound covers both.
 What is rounded has its own error E by then: a rounding of x + E is off by u (|x| + E) at most, not by u |x|.  Likewise two factors
 of 1 + u, and (1 + u) / (1 - u), are off from 1 by 2u + 4u^2 at most.
 """
@@ -300,7 +300,7 @@ def test_writes_nothing_beside_its_outputs(gpu):
     q, k, v, do = inputs(gpu, B, H, Hk, S, S, torch.bfloat16, 6)
     around = [torch.full((B + 2, h, S + 6, 136), 7.0, dtype=torch.bfloat16, device=gpu) for h in (H, H, Hk, Hk)]
     inner = [t[1:-1, :, 3:-3, :128] for t in around]
-    stats = torch.full((2 * B * H * S + 64,), 7.0, device=gpu)
+    stats = torch.full((3 * B * H * S + 64,), 7.0, device=gpu)
     of = lambda t: ctypes.byref(Strided(t.data_ptr(), *t.stride()[:3]))
     sizes = (B, H, Hk, S, S, 128, 40, 5, 1, 0)
     _lib.call("fba_window_fwd", of(q), of(k), of(v), of(inner[0]), None, ctypes.c_void_p(stats.data_ptr()), None, *sizes, _stream())
