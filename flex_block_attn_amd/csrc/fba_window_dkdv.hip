@@ -6,7 +6,8 @@
 // of 32 query rows travel global -> LDS into a ring of four (Q | dO | lse2 | -delta) buffers, three steps ahead, and feed all four waves, by rows (S, dP) and transposed
 // (dV, dK).  A step is 32 matrix instructions for a wave; two waves on a SIMD, of work-groups that know nothing of each other, cover each other's exponentials, fetches and
 // waits, and what a work-group takes before its first and behind its last slab: a tile has few of them, its window's.
-// (64 keys to a wave, one wave on a SIMD, as the kernel for block lists: half the LDS bytes, but nobody to cover the ends: 2351 us instead of 1880 for H24 S30720, 1152 to either side.)
+// (64 keys to a wave, one wave on a SIMD, as the kernel for block lists: half the LDS bytes, but nobody to cover the ends: 2351 us instead of 1880 for H24 S30720, window 1152 to
+// both sides, 384 sinks, where the matrix pipe is busy 59 % of the time.)
 //
 // The rows that see a key tile are those from its window, and, of a tile with sinks, all behind (and in front of) it.  A work item is a tile with a part of the rows inside
 // of the window, or of those outside; where a tile has more than one they leave fp32 sums, which a small kernel adds in order.  The last slab of a sequence is moved back to

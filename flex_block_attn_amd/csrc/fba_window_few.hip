@@ -3,7 +3,8 @@
 // The same products as in fba_window_fwd.hip and fba_window_dq.hip, dealt out otherwise: a work-group has 32 query rows, and its four waves take the slabs of 32 keys in turn,
 // each through a K slab and a V slab of its own in LDS, so that there is no barrier before the end, where the four sums meet in LDS.  A launch has four times the
 // work-groups, each with a quarter of the steps one after the other; K and V are read four times as often, from L2.
-// For launches that leave most compute units without a 128-row tile: bound by latency, of the first loads and of each step.
+// For launches that leave most compute units without a 128-row tile: bound by latency, of the first loads and of each step
+// (H1 S768 window 128: forward 7 us of which the launch is 3; B2 H8/2 S3136 window 384, padded: forward 36, dK and dV 62).
 #include "fba_types.h"
 #include "fba_window.h"
 #include "fba_window_keys.h"
