@@ -84,7 +84,7 @@ def _check_cache(cache, table, lengths):
         raise ValueError(f"lengths must be int32 of shape ({table.shape[0]},), got {lengths.dtype} {tuple(lengths.shape)}")
     if table.shape[1] * k.shape[2] > 1 << 28 or table.shape[0] > 0x7fffff or k.shape[1] > 65535 or k.shape[0] > 0x7fffffff:
         raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a sequence may have 2^28 slots at most, a pool 2^31 - 1 pages of 65535 heads, got table {tuple(table.shape)}, cache {tuple(k.shape)}")
-    for name, t in (("cache.k", k), ("cache.v", cache.v), ("cache.weights", cache.weights)):
+    for name, t in (("cache.k", k), ("cache.v", cache.v), ("cache.positions", cache.positions), ("cache.weights", cache.weights)):
         if t is not None and t.data_ptr() % 16:
             raise ValueError(f"{name} must be 16-byte aligned")
 
@@ -137,7 +137,8 @@ def cache_append(cache, table, lengths, k, v, counts=None, positions=None, weigh
             raise ValueError(f"weights must be float32 of shape {tuple(k.shape[:3])} on {k.device}, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
     _no_gradients(**{"cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights, "k": k, "v": v, "weights": weights})
     if k.shape[2] == 0:
-        return lengths.clone()
+        right = (lengths >= 0) & (lengths <= table.shape[1] * cache.k.shape[2])
+        return torch.where(right if counts is None else right & (counts == 0), lengths, -1)
     dense = lambda t: None if t is None else t.contiguous()
     return _answered(_lib.host().cache_append(*given, _rows_dense(k), _rows_dense(v), dense(counts), dense(positions), dense(weights)))
 

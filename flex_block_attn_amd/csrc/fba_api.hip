@@ -999,7 +999,7 @@ int take_cache(fba::CacheView& to, const fba_cache* c) {
     return fail(FBA_ERR_INVALID, "pages, kv_heads, batch and max_pages must be positive (got %lld %d %d %d)", (long long)c->pages, c->kv_heads, c->batch, c->max_pages);
   if (c->page_size < 16 || (c->page_size & (c->page_size - 1))) return fail(FBA_ERR_INVALID, "page_size (%d) must be a power of two, 16 at least", c->page_size);
   if (c->table == nullptr || c->lengths == nullptr) return fail(FBA_ERR_INVALID, "table or lengths is null");
-  if (c->weights != nullptr && !aligned16(c->weights)) return fail(FBA_ERR_INVALID, "weights is not 16-byte aligned");
+  if (!aligned16(c->positions) || !aligned16(c->weights)) return fail(FBA_ERR_INVALID, "positions or weights is not 16-byte aligned");
   const int64_t slots = (int64_t)c->max_pages * c->page_size;
   if (c->pages > 0x7fffffffLL || slots > 1LL << 28 || slots * c->batch > 1LL << 35 || (int64_t)c->batch * c->kv_heads > 1 << 24)
     return fail(FBA_ERR_UNSUPPORTED, "a sequence may have 2^28 slots at most, all together 2^35, batch * kv_heads 2^24 (got %lld slots, batch %d, kv_heads %d)", (long long)slots,

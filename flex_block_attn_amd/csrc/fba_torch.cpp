@@ -886,7 +886,7 @@ bool cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& positi
   if (k.numel() == 0 || k.size(0) > 0x7fffffffLL || k.size(1) > 65535 || page < 16 || page > 1 << 28 || (page & (page - 1)) != 0) return false;
   if (table.device() != k.device() || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || table.numel() == 0) return false;
   if (table.size(0) > 0x7fffff || table.size(1) * page > 1LL << 28 || !is_ints(lengths, k, table.size(0))) return false;
-  for (const at::Tensor* t : {&k, &v, &weights})
+  for (const at::Tensor* t : {&k, &v, &positions, &weights})
     if (t->defined() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) != 0) return false;
   *c = {k.data_ptr(), v.data_ptr(), positions.defined() ? positions.data_ptr<int32_t>() : nullptr, weights.defined() ? weights.data_ptr<float>() : nullptr,
         table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), k.size(0), (int32_t)k.size(1), (int32_t)page, (int32_t)table.size(0), (int32_t)table.size(1)};

@@ -37,7 +37,7 @@ ROW = Strided(A, 256, 128, 128)
 
 @pytest.mark.parametrize("change,code,text", [
     (dict(k=None), 1, "cache k"), (dict(v=0x1008), 1, "aligned"), (dict(pages=0), 1, "positive"), (dict(max_pages=0), 1, "positive"), (dict(batch=0), 1, "positive"),
-    (dict(page_size=8), 1, "page_size"), (dict(page_size=48), 1, "page_size"), (dict(table=None), 1, "table"), (dict(lengths=None), 1, "lengths"), (dict(weights=0x1004), 1, "weights"),
+    (dict(page_size=8), 1, "page_size"), (dict(page_size=48), 1, "page_size"), (dict(table=None), 1, "table"), (dict(lengths=None), 1, "lengths"), (dict(weights=0x1004), 1, "weights"), (dict(positions=0x1008), 1, "positions"),
     (dict(max_pages=1 << 25), 2, "2^28"), (dict(pages=1 << 31), 2, "slots"), (dict(page_size=256, max_pages=1 << 20, batch=256), 2, "2^35"),
 ])
 def test_c_entries_refuse_a_cache(change, code, text):

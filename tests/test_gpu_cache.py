@@ -102,6 +102,7 @@ def check_attend(q, cache, table, lengths, window=None, sinks=0, accumulate=Fals
 @pytest.mark.parametrize("lengths,H,Hk,page", [
     ([1], 1, 1, 16), ([0, 1, 2], 2, 1, 16), ([15, 16, 17, 31, 32, 33], 8, 2, 16), ([63, 64, 65, 127, 129], 6, 6, 64), ([255, 256, 257, 1000], 12, 4, 32),
     ([5000, 3, 0, 777], 16, 1, 128), ([2049], 17, 1, 16), ([700, 300], 33, 1, 256), ([700, 300], 70, 1, 32), ([640], 130, 2, 64), ([9001, 4000], 24, 6, 64),
+    ([5000, 4096, 1], 8, 2, 4096),
 ])
 def test_attend(gpu, dtype, accumulate, lengths, H, Hk, page):
     cache, table, g = make(gpu, len(lengths), Hk, max(lengths + [1]), page, dtype, seed=sum(lengths), extra=1)
@@ -285,7 +286,7 @@ def evict_reference(cache, table, lengths, budget, recent, sinks):
 @pytest.mark.parametrize("lengths,budget,recent,sinks,page", [
     ([1, 2, 0], 1, 0, 0, 16), ([33, 32, 31], 32, 4, 2, 16), ([100, 300, 64], 64, 64, 0, 16), ([1025, 1024, 2000], 1000, 30, 4, 64), ([3000, 2048], 1, 1, 0, 128),
     ([5000, 4097], 4096, 256, 4, 32), ([2500, 10], 700, 0, 700, 256), ([40000], 9000, 100, 10, 256),
-    (list(range(40, 50)), 40, 5, 2, 16), (list(range(1020, 1032)), 1022, 1000, 22, 64), ([1, 2, 3, 4, 5, 6, 7, 8], 1, 0, 0, 16), ([12293, 12290, 12289], 12288, 64, 4, 128),
+    (list(range(40, 50)), 40, 5, 2, 16), (list(range(1020, 1032)), 1022, 1000, 22, 64), ([1, 2, 3, 4, 5, 6, 7, 8], 1, 0, 0, 16), ([12293, 12290, 12289], 12288, 64, 4, 128), ([33000, 32900], 32850, 100, 4, 64),
 ])
 def test_evict(gpu, kind, lengths, budget, recent, sinks, page):
     import flex_block_attn_amd as fba
@@ -460,3 +461,60 @@ def test_strided_queries_and_rows(gpu):
     small = torch.tensor([10, 20], dtype=torch.int32, device=gpu)
     fba.cache_append(cache, table, small, rows_, rows_)
     assert torch.equal(rows(cache.k, table, 1, 25)[:, 20:], rows_[1])
+
+
+def test_append_of_nothing(gpu):
+    import flex_block_attn_amd as fba
+
+    cache, table, g = make(gpu, 5, 2, 64, 16)
+    n = torch.tensor([0, 64, 65, -2, 3], dtype=torch.int32, device=gpu)
+    k = torch.empty((5, 2, 0, 128), dtype=torch.bfloat16, device=gpu)
+    assert fba.cache_append(cache, table, n, k, k).tolist() == [0, 64, -1, -1, 3]
+    assert fba.cache_append(cache, table, n, k, k, counts=torch.tensor([0, 0, 0, 0, 1], dtype=torch.int32, device=gpu)).tolist() == [0, 64, -1, -1, -1]
+
+
+def test_pages_that_several_sequences_read(gpu):
+    """A prompt that all share stands in the table of each: only what is written to may not."""
+    import flex_block_attn_amd as fba
+
+    cache, table, g = make(gpu, 3, 2, 200, 16)
+    fill(cache, table, [200, 200, 200], g)
+    shared = table.clone()
+    shared[1:, :5] = table[0, :5]
+    lengths = [200, 120, 81]
+    q = torch.randn((3, 4, 1, 128), generator=g).to(torch.bfloat16).to(gpu)
+    check_attend(q, cache, shared, lengths)
+    check_attend(q, cache, shared, lengths, window=50, sinks=20)
+    n = torch.tensor([200, 80, 80], dtype=torch.int32, device=gpu)
+    k = torch.randn((3, 2, 1, 128), generator=g).to(torch.bfloat16).to(gpu)
+    n = fba.cache_append(cache, torch.cat([shared, table[:, :1]], 1).contiguous(), n, k, k, counts=torch.tensor([0, 1, 1], dtype=torch.int32, device=gpu))
+    assert n.tolist() == [200, 81, 81] and torch.equal(rows(cache.k, shared, 2, 81)[:, 80:], k[2])
+
+
+def test_graphs_that_replay_in_turn_on_two_streams(gpu):
+    """Each has a workspace of its own."""
+    import flex_block_attn_amd as fba
+
+    lengths = [2000, 100, 0, 900]
+    cache, table, g = make(gpu, 4, 2, 2000, 32)
+    fill(cache, table, lengths, g)
+    n = torch.tensor(lengths, dtype=torch.int32, device=gpu)
+    qs = [torch.randn((4, 8, 1, 128), generator=g).to(torch.bfloat16).to(gpu) for _ in range(2)]
+    want = [fba.cache_attn_func(q, cache, table, n) for q in qs]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for q in qs:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(fba.cache_attn_func(q, cache, table, n))
+    streams = [torch.cuda.Stream() for _ in qs]
+    for _ in range(4):
+        for o in outs:
+            o.fill_(math.nan)
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for o, w in zip(outs, want):
+            assert torch.equal(o, w)

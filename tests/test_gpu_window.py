@@ -419,3 +419,79 @@ def test_capture_beside_an_earlier_graph_of_the_same_leaves(gpu):
         torch.cuda.synchronize()
         for x, y in zip(out, want):
             assert torch.equal(x, y)
+
+
+def test_rows_and_batches_far_apart(gpu):
+    """Offsets in bytes beyond 32 bits, by the rows' stride (the largest there may be), and by the batches'."""
+    import flex_block_attn_amd as fba
+
+    step, S = 1 << 24, 150
+    buf = torch.zeros(S * step, dtype=torch.bfloat16, device=gpu)  # 5 GB
+    assert 2 * (S - 1) * step > 2**32
+    g = torch.Generator(device="cpu").manual_seed(1)
+    by_rows = [buf.as_strided((1, 2, S, 128), (0, 512, step, 1), 128 * i) for i in range(4)]
+    last = S * step - 2**18
+    by_batches = [buf.as_strided((2, 2, S, 128), (last, 128 * S, 128, 1), 2**16 * i) for i in range(4)]
+    for views in (by_rows, by_batches):
+        new = [torch.randn(v.shape, generator=g).to(torch.bfloat16).to(gpu) for v in views]
+        for v, x in zip(views, new):
+            v.copy_(x)
+        results = []
+        for prepare in (lambda t: t, lambda t: t.contiguous()):
+            leaves = [prepare(t).detach().requires_grad_(True) for t in views[:3]]
+            o = fba.window_attn_func(*leaves, 70, sinks=9)
+            results.append((o.detach(), *torch.autograd.grad(o, leaves, prepare(views[3]))))
+        for x, y in zip(*results):
+            assert torch.equal(x, y)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("H,S", [(2, 300), (140, 300)])
+def test_large_scores(gpu, dtype, H, S):
+    """So large that one key has all the weight: finite, a row of v each, and no gradient to speak of in q and k."""
+    import flex_block_attn_amd as fba
+
+    q, k, v, do = inputs(gpu, 1, H, H, S, S, dtype, 3, size=1.0)
+    leaves = [t.requires_grad_(True) for t in (q * 1000, k, v)]
+    o = fba.window_attn_func(*leaves, 40, sinks=3)
+    grads = torch.autograd.grad(o, leaves, do)
+    s = (leaves[0].detach().double() @ k.detach().double().transpose(-1, -2) * SCALE).masked_fill(~visible(S, S, 40, 3, True, device=gpu), -math.inf)
+    top = s.topk(2, -1)
+    clear = top.values[..., 0] - top.values[..., 1] > 40  # the second one's weight is below 2^-57
+    assert int(clear.sum()) > clear.numel() // 2
+    best = torch.gather(v.detach(), 2, top.indices[..., :1].expand(-1, -1, -1, 128))
+    assert torch.equal(o[clear], best[clear])
+    for x in grads:
+        assert bool(torch.isfinite(x).all())
+
+
+def test_graphs_that_replay_in_turn_on_two_streams(gpu):
+    """Whole steps; each graph has its own workspaces."""
+    import flex_block_attn_amd as fba
+
+    sets = [[t.requires_grad_(i < 3) for i, t in enumerate(inputs(gpu, 1, 4, 2, 400, 400, torch.bfloat16, seed))] for seed in (1, 2)]
+
+    def step(q, k, v, do):
+        o = fba.window_attn_func(q, k, v, 60, sinks=40)
+        return (o.detach(), *torch.autograd.grad(o, (q, k, v), do))
+
+    want = [[x.clone() for x in step(*s)] for s in sets]
+    torch.cuda.synchronize()
+    graphs, outs = [], []
+    for s in sets:
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(step(*s))
+    streams = [torch.cuda.Stream() for _ in sets]
+    for _ in range(4):
+        for out in outs:
+            for x in out:
+                x.fill_(math.nan)
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            for x, y in zip(out, w):
+                assert torch.equal(x, y)
