@@ -138,10 +138,30 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
   const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
   const int hkv = blockIdx.x % cache.kv_heads, b = blockIdx.x / cache.kv_heads;
   int32_t* const moves = p.moves + (int64_t)blockIdx.x * (1 + 2 * (int64_t)p.most);
+  // The table is fetched beside the length, as much as there is: what keys in registers can be of has kGroups * 256 pages at most.
+  constexpr int kPages = kGroups * 256, kOwnPages = (kPages + kSelectThreads - 1) / kSelectThreads;
+  __shared__ int pages[kPages > 0 ? kPages : 1];
+  int page[kOwnPages > 0 ? kOwnPages : 1];
+#pragma unroll
+  for (int i = 0; i < kOwnPages; ++i) {
+    const int at = tid + i * kSelectThreads;
+    page[i] = at < cache.max_pages ? cache.table[(int64_t)b * cache.max_pages + at] : -1;
+  }
   const int len = cache.lengths[b];
   bool bad = !cache.holds(len);
-  if (!bad)
-    for (int i = tid; i < (len + (1 << cache.page_log2) - 1) >> cache.page_log2; i += kSelectThreads) bad |= cache.page_of(b, i << cache.page_log2) < 0;
+  const int used = bad ? 0 : (len + (1 << cache.page_log2) - 1) >> cache.page_log2;
+  if constexpr (kGroups > 0) {
+#pragma unroll
+    for (int i = 0; i < kOwnPages; ++i) {
+      const int at = tid + i * kSelectThreads;
+      if (at < used) {
+        pages[at] = page[i];
+        bad |= page[i] < 0 || page[i] >= cache.pages;
+      }
+    }
+  } else {
+    for (int i = tid; i < used; i += kSelectThreads) bad |= cache.page_of(b, i << cache.page_log2) < 0;
+  }
   bad = __syncthreads_or(bad);
   if (tid == 0 && hkv == 0) p.lengths_out[b] = bad ? -1 : min(len, p.budget);
   if (bad || len <= p.budget) {
@@ -149,7 +169,7 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
     return;
   }
   typedef int32_t i32x4 __attribute__((ext_vector_type(4)));
-  auto row_of = [&](int slot) { return cache.row_of(cache.page_of(b, slot), hkv, slot); };  // of four slots, which are on one page
+  auto row_of = [&](int slot) { return cache.row_of(kGroups > 0 ? pages[slot >> cache.page_log2] : cache.page_of(b, slot), hkv, slot); };  // of four slots, which are on one page
   const int per = (len + 4 * kSelectThreads - 1) / (4 * kSelectThreads);  // groups of 256 slots that a wave has
   auto slot_of = [&](int j) { return (wave * per + j) * 256 + 4 * lane; };
 
