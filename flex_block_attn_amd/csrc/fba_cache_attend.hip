@@ -86,8 +86,11 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
     return b < cache.batch ? tiles_of(length_of(p, b, &bad), p.window, p.sinks).n : 0;
   };
   int total = 0;
-  const int of_first = tiles_in(lane);  // sequences 0 .. 63
-  for (int b0 = 0; b0 < cache.batch; b0 += 64) total += wave_sum(b0 == 0 ? of_first : tiles_in(b0 + lane));
+  const bool one = cache.batch == 1;              // (needs no sums over the wave: 8.1 us instead of 8.5 for 768 slots)
+  const int of_first = tiles_in(one ? 0 : lane);  // sequences 0 .. 63
+  if (one) total = __builtin_amdgcn_readfirstlane(of_first);
+  else
+    for (int b0 = 0; b0 < cache.batch; b0 += 64) total += wave_sum(b0 == 0 ? of_first : tiles_in(b0 + lane));
   const Shares shares{total, min(p.target, max(1, (total + kLeastTiles - 1) / kLeastTiles))};
   const int w = blockIdx.x;
   if (w >= shares.wgs) return;
@@ -95,7 +98,14 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   const int end = shares.begin(w + 1);
   const bool notes = w == 0 && blockIdx.y == 0;  // writes down which shares every sequence is in
   int b = -1, start = 0;                         // the sequence of `tile`, its first tile
-  for (int b0 = 0, before = 0; b0 < cache.batch && (b < 0 || notes); b0 += 64) {
+  if (one) {
+    b = 0;
+    if (notes && tid == 0) {
+      p.note[0] = 0;
+      p.note[1] = total > 0 ? shares.of(total - 1) + 1 : 0;
+    }
+  }
+  for (int b0 = 0, before = 0; !one && b0 < cache.batch && (b < 0 || notes); b0 += 64) {
     const int n = b0 == 0 ? of_first : tiles_in(b0 + lane);
     int sum = n;  // of the lanes up to this one
 #pragma unroll
