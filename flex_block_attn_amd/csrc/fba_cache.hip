@@ -56,7 +56,7 @@ hipError_t launch_cache_append(AppendParams p, hipStream_t stream) {
 // Eviction, first kernel: which slots of a (sequence, kv head) stay.  A work-group of 1024 threads reads weights and positions once, finds the budget-th largest key by
 // counting (11, 11 and 10 bits of it at a time), and lists the freed slots below the budget and the kept slots behind it, in order.  A wave has consecutive slots, 256 at a
 // time, four to a lane, so that loads are dense, ballots number the slots inside of a wave and one scan over the waves does the rest.  Bound by latency, of the loads and
-// some twenty barriers, and, where a sequence is long, by the arithmetic for each slot on the one compute unit that its head has (24 heads of 30720: 28 us; what moves the rows, 19 us for
+// some twenty barriers, and, where a sequence is long, by the arithmetic for each slot on the one compute unit that its head has (24 heads of 30720: 27 us; what moves the rows, 19 us for
 // 102 MB).
 //
 // A slot's key orders as its weight does (NaN below everything, the two zeros alike); the slots that are held are above all of them.

@@ -343,9 +343,10 @@ def test_many_rows_and_keys_in_padded_batches(gpu, causal, window, sinks):
             assert int(x[b, :, max(0, n):].count_nonzero()) == 0
 
 
-@pytest.mark.parametrize("B,H,Hk,S,window,sinks,causal", [(1, 4, 1, 2048, 1024, 0, True), (1, 8, 2, 1024, 512, 40, True), (2, 8, 1, 700, 300, 5, False), (1, 1, 1, 1536, 700, 64, False)])
+@pytest.mark.parametrize("B,H,Hk,S,window,sinks,causal", [(1, 4, 1, 2048, 1024, 0, True), (1, 8, 2, 1024, 512, 40, True), (2, 8, 1, 700, 300, 5, False), (1, 1, 1, 1536, 700, 64, False), (1, 8, 2, 2200, 1500, 40, True),
+                                                             (1, 8, 2, 2200, 1200, 0, False), (3, 16, 2, 900, 600, 200, True)])
 def test_few_keys_with_many_rows_each(gpu, B, H, Hk, S, window, sinks, causal):
-    """A tile's rows are cut into several items."""
+    """A tile's rows are cut into several items: tiles of 32 keys, and, where they have more than 4096 rows, of 128."""
     check(gpu, *inputs(gpu, B, H, Hk, S, S, torch.bfloat16, S), window, sinks, causal)
 
 
