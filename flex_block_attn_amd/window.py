@@ -89,7 +89,8 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     i + kv_seq_len - q_seq_len.  `window` None: no limit.  `lengths`, int32 (batch,) on the GPU: sequence b has lengths[b] tokens, the rows behind them are
     padding (not read, zeros in o and in the gradients); q and k then have one length.  A row that sees no key is zeros.
 
-    Scores of keys that a row does not see may be anything; v has to be finite there (a weight of zero times infinity is no number), padding excepted.
+    Scores of keys that a row does not see may be anything; v has to be finite there, and for gradients q, k and the gradient of o too (a weight of zero times infinity is no
+    number), padding excepted.
 
     Returns o, shaped like q.  Differentiable in q, k and v, once.  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
     graph of the same leaves may be alive then (backward raises)."""

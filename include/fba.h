@@ -376,7 +376,8 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  * count as the nearest of the two), its other rows are padding and row i stands at i.  Key j is visible to row i when both are tokens and
  *   causal != 0:  j <= p and (p - j < window or j < sinks)        causal = 0:  |p - j| < window or j < sinks
  * o = softmax(q k^T / sqrt(128)) v over the visible keys; rows without any, and padding, are zeros, and so are their gradients.  Padding of q, k, v and d_o
- * is not read.  A value of v that is no number or infinite reaches the rows that see it, and others of its 32-row neighbourhood.
+ * is not read.  A value of v that is no number or infinite reaches the rows that see it, and others of its 32-row neighbourhood; in backward one of q, k or d_o does so in dk,
+ * dq and dk, and dv and dk.
  *
  * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
  * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [3, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first
