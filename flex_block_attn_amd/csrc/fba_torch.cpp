@@ -735,29 +735,30 @@ void check_window_saved(std::initializer_list<at::Tensor> tensors, const at::Ten
                     "saved tensors must come back in their shapes");
 }
 
-// A leaf's place in autograd's graph keeps the stream on which it was first used for as long as a graph with it lives.  While backward is captured, autograd would make
-// that stream, which has no part in the capture, wait for the capturing one: that breaks the capture and ends the process.
-void refuse_foreign_leaves(const at::Tensor& q) {
+// A leaf's place in autograd's graph keeps the stream on which it was first used for as long as a graph with it lives.  While backward is captured, autograd makes that stream
+// wait for the capturing one.  Any other stream becomes part of the capture by that; the default one cannot, which breaks the capture and ends the process.
+void refuse_leaves_of_the_default_stream(const at::Tensor& q) {
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
-  const c10::hip::HIPStream here = c10::hip::getCurrentHIPStream(q.device().index());
-  bool foreign = false;
+  const auto of_default = c10::hip::getDefaultHIPStream(q.device().index()).id();
+  if (c10::hip::getCurrentHIPStream(q.device().index()).id() == of_default) return;
+  bool there = false;
   for (const torch::autograd::Edge& edge : node->next_edges())
     if (edge.function != nullptr && dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) != nullptr) {
       const auto stream = edge.function->stream();
-      foreign = foreign || (stream.has_value() && (stream->device_index() != here.device_index() || stream->id() != here.id()));
+      there = there || (stream.has_value() && stream->id() == of_default);
     }
-  if (!foreign) return;
+  if (!there) return;
   pybind11::gil_scoped_acquire gil;
   const bool capturing = pybind11::module_::import("torch").attr("cuda").attr("is_current_stream_capturing")().cast<bool>();
-  TORCH_CHECK(!capturing, "backward is captured on another stream than that of an earlier graph of the same leaves: drop what holds that graph before the capture");
+  TORCH_CHECK(!capturing, "backward is captured while an earlier graph of the same leaves, made on the default stream, is alive: drop what holds that graph before the capture");
 }
 
 std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
                                             const at::Tensor& stats, at::Tensor d_o, const Window& w) {
   check_window_saved({given_q, k, v, o, low, stats}, d_o, w);
   const c10::DeviceGuard guard(given_q.device());
-  refuse_foreign_leaves(given_q);
+  refuse_leaves_of_the_default_stream(given_q);
   at::Tensor q = given_q;
   std::vector<at::Tensor> grads;
   for (const at::Tensor* t : {&given_q, &k, &v}) {

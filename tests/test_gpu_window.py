@@ -408,6 +408,9 @@ def test_capture_beside_an_earlier_graph_of_the_same_leaves(gpu):
                 torch.autograd.grad(f(*leaves, 30, sinks=3), leaves, do)
         for x, y in zip(torch.autograd.grad(earlier, leaves, do), want[1:]):
             assert torch.equal(x, y)
+        with torch.cuda.stream(torch.cuda.Stream()):  # outside of a capture another stream is nobody's business
+            assert len(torch.autograd.grad(f(*leaves, 30, sinks=3), leaves, do)) == 3
+        torch.cuda.synchronize()
         del earlier
         graph = torch.cuda.CUDAGraph()
         with torch.cuda.graph(graph):
