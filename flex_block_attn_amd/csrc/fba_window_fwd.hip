@@ -136,11 +136,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
       for (int ks = 0; ks < 8; ++ks) s = Elem<T>::mfma32(read_b128<T>(slab + rm.rd[ks]), qreg[ks], s);
       return s;
     };
-    f32x16 s_cur;
-#pragma unroll
-    for (int r = 0; r < 16; ++r) s_cur[r] = 0.f;
-    int kind = kind_of(0), kind_before = kNone;  // of the step's slab and the one before
-    if (kind != kNone) s_cur = scores(k_lds);
+    int kind_before = kNone;  // of the slab before the step's
+    f32x16 s_cur = scores(k_lds);
     pin(s_cur);
     __syncthreads();
 
@@ -197,21 +194,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
     // Behind it K_{t+2} and V_t must have landed; what steps t-1 and t requested may still fly.
     auto step = [&](auto ring_c, int t) {
       constexpr int R = decltype(ring_c)::value;
-      const int kind_next = kind_of(t + 1);
       const int k_slab = slab_at(t + 4), v_slab = slab_at(t + 2);
-      const uint32_t k_into = k_dst + R * kSlabBytes, v_into = v_dst + ((R + 2) & 3) * kSlabBytes;
-      if (kind_before != kNone) {
-        add_pv(v_lds + ((R + 3) & 3) * kSlabBytes, [&](int i) {
-          if (i == 0) k_dma.piece(0, k_into, kp + k_slab * k_step, k_slab);
-          if (i == 2) k_dma.piece(1, k_into, kp + k_slab * k_step, k_slab);
-          if (i == 4) v_dma.piece(0, v_into, vp + v_slab * v_step, v_slab);
-          if (i == 6) v_dma.piece(1, v_into, vp + v_slab * v_step, v_slab);
-        });
-      } else {
-        k_dma.copy(k_into, kp + k_slab * k_step, k_slab);
-        if (t > 0) v_dma.copy(v_into, vp + v_slab * v_step, v_slab);  // (the first three V slabs are there)
-      }
-      if (kind == kMasked) {
+      k_dma.copy(k_dst + R * kSlabBytes, kp + k_slab * k_step, k_slab);
+      if (t > 0) v_dma.copy(v_dst + ((R + 2) & 3) * kSlabBytes, vp + v_slab * v_step, v_slab);  // (the first three V slabs are there)
+      if (kind_before != kNone) add_pv(v_lds + ((R + 3) & 3) * kSlabBytes, [](int) {});
+      const int kind = kind_of(t);
+      if (kind != kFull) {
         const int k0 = slab_of(t) * kSlab + 4 * h, a = lo - k0, z = hi - k0, y = sk - k0;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
@@ -219,13 +207,12 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           s_cur[r] = (e >= a && e <= z) || e < y ? s_cur[r] : -INFINITY;
         }
       }
-      if (kind != kNone) raise();
-      f32x16 s_nxt = s_cur;
-      if (kind_next != kNone) s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
-      if (kind != kNone) weights();
+      // (where no row sees the slab its weights are zero, and V is not touched; there is no branch around them, which would cost registers that are not there)
+      raise();
+      const f32x16 s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
+      weights();
       s_cur = s_nxt;
       kind_before = kind;
-      kind = kind_next;
       wait_vmem<8>();
       __syncthreads();
     };
@@ -265,7 +252,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           whole_step(IC<3>{});
           t += 4;
         } while (t + 4 <= whole_end);
-        kind_before = kind = kFull;
+        kind_before = kFull;
       }
       step(IC<0>{}, t);
       if (t + 1 < n) step(IC<1>{}, t + 1);
