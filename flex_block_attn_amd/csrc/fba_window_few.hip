@@ -270,7 +270,7 @@ constexpr int kFewPartFloats = 2 * kRows * kHeadDim;
 
 template <typename T>
 __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves), amdgpu_waves_per_eu(2, 2))) void window_few_dkdv_kernel(const WindowParams p) {
-  __shared__ __attribute__((aligned(16))) char smem[kWaves * kStageBytes];  // at the end [wave][32 keys][128] floats, dV and then dK
+  __shared__ __attribute__((aligned(256))) char smem[kWaves * kStageBytes];  // at the end [wave][32 keys][128] floats, dV and then dK
   using x8 = x8_of<T>;
   const int tid = threadIdx.x, lane = tid & 63, l32 = lane & 31, h = lane >> 5;
   const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -306,25 +306,23 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
     const uint32_t stat_off = (uint32_t)(h * ((const char*)p.neg_delta - (const char*)p.lse));
     // Slab s_begin + t; the last slab of the rows is moved back to end with them (its first rows are masked then).
     const int tail = max(0, rows - kSlab), least = min(31, rows - 1);
-    auto place_of = [&](int t, int* g, int* row_min) {
-      const int s = item.s_begin + t;
-      *g = s / slabs.n;
-      *row_min = slabs.at(s % slabs.n) * kSlab;
-      return min(*row_min, tail);
-    };
-    auto request = [&](uint32_t to, const char* from, uint32_t stride) __attribute__((always_inline)) {
+    int g = (item.s_begin + wave) / slabs.n, i_slab = (item.s_begin + wave) % slabs.n, row_min = slabs.at(i_slab) * kSlab, row0 = min(row_min, tail);
+    uint32_t off[8];  // of Q and dO, whose rows are equally far apart
 #pragma unroll
-      for (int i = 0; i < 8; ++i) {
-        const int r = 4 * i + (lane >> 4);
-        dma16(to + i * 4 * kRowBytes, from, (uint32_t)min(r, least) * stride + (((lane & 15) ^ swz(r)) << 4));
-      }
+    for (int i = 0; i < 8; ++i) {
+      const int r = 4 * i + (lane >> 4);
+      off[i] = (uint32_t)min(r, least) * p.q.row + (((lane & 15) ^ swz(r)) << 4);
+      asm volatile("" : "+v"(off[i]));  // (worked out again in every step otherwise)
+    }
+    auto request = [&](uint32_t to, const char* from) __attribute__((always_inline)) {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) dma16(to + i * 4 * kRowBytes, from, off[i]);
     };
     auto request_do = [&](int g, int row0) __attribute__((always_inline)) {
-      request(dst + kSlabBytes, db + g * p.d_o.head + (int64_t)row0 * p.d_o.row, p.d_o.row);
+      request(dst + kSlabBytes, db + g * p.d_o.head + (int64_t)row0 * p.d_o.row);
       dma4(dst + 2 * kSlabBytes, sb + ((int64_t)g * p.Sq + row0) * 4, stat_off + min(l32, least) * 4);
     };
-    auto request_q = [&](int g, int row0) __attribute__((always_inline)) { request(dst, qb + g * p.q.head + (int64_t)row0 * p.q.row, p.q.row); };
-    int g, row_min, row0 = place_of(wave, &g, &row_min);
+    auto request_q = [&](int g, int row0) __attribute__((always_inline)) { request(dst, qb + g * p.q.head + (int64_t)row0 * p.q.row); };
     request_do(g, row0);
     request_q(g, row0);
 
@@ -332,25 +330,28 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
     rm.init(lane);
     TransposedOffsets tr;
     tr.init(lane);
-    const LdsPtr qt = lds_ptr(smem + wave * kStageBytes), dt = qt + kSlabBytes, st = qt + 2 * kSlabBytes + 16 * h;
+    // operand steps and column blocks only move the 16-byte chunk inside a 256-byte row, by an exclusive-or
+    static_assert(kStageBytes % 256 == 0 && kSlabBytes % 256 == 0, "the exclusive-ors below touch bits 5..7");
+    const LdsPtr st = lds_ptr(smem + wave * kStageBytes), q_base = st + rm.rd[0], t_base = st + tr.rd[0][0], stat = st + 2 * kSlabBytes + 16 * h;
+    auto flip = [](LdsPtr ptr, uint32_t bits) { return (LdsPtr)(uintptr_t)((uint32_t)(uintptr_t)ptr ^ bits); };
     const float c = p.scale_log2e;
     for (int t = wave; t < n; t += kWaves) {
       wait_copies<0>();
       f32x16 s, dp;
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 d4 = lds_read_f32x4(st + 4 * kSlab + 32 * i);
+        const f32x4 d4 = lds_read_f32x4(stat + 4 * kSlab + 32 * i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) { s[4 * i + e] = 0.f; dp[4 * i + e] = d4[e]; }
       }
 #pragma unroll
       for (int ks = 0; ks < 8; ++ks) {
-        s = Elem<T>::mfma32(read_b128<T>(qt + rm.rd[ks]), kreg[ks], s);
-        dp = Elem<T>::mfma32(read_b128<T>(dt + rm.rd[ks]), vreg[ks], dp);
+        s = Elem<T>::mfma32(read_b128<T>(flip(q_base, 32u * ks)), kreg[ks], s);
+        dp = Elem<T>::mfma32(read_b128<T>(flip(q_base, 32u * ks) + kSlabBytes), vreg[ks], dp);
       }
 #pragma unroll
       for (int i = 0; i < 4; ++i) {
-        const f32x4 l4 = lds_read_f32x4(st + 32 * i);
+        const f32x4 l4 = lds_read_f32x4(stat + 32 * i);
 #pragma unroll
         for (int e = 0; e < 4; ++e) {
           const float pv = fast_exp2(__builtin_fmaf(s[4 * i + e], c, -l4[e]));
@@ -370,19 +371,22 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int mb = 0; mb < 4; ++mb) {
-          const int roff = 16 * j * kRowBytes;
-          acc_v[mb] = Elem<T>::mfma32(read_tr8<T>(dt + tr.rd[mb][0] + roff, dt + tr.rd[mb][1] + roff), pk[j], acc_v[mb]);
+          const LdsPtr t0 = flip(t_base, (uint32_t)(mb << 6)) + 16 * j * kRowBytes, t1 = flip(t_base, (uint32_t)(mb << 6 | 32)) + (16 * j + 8) * kRowBytes;
+          acc_v[mb] = Elem<T>::mfma32(read_tr8<T>(t0 + kSlabBytes, t1 + kSlabBytes), pk[j], acc_v[mb]);
         }
       // (past the last slab: that one again, into places that nobody reads any more)
-      const int next0 = place_of(min(t + kWaves, n - 1), &g, &row_min);
+      if (t + kWaves < n)
+        for (i_slab += kWaves; i_slab >= slabs.n; i_slab -= slabs.n) ++g;
+      row_min = slabs.at(i_slab) * kSlab;
+      const int next0 = min(row_min, tail);
       wait_fetches();
       request_do(g, next0);
 #pragma unroll
       for (int j = 0; j < 2; ++j)
 #pragma unroll
         for (int mb = 0; mb < 4; ++mb) {
-          const int roff = 16 * j * kRowBytes;
-          acc_k[mb] = Elem<T>::mfma32(read_tr8<T>(qt + tr.rd[mb][0] + roff, qt + tr.rd[mb][1] + roff), dsk[j], acc_k[mb]);
+          const LdsPtr t0 = flip(t_base, (uint32_t)(mb << 6)) + 16 * j * kRowBytes, t1 = flip(t_base, (uint32_t)(mb << 6 | 32)) + (16 * j + 8) * kRowBytes;
+          acc_k[mb] = Elem<T>::mfma32(read_tr8<T>(t0, t1), dsk[j], acc_k[mb]);
         }
       wait_fetches();
       request_q(g, next0);
