@@ -4,7 +4,7 @@
 // each through a K slab and a V slab of its own in LDS, so that there is no barrier before the end, where the four sums meet in LDS.  A launch has four times the
 // work-groups, each with a quarter of the steps one after the other; K and V are read four times as often, from L2.
 // For launches that leave most compute units without a 128-row tile: bound by latency, of the first loads and of each step
-// (H1 S768 window 128: forward 7 us of which the launch is 3; B2 H8/2 S3136 window 384, padded: forward 36, dK and dV 62).
+// (H1 S768 window 128: forward 7 us of which the launch is 3; B2 H8/2 S3136 window 384, padded: dK and dV 55).
 #include "fba_types.h"
 #include "fba_window.h"
 #include "fba_window_keys.h"
@@ -422,29 +422,27 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   finish(acc_k, 1, p.dk, p.scale);
 }
 
-// Which launches.  Rows: dQ where tiles of 128 rows leave half of the compute units idle and more; forward, which reads less, up to three quarters of them, and up to one and a
-// half tiles to each (three of a padded batch, where some are empty: two sequences of up to 3136 tokens, 8 heads, window 384, 43 / 37 us) as long as the keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
+// Which launches.  Rows: dQ where tiles of 128 rows leave half of the compute units idle and more; forward, which reads less, up to seven eighths of them, and up to all where the
+// keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
 // Tiles of 128 / of 32, in us:
-//   forward    window      64          256         1024        2048         4096        dQ, dK, dV    64         256        1024
-//     32 tiles (H1 S4096)    17 / 7      24 / 9      36 / 14                  73 / 33                 35 / 27    42 / 31    74 / 51
-//    100 (B2 H2 S3136)       18 / 9      25 / 11     45 / 19                                          41 / 37    52 / 45    87 / 70
-//    128 (B4 H4 S1024)       18 / 9      25 / 12     31 / 17                                          50 / 46    65 / 58    70 / 56
-//    200 (B2 H4 S3136)       20 / 15     27 / 20     48 / 33     81 / 40                              59 / 63    64 / 68   104 / 106
-//    256 (H4 S8192)          21 / 15     30 / 20     40 / 38     57 / 61      89 / 108                66 / 69    75 / 78   120 / 126
-//    384 (H6 S8192)          27 / 20     39 / 29     61 / 54
-//    400 (B2 H8 S3136)       28 / 23     38 / 33     64 / 52    107 / 76
-//    512 (H8 S8192)          30 / 27     41 / 38     61 / 69     89 / 116
+//   window, forward          64          128         256         512        1024        2048        4096      dQ, dK, dV  128         512         2048
+//     32 tiles (H1 S4096)    13 / 7      15 / 8      18 / 8      23 / 10     30 / 14     44 / 20     68 / 31              31 / 23     50 / 35     95 / 54
+//    100 (B2 H2 S3136)       14 / 8      16 / 10     19 / 11     24 / 14     37 / 18     64 / 27                          37 / 33     54 / 45    119 / 85
+//    128 (B4 H4 S1024)       14 / 8      16 / 10     19 / 11     24 / 14     27 / 17                                      37 / 33     53 / 44
+//    200 (B2 H4 S3136)       15 / 12     17 / 16     20 / 19     25 / 23     38 / 31     65 / 38                          41 / 48     62 / 68    152 / 135
+//    256 (H4 S8192)          16 / 13     18 / 17     21 / 20     26 / 25     33 / 36     48 / 57     78 / 103             45 / 51     67 / 72    151 / 162
+//    384 (H6 S8192)          22 / 20     24 / 24     28 / 29     36 / 36     50 / 51     77 / 84    125 / 152             62 / 71     97 / 105   231 / 244
+//    512 (H8 S8192)          24 / 25     26 / 31     29 / 36     37 / 46     51 / 66     79 / 110   128 / 200             65 / 83    100 / 121   238 / 283
 //   keys, dQ, dK, dV  window 128         512         2048
-//     16 tiles (H4/1 S2048)  46 / 33     53 / 50    110 / 110
-//     32 (H4/1 S4096)        63 / 50     85 / 86    159 / 203
-//    100 (B2 H8/2 S3136)     86 / 68    133 / 117   223 / 272
+//     16 tiles (H4/1 S2048)  46 / 32     53 / 47    110 / 101
+//     32 (H4/1 S4096)        63 / 48     85 / 84    159 / 203
+//    100 (B2 H8/2 S3136)     86 / 64    133 / 110   221 / 272
 bool window_takes_few(const WindowParams& p, int compute_units, bool backward) {
   const int64_t tiles = (int64_t)p.B * p.Hq * ((p.Sq + kWindowTile - 1) / kWindowTile);
   if (2 * tiles <= compute_units) return true;
   if (backward) return false;
   const int window = p.causal ? p.window : 2 * p.window - 1, keys = (window < p.Skv ? window : p.Skv) + p.sinks;
-  const int real = p.lengths != nullptr ? 1 : 2;  // of two tiles
-  return 4 * tiles <= 3 * compute_units || (real * tiles <= 3 * compute_units && keys <= 2048);
+  return 8 * tiles <= 7 * compute_units || (tiles <= compute_units && keys <= 512);
 }
 bool window_keys_few(const WindowParams& p, int compute_units) {
   const int64_t tiles = (int64_t)p.B * p.Hkv * ((p.Skv + kWindowTile - 1) / kWindowTile);

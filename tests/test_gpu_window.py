@@ -325,7 +325,7 @@ def test_writes_nothing_beside_its_outputs(gpu):
     (1, 78, 78, 513, 513, 512, 600), (400, 1, 1, 33, 33, 7, 2), (2, 100, 20, 130, 130, 64, 9), (1, 56, 7, 777, 777, 1, 97), (1, 13, 13, 2100, 2100, None, 5),
 ])
 def test_many_rows_and_keys(gpu, dtype, causal, B, H, Hk, Sq, Skv, window, sinks):
-    """More than 128 tiles of 128: so are those of dQ, dK and dV, from 384 on (192, where a row has more than 2048 keys) those of forward.  (What comes before has tiles of 32.)"""
+    """More than 128 tiles of 128: so are those of dQ, dK and dV, from 256 on those of forward.  (What comes before has tiles of 32.)"""
     check(gpu, *inputs(gpu, B, H, Hk, Sq, Skv, dtype, Sq + H), window, sinks, causal)
 
 
