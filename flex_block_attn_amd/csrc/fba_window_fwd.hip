@@ -9,9 +9,9 @@
 // A slab that all 32 rows of a wave see whole needs no mask, one that none of them sees no work; of a window's slabs only the first and the last two or so
 // are masked, by two compares for every score.
 //
-// Bound by issue: the matrix pipe is busy 44 to 46 % of the time and the VALU 42, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
+// Bound by issue: the matrix pipe is busy 49 % of the time and the VALU 45, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
 // time, with longer waits for copies none).  H24 S30720, window 1152 to both sides, 384 sinks: 1.07 ms, 0.99 TFLOP of visible pairs, 920 TFLOP/s; H24/6 S69120 window 1536, 128
-// sinks: 1.53 ms, 915 TFLOP/s, read from memory 0.55 GB; H24 S30720 window 128: 243 us, 0.95 GB.
+// sinks: 1.53 ms, 915 TFLOP/s, read from memory 0.48 GB; H24 S30720 window 128: 243 us, 0.95 GB.
 #include <type_traits>
 
 #include "fba_types.h"
@@ -24,7 +24,7 @@ namespace {
 constexpr int kSlab = 32;
 constexpr int kSlabBytes = kSlab * kRowBytes;  // 8 KiB
 constexpr int kRing = 4;
-constexpr float kLazy = 8.f;             // log2 headroom before the softmax reference is raised
+constexpr float kMostSum = 256.f;         // of a lane's weights in a step (far from where fp16 ends)
 constexpr float kNoReference = -3e38f;   // of a row that has met no score yet: finite, so that exp2 never sees inf - inf
 
 template <int N>
@@ -158,11 +158,32 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           between(4 * j + mb);
         }
     };
-    auto raise = [&]() {  // the reference, if some row would otherwise see exponents above kLazy
-      float mx = s_cur[0];
+    // p_prev := P_t against the rows' reference m.  Where they add up to more than kMostSum, m has fallen behind: it is raised, with what has been summed, and they are formed anew.
+    // (The sum is there anyway; the maximum in front of every step costs H24/6 S69120 window 1536 1585 us instead of 1550.)
+    auto weights = [&]() {
+      const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
+      float sum[2];
+      auto form = [&]() __attribute__((always_inline)) {
+        const float mc = m_run * c;
+        f32x16 w;
 #pragma unroll
-      for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
-      if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kLazy) != 0) {
+        for (int r = 0; r < 16; ++r) w[r] = fast_exp2(__builtin_fmaf(s_cur[r], c, -mc));
+        sum[0] = sum[1] = 0.f;
+#pragma unroll
+        for (int j = 0; j < 2; ++j) {
+          // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one (lse, of that sum, is off by half
+          // a step of T at most for it; backward finds the sum before rounding, where there is more time for sixteen additions: 25 us against 130)
+          p_prev[j] = narrow8<T>(w, j);
+#pragma unroll
+          for (int i = 0; i < 4; ++i) sum[j] = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, sum[j]);
+        }
+        sum[0] += sum[1];
+      };
+      form();
+      if (__builtin_amdgcn_ballot_w64(sum[0] > kMostSum) != 0) {
+        float mx = s_cur[0];
+#pragma unroll
+        for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
         const float m_new = fmaxf(m_run, max_halves(mx));
         const float alpha = fast_exp2((m_run - m_new) * c);
         m_run = m_new;
@@ -171,27 +192,15 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         for (int mb = 0; mb < 4; ++mb)
 #pragma unroll
           for (int r = 0; r < 16; ++r) acc[mb][r] *= alpha;
+        form();
       }
-    };
-    auto weights = [&]() {  // p_prev := P_t
-      const float mc = m_run * c;
-#pragma unroll
-      for (int r = 0; r < 16; ++r) s_cur[r] = fast_exp2(__builtin_fmaf(s_cur[r], c, -mc));
-      const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
-#pragma unroll
-      for (int j = 0; j < 2; ++j) {
-        // rounded to T as the matrix instruction takes it; the denominator sums the rounded values, so that the weights still add up to one (lse, of
-        // that sum, is off by half a step of T at most for it; backward finds the sum before rounding, where there is more time for sixteen additions: 25 us against 130)
-        p_prev[j] = narrow8<T>(s_cur, j);
-#pragma unroll
-        for (int i = 0; i < 4; ++i) l_run = Elem<T>::dot2((typename Elem<T>::x2){p_prev[j][2 * i], p_prev[j][2 * i + 1]}, one2, l_run);
-      }
+      l_run += sum[0];
       pin(p_prev[0]);
       pin(p_prev[1]);
     };
     // Step t (t % 4 == R): O += P_{t-1} V_{t-1} | softmax(S_t) | S_{t+1} = K_{t+1} Q^T.  P_{t-1} was formed against the reference m of step t-1, so it reaches O before
-    // step t may raise m.  The copies that a step owes, K_{t+4} into the buffer of K_t and V_{t+2} into that of V_{t-2}, go between its first matrix instructions.
-    // Behind it K_{t+2} and V_t must have landed; what steps t-1 and t requested may still fly.
+    // step t may raise m.  The copies that a step owes, K_{t+4} into the buffer of K_t and V_{t+2} into that of V_{t-2}, go in front of the matrix instructions (between
+    // them in steps without masks).  Behind it K_{t+2} and V_t must have landed; what steps t-1 and t requested may still fly.
     auto step = [&](auto ring_c, int t) {
       constexpr int R = decltype(ring_c)::value;
       const int k_slab = slab_at(t + 4), v_slab = slab_at(t + 2);
@@ -207,8 +216,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
           s_cur[r] = (e >= a && e <= z) || e < y ? s_cur[r] : -INFINITY;
         }
       }
-      // (where no row sees the slab its weights are zero, and V is not touched; there is no branch around them, which would cost registers that are not there)
-      raise();
+      // (Where no row sees the slab its weights are zero, and V is not touched.  A branch around the products costs registers that are not there: what was spilled came back behind
+      // the copies in flight, 4100 cycles a step instead of 1600; H24 S30720 window 128 315 us instead of 243.)
       const f32x16 s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
       weights();
       s_cur = s_nxt;
@@ -227,7 +236,6 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         if (i == 4) dma16(v_into + v_dma.wave_dst, v_src, v_dma.off[0]);
         if (i == 6) dma16(v_into + v_dma.wave_dst + 4 * kRowBytes, v_src, v_dma.off[1]);
       });
-      raise();
       const f32x16 s_nxt = scores(k_lds + ((R + 1) & 3) * kSlabBytes);
       weights();
       s_cur = s_nxt;
