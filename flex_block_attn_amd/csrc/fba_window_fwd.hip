@@ -9,9 +9,9 @@
 // A slab that all 32 rows of a wave see whole needs no mask, one that none of them sees no work; of a window's slabs only the first and the last two or so
 // are masked, by two compares for every score.
 //
-// Bound by issue: the matrix pipe is busy 49 % of the time and the VALU 45, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
+// Bound by issue: the matrix pipe is busy 50 % of the time and the VALU 41, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
 // time, with longer waits for copies none).  H24 S30720, window 1152 to both sides, 384 sinks: 1.07 ms, 0.99 TFLOP of visible pairs, 920 TFLOP/s; H24/6 S69120 window 1536, 128
-// sinks: 1.53 ms, 915 TFLOP/s, read from memory 0.48 GB; H24 S30720 window 128: 243 us, 0.95 GB.
+// sinks: 1.51 ms, 925 TFLOP/s, read from memory 0.47 GB; H24 S30720 window 128: 243 us, 0.95 GB.
 #include <type_traits>
 
 #include "fba_types.h"
