@@ -165,7 +165,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
         if (__builtin_amdgcn_ballot_w64((mx - m_run) * c > kLazy) != 0) {
-          const float m_new = fmaxf(m_run, max_halves(mx)), alpha = fast_exp2((m_run - m_new) * c);
+          // (of the rows that need it only, so that a row's result does not depend on its neighbours)
+          const float top = max_halves(mx), m_new = (top - m_run) * c > kLazy ? top : m_run, alpha = fast_exp2((m_run - m_new) * c);
           m_run = m_new;
           l_run *= alpha;
 #pragma unroll

@@ -184,7 +184,8 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         float mx = s_cur[0];
 #pragma unroll
         for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s_cur[r]);
-        const float m_new = fmaxf(m_run, max_halves(mx));
+        // (of the rows that need it only, so that a row's result does not depend on its neighbours)
+        const float top = max_halves(mx), m_new = max_halves(sum[0]) > kMostSum ? fmaxf(m_run, top) : m_run;
         const float alpha = fast_exp2((m_run - m_new) * c);
         m_run = m_new;
         l_run *= alpha;

@@ -181,12 +181,13 @@ def test_gradients_against_differences(gpu, causal):
         assert abs(difference - along) <= (off[1 + i] * d.abs()).sum() + 1e-5 * (1 + abs(difference))
 
 
-def test_masked_places(gpu):
+@pytest.mark.parametrize("H", [1, 80])  # tiles of 32 rows, of 128
+def test_masked_places(gpu, H):
     """Keys that a row does not see may hold the type's lowest value, infinities and no numbers in k; in v where no row of their neighbourhood sees them."""
     import flex_block_attn_amd as fba
 
     S, window, sinks = 512, 64, 4
-    q, k, v, _ = inputs(gpu, 1, 1, 1, S, S, torch.bfloat16, 4)
+    q, k, v, _ = inputs(gpu, 1, H, H, S, S, torch.bfloat16, 4)
     # rows 256.. see the sinks and keys from 193 on: what stands between is seen by rows below 160 + 64 only
     want = fba.window_attn_func(q, k, v, window, sinks=sinks)[:, :, 256:]
     for value in (torch.finfo(torch.bfloat16).min, math.inf, -math.inf, math.nan):
