@@ -21,6 +21,7 @@
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/accumulate_grad.h>
+#include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/function.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
@@ -754,8 +755,22 @@ void refuse_leaves_of_the_default_stream(const at::Tensor& q) {
   TORCH_CHECK(!capturing, "backward is captured while an earlier graph of the same leaves, made on the default stream, is alive: drop what holds that graph before the capture");
 }
 
-std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
-                                            const at::Tensor& stats, at::Tensor d_o, const Window& w) {
+// The gradients of a backward pass that autograd makes a graph of (create_graph): kernels know nothing of that graph, so that without this a loss that contains a gradient would
+// lose that term in silence.  They get a node that raises, between them and what they depend on: the operator's inputs and the gradient of o.
+void differentiable_once(std::vector<at::Tensor>& grads, const at::Tensor& d_o) {
+  torch::autograd::edge_list edges;
+  if (const auto node = torch::autograd::get_current_node())
+    for (const torch::autograd::Edge& edge : node->next_edges())
+      if (edge.is_valid()) edges.push_back(edge);
+  if (d_o.requires_grad()) edges.push_back(torch::autograd::impl::gradient_edge(d_o));
+  if (edges.empty()) return;
+  const auto raises = std::make_shared<torch::autograd::Error>("window_attn_func is differentiable once: its gradients have no derivatives", std::move(edges));
+  for (at::Tensor& t : grads) torch::autograd::create_gradient_edge(t, raises);
+}
+
+std::vector<at::Tensor> window_gradients(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
+                                         const at::Tensor& stats, at::Tensor d_o, const Window& w) {
+  const at::NoGradGuard no_grad;
   check_window_saved({given_q, k, v, o, low, stats}, d_o, w);
   const c10::DeviceGuard guard(given_q.device());
   refuse_leaves_of_the_default_stream(given_q);
@@ -783,6 +798,13 @@ std::vector<at::Tensor> run_window_backward(const at::Tensor& given_q, const at:
                     dv = strided(grads[2]);
   check(lib.fba_window_bwd(&sq, &sk, &sv, &so, &sl, &sd, stats.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
                            q.size(2), k.size(2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
+  return grads;
+}
+
+std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
+                                            const at::Tensor& stats, const at::Tensor& d_o, const Window& w) {
+  std::vector<at::Tensor> grads = window_gradients(q, k, v, o, low, stats, d_o, w);
+  if (at::GradMode::is_enabled()) differentiable_once(grads, d_o);
   return grads;
 }
 

@@ -70,9 +70,8 @@ class WindowAttnFunc(torch.autograd.Function):
         return o
 
     @staticmethod
-    @torch.autograd.function.once_differentiable
     def backward(ctx, do):
-        q, k, v, o, low, stats = ctx.saved_tensors
+        q, k, v, o, low, stats = ctx.saved_tensors  # (the native side sees to it that this is not differentiated again)
         grads = _lib.host().window_backward(q, k, v, _rows_dense(o), low, stats, do, *ctx.args)
         return (*(_typed_like(g, t) for g, t in zip(grads, (q, k, v))), None, None, None, None)
 
@@ -92,7 +91,7 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     Scores of keys that a row does not see may be anything; v has to be finite there, and for gradients q, k and the gradient of o too (a weight of zero times infinity is no
     number), padding excepted.
 
-    Returns o, shaped like q.  Differentiable in q, k and v, once.  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
+    Returns o, shaped like q.  Differentiable in q, k and v, once (differentiating a gradient raises).  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
     graph of the same leaves that was made on the default stream may be alive then (backward raises)."""
     o = _lib.host().window_attention(q, k, v, window, sinks, bool(causal), lengths)
     if o is not None:
