@@ -12,6 +12,8 @@ A step of a batch of sequences, which may be captured into a graph:
 `table`, int32 (batch, max_pages): the pages of every sequence, in order; which pages are free is the caller's to keep.  `lengths`, int32 (batch,): filled slots.  Both
 are read on the GPU: a length that is negative or beyond the table, or a page outside of the pool, answers NaN or a length of -1 for that sequence.  A page that a call
 writes to may be in one place of the table only.
+
+What a call writes to counts as changed in place: a backward pass that has saved it raises.
 """
 from dataclasses import dataclass
 from typing import Optional

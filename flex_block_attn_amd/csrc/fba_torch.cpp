@@ -923,6 +923,12 @@ bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
   return false;
 }
 
+// A call has written to these by raw pointer: what has saved one of them for backward has to notice, as after any operation in place.
+void written(std::initializer_list<const at::Tensor*> tensors) {
+  for (const at::Tensor* t : tensors)
+    if (t->defined() && !t->is_inference()) torch::autograd::impl::bump_version(*t);  // (what is made in inference mode has no version)
+}
+
 // The entry points of cache.py: nothing for arguments that do not fit, which Python then prepares or reports.
 c10::optional<at::Tensor> cache_attention(pybind11::handle q_, pybind11::handle k_, pybind11::handle v_, pybind11::handle weights_, pybind11::handle table_,
                                           pybind11::handle lengths_, pybind11::handle window_, pybind11::handle sinks_, bool accumulate) {
@@ -943,6 +949,7 @@ c10::optional<at::Tensor> cache_attention(pybind11::handle q_, pybind11::handle 
   SplitWorkspace ws(q, bytes);
   const fba_strided sq = strided(q), so = strided(o);
   check(lib.fba_cache_attn(&cache, &sq, &so, q.size(1), window, sinks, accumulate, type_of(q), ws.ptr(), bytes, current_stream(q)));
+  if (accumulate) written({&weights});
   return o;
 }
 
@@ -968,6 +975,7 @@ c10::optional<at::Tensor> cache_append(pybind11::handle cache_k_, pybind11::hand
   auto ints_of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; };
   check(lib.fba_cache_append(&cache, &sk, &sv, ints_of(counts), ints_of(first), given.defined() ? given.data_ptr<float>() : nullptr, k.size(2), out.data_ptr<int32_t>(),
                              current_stream(ck)));
+  written({&ck, &cv, &positions, &weights});
   return out;
 }
 
@@ -988,6 +996,7 @@ c10::optional<at::Tensor> cache_evict(pybind11::handle k_, pybind11::handle v_, 
   SplitWorkspace ws(k, bytes);
   at::Tensor out = at::empty_like(lengths);
   check(lib.fba_cache_evict(&cache, budget, recent, sinks, out.data_ptr<int32_t>(), ws.ptr(), bytes, current_stream(k)));
+  written({&k, &v, &positions, &weights});
   return out;
 }
 
