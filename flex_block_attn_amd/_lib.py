@@ -71,6 +71,7 @@ SIGNATURES = {
     "fba_window_fwd": (_c_i32, [_c_ptr] * 7 + [_c_i32] * 10 + [_c_ptr]),
     "fba_window_workspace_bytes": (_c_i64, [_c_i32] * 9),
     "fba_window_bwd": (_c_i32, [_c_ptr] * 12 + [_c_i64] + [_c_i32] * 10 + [_c_ptr]),
+    "fba_window_bwd_apart": (_c_i32, [_c_ptr] * 13 + [_c_i64] + [_c_i32] * 10 + [_c_ptr]),
     "fba_cache_append": (_c_i32, [_c_ptr] * 6 + [_c_i32] + [_c_ptr] * 2),
     "fba_cache_attn_workspace_bytes": (_c_i64, [_c_ptr] + [_c_i32] * 2),
     "fba_cache_attn": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 5 + [_c_ptr, _c_i64, _c_ptr]),
@@ -82,7 +83,7 @@ SIGNATURES = {
 }
 
 # fba_version() of the library these signatures describe (include/fba.h; bumped whenever an argument list changes)
-ABI_VERSION = 2012
+ABI_VERSION = 2013
 
 _lib = None
 _host = None

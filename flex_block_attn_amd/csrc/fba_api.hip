@@ -909,15 +909,16 @@ int take_strided(fba::Strided& to, const fba_strided* t, const char* name) {
   return FBA_OK;
 }
 
-int fill_window(fba::WindowParams& p, float* stats, const int32_t* lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim,
+// scratch: null for forward
+int fill_window(fba::WindowParams& p, float* lse, float* scratch, const int32_t* lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim,
                 int32_t window, int32_t sinks, int32_t causal, int32_t type) {
   if (head_dim != 128) return fail(FBA_ERR_INVALID, "head_dim must be 128, got %d", head_dim);
   if (type != FBA_BF16 && type != FBA_FP16) return fail(FBA_ERR_INVALID, "type must be FBA_BF16 or FBA_FP16, got %d", type);
   if (int rc = check_window(lengths != nullptr, B, Hq, Hkv, Sq, Skv, window, sinks)) return rc;
-  if (stats == nullptr) return fail(FBA_ERR_INVALID, "stats is null");
-  p.lse = stats;
-  p.lse_exact = stats + (int64_t)B * Hq * Sq;
-  p.neg_delta = p.lse_exact + (int64_t)B * Hq * Sq;
+  if (lse == nullptr) return fail(FBA_ERR_INVALID, "stats is null");
+  p.lse = lse;
+  p.lse_exact = scratch;
+  p.neg_delta = scratch == nullptr ? nullptr : scratch + (int64_t)B * Hq * Sq;
   p.lengths = lengths;
   p.B = B; p.Hq = Hq; p.Hkv = Hkv; p.Sq = Sq; p.Skv = Skv;
   p.window = window < (Sq > Skv ? Sq : Skv) ? window : (Sq > Skv ? Sq : Skv);  // no two positions are further apart
@@ -936,7 +937,7 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream) {
   fba::WindowParams p{};
-  if (int rc = fill_window(p, stats, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
+  if (int rc = fill_window(p, stats, nullptr, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
   if (int rc = take_strided(p.q, q, "q")) return rc;
   if (int rc = take_strided(p.k, k, "k")) return rc;
   if (int rc = take_strided(p.v, v, "v")) return rc;
@@ -950,9 +951,9 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
 
 int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t window, int32_t sinks, int32_t causal) {
   fba::WindowParams p{};
-  float stats;
+  float lse;
   const int32_t lengths = 0;
-  if (fill_window(p, &stats, has_lengths ? &lengths : nullptr, B, Hq, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
+  if (fill_window(p, &lse, nullptr, has_lengths ? &lengths : nullptr, B, Hq, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
   return fba::plan_window_dkdv(p, fba::device_compute_units());
 }
 
@@ -960,8 +961,19 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
                        const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream) {
+  if (stats == nullptr) return fail(FBA_ERR_INVALID, "stats is null");
+  // (numbers that are out of range are refused before the pointer is used)
+  float* const scratch = reinterpret_cast<float*>(reinterpret_cast<uintptr_t>(stats) + 4 * (uintptr_t)((int64_t)B * Hq) * (uintptr_t)Sq);
+  return fba_window_bwd_apart(q, k, v, o, o_low, d_o, stats, scratch, lengths, dq, dk, dv, ws, ws_bytes, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type, hip_stream);
+}
+
+int32_t fba_window_bwd_apart(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* o_low, const fba_strided* d_o,
+                             const float* lse, float* scratch, const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws,
+                             int64_t ws_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal,
+                             int32_t type, void* hip_stream) {
+  if (lse == nullptr || scratch == nullptr) return fail(FBA_ERR_INVALID, "lse or scratch is null");
   fba::WindowParams p{};
-  if (int rc = fill_window(p, stats, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
+  if (int rc = fill_window(p, const_cast<float*>(lse), scratch, lengths, B, Hq, Hkv, Sq, Skv, head_dim, window, sinks, causal, type)) return rc;
   if (int rc = take_strided(p.q, q, "q")) return rc;
   if (int rc = take_strided(p.k, k, "k")) return rc;
   if (int rc = take_strided(p.v, v, "v")) return rc;

@@ -45,7 +45,7 @@ constexpr int64_t kXcds = 8;
 #define FBA_FUNCTIONS(X)                                                                                                \
   X(fba_version) X(fba_last_error) X(fba_split_workspace_bytes) X(fba_lists_cut) X(fba_pair_slots_bounds) X(fba_tile_slots_bounds)        \
   X(fba_fwd) X(fba_fwd_tiled) X(fba_fwd_blocks) X(fba_fwd_blocks_use) X(fba_fwd_mask_copy) X(fba_fwd_takes_mask) X(fba_bwd_mask) X(fba_bwd_takes_mask) X(fba_bwd) X(fba_bwd_handover) X(fba_bwd_tiled_cut) X(fba_bwd_dense) \
-  X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd) \
+  X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd_apart) \
   X(fba_cache_append) X(fba_cache_attn_workspace_bytes) X(fba_cache_attn) X(fba_cache_evict_workspace_bytes) X(fba_cache_evict)
 
 struct Library {
@@ -703,21 +703,21 @@ struct Window : torch::CustomClassHolder {
 };
 int32_t type_of(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FBA_FP16 : FBA_BF16; }
 
-// -> o, statistics with room for those of backward and, where backward may come, what rounding o has left
+// -> o, its statistics and, where backward may come, what rounding o has left
 std::tuple<at::Tensor, at::Tensor, at::Tensor> run_window_forward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const Window& w, bool backward) {
   const c10::DeviceGuard guard(q.device());
   at::Tensor o = at::empty_like(q);
   if (!takes_strides(o)) o = at::empty(q.sizes(), q.options());
-  at::Tensor low = backward ? at::empty_like(o) : at::Tensor(), stats = at::empty({backward ? 3 : 1, q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
-  if (q.numel() == 0) return {o, stats, low};
+  at::Tensor low = backward ? at::empty_like(o) : at::Tensor(), lse = at::empty({q.size(0), q.size(1), q.size(2)}, q.options().dtype(at::kFloat));
+  if (q.numel() == 0) return {o, lse, low};
   if (k.numel() == 0) {  // there is nothing to see
     o.zero_();
-    return {o, stats, low};
+    return {o, lse, low};
   }
   const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = backward ? strided(low) : so;
-  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, backward ? &sl : nullptr, stats.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
+  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, backward ? &sl : nullptr, lse.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
                            w.sinks, w.causal, type_of(q), current_stream(q)));
-  return {o, stats, low};
+  return {o, lse, low};
 }
 
 // What a saved-tensor hook hands back is read by raw pointer.
@@ -731,7 +731,7 @@ void check_window_saved(std::initializer_list<at::Tensor> tensors, const at::Ten
     TORCH_CHECK_VALUE(i == 5 ? t.is_contiguous() : takes_strides(t), "saved tensors must come back as dense rows");
   }
   TORCH_CHECK_VALUE(q.sizes() == d_o.sizes() && saved[3].sizes() == d_o.sizes() && saved[4].sizes() == d_o.sizes() && k.sizes() == saved[2].sizes() &&
-                        saved[5].numel() == 3 * q.size(0) * q.size(1) * q.size(2) && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
+                        saved[5].numel() == q.size(0) * q.size(1) * q.size(2) && k.size(0) == q.size(0) && k.size(1) > 0 && q.size(1) % k.size(1) == 0 &&
                         (!w.lengths.defined() || (w.lengths.size(0) == q.size(0) && q.size(2) == k.size(2))),
                     "saved tensors must come back in their shapes");
 }
@@ -769,9 +769,9 @@ void differentiable_once(std::vector<at::Tensor>& grads, const at::Tensor& d_o) 
 }
 
 std::vector<at::Tensor> window_gradients(const at::Tensor& given_q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
-                                         const at::Tensor& stats, at::Tensor d_o, const Window& w) {
+                                         const at::Tensor& lse, at::Tensor d_o, const Window& w) {
   const at::NoGradGuard no_grad;
-  check_window_saved({given_q, k, v, o, low, stats}, d_o, w);
+  check_window_saved({given_q, k, v, o, low, lse}, d_o, w);
   const c10::DeviceGuard guard(given_q.device());
   refuse_leaves_of_the_default_stream(given_q);
   at::Tensor q = given_q;
@@ -794,16 +794,18 @@ std::vector<at::Tensor> window_gradients(const at::Tensor& given_q, const at::Te
   }
   const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
   SplitWorkspace ws(q, bytes);
+  // What dQ leaves for dK and dV is the pass's own: several of one forward may run at a time.
+  at::Tensor scratch = at::empty({2, q.size(0), q.size(1), q.size(2)}, lse.options());
   const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = strided(low), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
                     dv = strided(grads[2]);
-  check(lib.fba_window_bwd(&sq, &sk, &sv, &so, &sl, &sd, stats.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
+  check(lib.fba_window_bwd_apart(&sq, &sk, &sv, &so, &sl, &sd, lse.data_ptr<float>(), scratch.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
                            q.size(2), k.size(2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
   return grads;
 }
 
 std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
-                                            const at::Tensor& stats, const at::Tensor& d_o, const Window& w) {
-  std::vector<at::Tensor> grads = window_gradients(q, k, v, o, low, stats, d_o, w);
+                                            const at::Tensor& lse, const at::Tensor& d_o, const Window& w) {
+  std::vector<at::Tensor> grads = window_gradients(q, k, v, o, low, lse, d_o, w);
   if (at::GradMode::is_enabled()) differentiable_once(grads, d_o);
   return grads;
 }
@@ -811,8 +813,8 @@ std::vector<at::Tensor> run_window_backward(const at::Tensor& q, const at::Tenso
 struct WindowAttention : torch::autograd::Function<WindowAttention> {
   static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, c10::intrusive_ptr<Window> w) {
     if (w->lengths.defined()) w->lengths = w->lengths.clone();  // the caller may write to theirs before backward comes
-    auto [o, stats, low] = run_window_forward(q, k, v, *w, true);
-    ctx->save_for_backward({q, k, v, o, low, stats});
+    auto [o, lse, low] = run_window_forward(q, k, v, *w, true);
+    ctx->save_for_backward({q, k, v, o, low, lse});
     ctx->saved_data["w"] = c10::IValue::make_capsule(std::move(w));
     return o;
   }
@@ -877,8 +879,8 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> window_forward(const at::Tensor& 
   return run_window_forward(q, k, v, window_of(window, sinks, causal, lengths), true);
 }
 std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k, const at::Tensor& v, const at::Tensor& o, const at::Tensor& low,
-                                        const at::Tensor& stats, const at::Tensor& d_o, int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
-  return run_window_backward(q, k, v, o, low, stats, d_o, window_of(window, sinks, causal, lengths));
+                                        const at::Tensor& lse, const at::Tensor& d_o, int64_t window, int64_t sinks, bool causal, const c10::optional<at::Tensor>& lengths) {
+  return run_window_backward(q, k, v, o, low, lse, d_o, window_of(window, sinks, causal, lengths));
 }
 
 // ---------------------------------------------------------------------------------------------------------------------

@@ -62,17 +62,17 @@ class WindowAttnFunc(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, causal, lengths):
         q, k, v = (_rows_dense(t) for t in (q, k, v))
-        o, stats, low = _lib.host().window_forward(q, k, v, window, sinks, causal, lengths)
+        o, lse, low = _lib.host().window_forward(q, k, v, window, sinks, causal, lengths)
         o = _typed_like(o, q)
-        ctx.save_for_backward(q, k, v, o, low, stats)
+        ctx.save_for_backward(q, k, v, o, low, lse)
         # the caller may write to their lengths before backward comes
         ctx.args = (window, sinks, causal, None if lengths is None else lengths.clone())
         return o
 
     @staticmethod
     def backward(ctx, do):
-        q, k, v, o, low, stats = ctx.saved_tensors  # (the native side sees to it that this is not differentiated again)
-        grads = _lib.host().window_backward(q, k, v, _rows_dense(o), low, stats, do, *ctx.args)
+        q, k, v, o, low, lse = ctx.saved_tensors  # (the native side sees to it that this is not differentiated again)
+        grads = _lib.host().window_backward(q, k, v, _rows_dense(o), low, lse, do, *ctx.args)
         return (*(_typed_like(g, t) for g, t in zip(grads, (q, k, v))), None, None, None, None)
 
 

@@ -36,7 +36,7 @@ extern "C" {
 
 /* Library version: major * 1000 + minor; the minor number goes up whenever an argument list in this header changes, so a
  * binding can refuse a library built from another header (flex_block_attn_amd/_lib.py does). */
-#define FBA_VERSION 2012
+#define FBA_VERSION 2013
 int32_t fba_version(void);
 
 /* Message for the last non-OK return on the calling thread ("" if none). The pointer stays valid until the next
@@ -381,7 +381,8 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  *
  * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
  * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [3, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first
- * third (+inf for rows without a visible key), backward uses the others.
+ * third (+inf for rows without a visible key) and does not touch the others, which backward uses.  fba_window_bwd_apart takes the two apart: lse, [B, Hq, Sq] as forward has left
+ * it, is only read, so that several backward passes of one forward may run at a time; scratch is fp32 [2, B, Hq, Sq].
  * o_low, shaped like o, may be null: what rounding o has left, rounded.  Backward subtracts rowsum(d_o o) from every row, and takes o + o_low for it where it is there (dq of
  * a window of 350 keys: off by 0.0024 of its size instead of 0.0027, of which 0.0017 are its own rounding).
  * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes on the same GPU, 16-byte aligned, for partial sums of dk and dv (0 bytes: may be null), and d_o with the row
@@ -402,6 +403,10 @@ int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_str
                        const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws, int64_t ws_bytes, int32_t B,
                        int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal, int32_t type,
                        void* hip_stream);
+int32_t fba_window_bwd_apart(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* o_low, const fba_strided* d_o,
+                             const float* lse, float* scratch, const int32_t* lengths, const fba_strided* dq, const fba_strided* dk, const fba_strided* dv, void* ws,
+                             int64_t ws_bytes, int32_t B, int32_t Hq, int32_t Hkv, int32_t Sq, int32_t Skv, int32_t head_dim, int32_t window, int32_t sinks, int32_t causal,
+                             int32_t type, void* hip_stream);
 
 /*
  * A paged cache of keys and values, and attention of single new tokens over it (no counterpart in the reference).

@@ -43,3 +43,53 @@ def test_second_derivatives_are_refused(gpu, path):
     for t, y in zip(leaves, want):
         assert torch.equal(t.grad, y)
         t.grad = None
+
+
+@pytest.mark.parametrize("path", range(2), ids=["native", "python"])
+@pytest.mark.parametrize("H", [4, 140])  # tiles of 32 rows and keys, of 128
+def test_backward_leaves_saved_tensors_as_they_are(gpu, path, H):
+    leaves, do = _inputs(gpu, H, H)
+    saved = []
+
+    def keep(t):
+        saved.append((t, t.detach().clone()))
+        return t
+
+    with torch.autograd.graph.saved_tensors_hooks(keep, lambda t: t):
+        o = _paths()[path](*leaves)
+    torch.autograd.grad(o, leaves, do)
+    assert len(saved) >= 5
+    for t, before in saved:
+        assert torch.equal(t, before)
+
+
+def test_backward_passes_of_one_forward_at_the_same_time(gpu):
+    """Two captured backward passes that replay on two streams: each has statistics of its own."""
+    leaves, do = _inputs(gpu, 24, 8, 1500)
+    other = torch.randn(do.shape, generator=torch.Generator(device="cpu").manual_seed(9)).to(do)
+    f = _paths()[0]
+    want = []
+    for d in (do, other):
+        copies = [t.detach().clone().requires_grad_(True) for t in leaves]
+        want.append(torch.autograd.grad(f(*copies), copies, d))
+    torch.cuda.synchronize()
+    forward, graphs, outs = torch.cuda.CUDAGraph(), [], []
+    with torch.cuda.graph(forward):
+        o = f(*leaves)
+    for d in (do, other):
+        graphs.append(torch.cuda.CUDAGraph())
+        with torch.cuda.graph(graphs[-1]):
+            outs.append(torch.autograd.grad(o, leaves, d, retain_graph=True))
+    streams = [torch.cuda.Stream() for _ in graphs]
+    for _ in range(4):
+        for x in (x for out in outs for x in out):
+            x.fill_(float("nan"))
+        forward.replay()
+        for s, graph in zip(streams, graphs):
+            s.wait_stream(torch.cuda.current_stream())
+            with torch.cuda.stream(s):
+                graph.replay()
+        torch.cuda.synchronize()
+        for out, w in zip(outs, want):
+            for x, y in zip(out, w):
+                assert torch.equal(x, y)
