@@ -11,6 +11,7 @@
 
 #include <cstdlib>
 #include <numeric>
+#include <unordered_set>
 
 #include <ATen/ATen.h>
 #include <ATen/core/CachingHostAllocator.h>
@@ -20,9 +21,9 @@
 #include <c10/hip/HIPStream.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
-#include <torch/csrc/autograd/functions/accumulate_grad.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/function.h>
+#include <torch/csrc/autograd/graph_task.h>
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <torch/custom_class.h>
@@ -736,23 +737,39 @@ void check_window_saved(std::initializer_list<at::Tensor> tensors, const at::Ten
                     "saved tensors must come back in their shapes");
 }
 
-// A leaf's place in autograd's graph keeps the stream on which it was first used for as long as a graph with it lives.  While backward is captured, autograd makes that stream
-// wait for the capturing one.  Any other stream becomes part of the capture by that; the default one cannot, which breaks the capture and ends the process.
-void refuse_leaves_of_the_default_stream(const at::Tensor& q) {
+// A node of autograd's graph keeps the stream on which it was made, a leaf's place in it the one on which the leaf was first used, for as long as a graph with it lives.  While
+// backward is captured, autograd makes the stream of every node that it comes to wait for the capturing one.  Any other stream becomes part of the capture by that; the default one
+// cannot, which breaks the capture and ends the process.  So everything that this pass goes on to from here is looked at, through views, projections and what else is between the
+// operator and its leaves.
+void refuse_nodes_of_the_default_stream(const at::Tensor& q) {
   const auto node = torch::autograd::get_current_node();
   if (!node) return;
   const auto of_default = c10::hip::getDefaultHIPStream(q.device().index()).id();
   if (c10::hip::getCurrentHIPStream(q.device().index()).id() == of_default) return;
-  bool there = false;
-  for (const torch::autograd::Edge& edge : node->next_edges())
-    if (edge.function != nullptr && dynamic_cast<torch::autograd::AccumulateGrad*>(edge.function.get()) != nullptr) {
-      const auto stream = edge.function->stream();
-      there = there || (stream.has_value() && stream->id() == of_default);
+  {
+    pybind11::gil_scoped_acquire gil;
+    if (!pybind11::module_::import("torch").attr("cuda").attr("is_current_stream_capturing")().cast<bool>()) return;
+  }
+  const auto* const executed = torch::autograd::get_current_graph_task_exec_info();  // null or empty: everything
+  std::unordered_set<const torch::autograd::Node*> seen;
+  std::vector<torch::autograd::Node*> next{node.get()};
+  while (!next.empty()) {
+    torch::autograd::Node* const from = next.back();
+    next.pop_back();
+    for (const torch::autograd::Edge& edge : from->next_edges()) {
+      torch::autograd::Node* const to = edge.function.get();
+      if (to == nullptr) continue;
+      if (executed != nullptr && !executed->empty()) {
+        const auto at = executed->find(to);
+        if (at == executed->end() || !at->second.should_execute()) continue;
+      }
+      if (!seen.insert(to).second) continue;
+      const auto stream = to->stream();
+      TORCH_CHECK(!stream.has_value() || stream->id() != of_default,
+                  "backward is captured and comes to leaves or operations of an earlier graph, made on the default stream, that is alive: drop what holds that graph before the capture");
+      next.push_back(to);
     }
-  if (!there) return;
-  pybind11::gil_scoped_acquire gil;
-  const bool capturing = pybind11::module_::import("torch").attr("cuda").attr("is_current_stream_capturing")().cast<bool>();
-  TORCH_CHECK(!capturing, "backward is captured while an earlier graph of the same leaves, made on the default stream, is alive: drop what holds that graph before the capture");
+  }
 }
 
 // The gradients of a backward pass that autograd makes a graph of (create_graph): kernels know nothing of that graph, so that without this a loss that contains a gradient would
@@ -773,7 +790,7 @@ std::vector<at::Tensor> window_gradients(const at::Tensor& given_q, const at::Te
   const at::NoGradGuard no_grad;
   check_window_saved({given_q, k, v, o, low, lse}, d_o, w);
   const c10::DeviceGuard guard(given_q.device());
-  refuse_leaves_of_the_default_stream(given_q);
+  refuse_nodes_of_the_default_stream(given_q);
   at::Tensor q = given_q;
   std::vector<at::Tensor> grads;
   for (const at::Tensor* t : {&given_q, &k, &v}) {

@@ -92,7 +92,7 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     number), padding excepted.
 
     Returns o, shaped like q.  Differentiable in q, k and v, once (differentiating a gradient raises).  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
-    graph of the same leaves that was made on the default stream may be alive then (backward raises)."""
+    graph of leaves that the captured backward pass reaches, through views and projections too, may be alive then if it was made on the default stream (backward raises)."""
     o = _lib.host().window_attention(q, k, v, window, sinks, bool(causal), lengths)
     if o is not None:
         return o

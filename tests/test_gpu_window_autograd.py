@@ -93,3 +93,60 @@ def test_backward_passes_of_one_forward_at_the_same_time(gpu):
         for out, w in zip(outs, want):
             for x, y in zip(out, w):
                 assert torch.equal(x, y)
+
+
+def _leaf_and_way(gpu, kind):
+    """(the leaves, from them to q, k and v): through a transpose each, or all from one leaf by a product, a transpose and a split."""
+    g = torch.Generator(device="cpu").manual_seed(4)
+    new = lambda *shape: torch.randn(shape, generator=g).to(torch.bfloat16).to(gpu)
+    if kind == "transpose":
+        leaves = [new(1, 100, h, 128).requires_grad_(True) for h in (4, 2, 2)]
+        return leaves, lambda: [t.transpose(1, 2) for t in leaves]
+    x, weight = new(1, 100, 1, 128), new(1, 100, 8, 128).requires_grad_(True)
+    return [weight], lambda: (x * weight).transpose(1, 2).split((4, 2, 2), 1)
+
+
+@pytest.mark.parametrize("path", range(2), ids=["native", "python"])
+@pytest.mark.parametrize("kind", ["transpose", "product"])
+def test_capture_beside_an_earlier_graph_of_leaves_further_away(gpu, kind, path):
+    """The leaves are some steps away from the operator.  Refused while the earlier graph lives; what the pass does not come to is no reason."""
+    f = _paths()[path]
+    leaves, way = _leaf_and_way(gpu, kind)
+    do = torch.randn((1, 4, 100, 128), generator=torch.Generator(device="cpu").manual_seed(5)).to(torch.bfloat16).to(gpu)
+    earlier = f(*way())
+    want = [t.clone() for t in torch.autograd.grad(earlier, leaves, do, retain_graph=True)]
+    torch.cuda.synchronize()
+    with pytest.raises(RuntimeError, match="earlier graph"):
+        with torch.cuda.graph(torch.cuda.CUDAGraph()):
+            torch.autograd.grad(f(*way()), leaves, do)
+    for x, y in zip(torch.autograd.grad(earlier, leaves, do, retain_graph=True), want):
+        assert torch.equal(x, y)
+    # outside of a capture another stream is nobody's business
+    with torch.cuda.stream(torch.cuda.Stream()):
+        assert len(torch.autograd.grad(f(*way()), leaves, do)) == len(leaves)
+    torch.cuda.synchronize()
+    # a capture that stops at q, k and v does not come to the leaves
+    parts = [t.detach() for t in way()]
+    direct = torch.autograd.grad(f(*(t.requires_grad_(True) for t in parts)), parts, do)
+    torch.cuda.synchronize()
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        qkv = way()
+        out = torch.autograd.grad(f(*qkv), qkv, do)
+    graph.replay()
+    torch.cuda.synchronize()
+    for x, y in zip(out, direct):
+        assert torch.equal(x, y)
+    del earlier, qkv
+    graph = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(graph):
+        o = f(*way())
+        out = torch.autograd.grad(o, leaves, do)
+    del o
+    for _ in range(2):
+        for x in out:
+            x.fill_(float("nan"))
+        graph.replay()
+        torch.cuda.synchronize()
+        for x, y in zip(out, want):
+            assert torch.equal(x, y)
