@@ -277,7 +277,11 @@ __global__ __launch_bounds__(256) void window_sum_kernel(const WindowParams p) {
 //   to an item at least.  dQ, dK and dV, one item / several, H4/1 S2048 window 1024 (64 tiles of 32): 95 / 56 us, H8/2 S1024 window 512: 67 / 47, B2 H8/1 S1024, 400 to either
 //   side: 136 / 70.
 //   Outside (tiles with sinks): into as many as are about as long as the items inside, for the longest sequence there may be, of 16 slabs (tiles of 32 keys: 8) at least.
+//   No more items outside than twice what is on the GPU at once (two to a compute unit), and one for each tile: every part leaves 128 KiB of sums, which are written and read again.
+//   Backward, cut by length alone / once, twice, four and eight times what is on the GPU, H24 S30720: window 128, 4096 sinks 7296 / 5249, 5136, 5169, 5317 us (6.1 GB of sums / 0.2, 0.3, 0.4,
+//   0.7), 1024 sinks 2390 / 2007, 1944, 1948, 2063; 1152 to either side, 4096 sinks 7919 / 7478, 7511, 7513, 7659, and with 384, which twice leaves as they are, 3418 / 3485 with once.
 constexpr int kLeastSlabs = 16, kLeastSlabsFew = 8;
+constexpr int64_t kSinkRounds = 2;
 int64_t plan_window_dkdv(WindowParams& p, int compute_units) {
   p.key_tile = window_keys_few(p, compute_units) ? 32 : kWindowTile;
   p.tiles = (p.Skv + p.key_tile - 1) / p.key_tile;
@@ -301,6 +305,8 @@ int64_t plan_window_dkdv(WindowParams& p, int compute_units) {
     p.sink_tiles = 0;
   } else {
     parts = (outside + inside - 1) / inside;
+    const int64_t sink_tiles = (int64_t)p.B * p.Hkv * p.sink_tiles, most = (kSinkRounds * 2 * compute_units + sink_tiles - 1) / sink_tiles;
+    if (parts > most) parts = most;
     p.sink_parts = (int)(parts > 64 ? 64 : parts);
   }
   return part_place(p, (int64_t)p.B * p.Hkv, 0, false, 0) * part_floats(p) * 4;
