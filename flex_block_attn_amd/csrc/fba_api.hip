@@ -898,6 +898,23 @@ int check_window(int32_t has_lengths, int32_t B, int32_t Hq, int32_t Hkv, int32_
   return FBA_OK;
 }
 
+// A launch has fewer than 2^32 threads: work-groups of 256 that it may have.
+constexpr int64_t kMostWorkGroups = (1 << 24) - 1;
+
+// The launches of a pass: tiles of 128 rows (of 32 only where those are few) and, in backward, items and the sums of tiles with several, 32 work-groups to a tile.
+int check_window_launches(const fba::WindowParams& p, bool backward) {
+  constexpr int64_t kPad = 8 * 32;  // (a grid is filled up to whole rounds of its XCDs)
+  const int64_t row_tiles = (int64_t)p.B * p.Hq * ((p.Sq + fba::kWindowTile - 1) / fba::kWindowTile);
+  if (row_tiles > kMostWorkGroups - kPad)
+    return fail(FBA_ERR_UNSUPPORTED, "B * Hq * ceil(Sq / 128) is %lld, more than the %lld of a launch", (long long)row_tiles, (long long)(kMostWorkGroups - kPad));
+  if (!backward) return FBA_OK;
+  const int64_t bh = (int64_t)p.B * p.Hkv, tiles = (p.Skv + p.key_tile - 1) / p.key_tile, items = bh * (tiles * p.band_parts + (int64_t)p.sink_tiles * p.sink_parts);
+  const int64_t summed = bh * (p.band_parts > 1 ? tiles : p.sink_tiles) * (p.key_tile / 4);
+  if (items > kMostWorkGroups - kPad || summed > kMostWorkGroups)
+    return fail(FBA_ERR_UNSUPPORTED, "B * Hkv * ceil(Skv / 128) is %lld, of which %lld have sums of several parts: more than a launch takes", (long long)(bh * tiles), (long long)(bh * p.sink_tiles));
+  return FBA_OK;
+}
+
 int take_strided(fba::Strided& to, const fba_strided* t, const char* name) {
   if (t == nullptr || t->ptr == nullptr) return fail(FBA_ERR_INVALID, "%s is null", name);
   if (!aligned16(t->ptr)) return fail(FBA_ERR_INVALID, "%s is not 16-byte aligned", name);
@@ -944,6 +961,7 @@ int32_t fba_window_fwd(const fba_strided* q, const fba_strided* k, const fba_str
   if (int rc = take_strided(p.o, o, "o")) return rc;
   if (o_low != nullptr)
     if (int rc = take_strided(p.o_low, o_low, "o_low")) return rc;
+  if (int rc = check_window_launches(p, false)) return rc;
   const bool few = fba::window_takes_few(p, fba::device_compute_units(), false);
   hipError_t e = few ? fba::launch_window_few(p, type == FBA_FP16, false, (hipStream_t)hip_stream) : fba::launch_window_fwd(p, type == FBA_FP16, (hipStream_t)hip_stream);
   return e == hipSuccess ? FBA_OK : hip_fail(e, "window forward launch");
@@ -954,7 +972,8 @@ int64_t fba_window_workspace_bytes(int32_t has_lengths, int32_t B, int32_t Hq, i
   float lse;
   const int32_t lengths = 0;
   if (fill_window(p, &lse, nullptr, has_lengths ? &lengths : nullptr, B, Hq, Hkv, Sq, Skv, 128, window, sinks, causal, FBA_BF16)) return -1;
-  return fba::plan_window_dkdv(p, fba::device_compute_units());
+  const int64_t bytes = fba::plan_window_dkdv(p, fba::device_compute_units());
+  return check_window_launches(p, true) ? -1 : bytes;
 }
 
 int32_t fba_window_bwd(const fba_strided* q, const fba_strided* k, const fba_strided* v, const fba_strided* o, const fba_strided* o_low, const fba_strided* d_o, float* stats,
@@ -986,6 +1005,7 @@ int32_t fba_window_bwd_apart(const fba_strided* q, const fba_strided* k, const f
   if (int rc = take_strided(p.dv, dv, "dv")) return rc;
   if (p.d_o.row != p.q.row) return fail(FBA_ERR_UNSUPPORTED, "q and d_o must have the same row stride");
   const int64_t need = fba::plan_window_dkdv(p, fba::device_compute_units());
+  if (int rc = check_window_launches(p, true)) return rc;
   if (need > 0 && (ws == nullptr || !aligned16(ws) || ws_bytes < need))
     return fail(FBA_ERR_INVALID, "ws must be 16-byte aligned and hold %lld bytes (fba_window_workspace_bytes), got %lld", (long long)need, (long long)ws_bytes);
   p.parts = (float*)ws;
@@ -1038,7 +1058,7 @@ int take_attend(fba::AttendParams& p, const fba_cache* cache, int32_t heads, int
   p.heads = heads;
   fba::plan_cache_attend(p, fba::device_compute_units());
   const int64_t spans = (p.cache.slots() + 1023) / 1024;
-  if ((int64_t)p.slots * heads > 1LL << 30 || (accumulate && spans * cache->kv_heads * cache->batch > 1LL << 30))
+  if ((int64_t)p.slots * heads > 1LL << 30 || (int64_t)cache->batch * heads + (accumulate ? spans * cache->kv_heads * cache->batch : 0) > kMostWorkGroups)
     return fail(FBA_ERR_UNSUPPORTED, "batch (%d) and heads (%d) are too many for one call", cache->batch, heads);
   return FBA_OK;
 }
@@ -1074,7 +1094,7 @@ int32_t fba_cache_append(const fba_cache* cache, const fba_strided* k, const fba
   if (int rc = take_strided(p.v, v, "v")) return rc;
   if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
   if (lengths_out == cache->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
-  if ((int64_t)cache->batch * cache->kv_heads > 0x7fffffffLL) return fail(FBA_ERR_UNSUPPORTED, "batch * kv_heads is too large");
+  if (cache->batch > kMostWorkGroups - 8192) return fail(FBA_ERR_UNSUPPORTED, "batch (%d) is more than a launch takes", cache->batch);
   p.counts = counts;
   p.first = first;
   p.weights = weights;

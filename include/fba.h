@@ -387,7 +387,8 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  * a window of 350 keys: off by 0.0024 of its size instead of 0.0027, of which 0.0017 are its own rounding).
  * fba_window_bwd takes `ws`, fba_window_workspace_bytes(...) bytes on the same GPU, 16-byte aligned, for partial sums of dk and dv (0 bytes: may be null), and d_o with the row
  * stride of q (FBA_ERR_UNSUPPORTED otherwise).
- * Sq and Skv at most 2^28, B * Hq * Sq and B * Hkv * Skv below 2^29.
+ * Sq and Skv at most 2^28, B * Hq * Sq and B * Hkv * Skv below 2^29; tiles of 128 rows or keys, B * Hq * ceil(Sq / 128) and B * Hkv * ceil(Skv / 128), no more than a launch has
+ * work-groups, 2^24 - 257, and in backward of tiles with sinks, which leave partial sums, 2^19 - 1.
  */
 #define FBA_BF16 0
 #define FBA_FP16 1
@@ -427,6 +428,7 @@ int32_t fba_window_bwd_apart(const fba_strided* q, const fba_strided* k, const f
  *   `recent` ones (above the largest position - recent), then those with the largest weights, of equal ones the lower slot.  The i-th slot below `budget` that is freed
  *   receives the i-th kept one from `budget` on: row, position and weight; all other slots stay as they are.  lengths_out[b] = min(lengths[b], budget); -1, and nothing
  *   moved, for a wrong length or page.  NaN is the lowest weight.  recent + sinks <= budget.
+ * batch * heads, with accumulate and batch * kv_heads * ceil(slots of a sequence / 1024) added to it, may be 2^24 - 1 at most (work-groups of a launch).
  * Workspaces: as many bytes as the function of that name says, 16-byte aligned.  fba_cache_attn needs a multiple of the cache's scores with accumulate, little without.
  */
 typedef struct {
