@@ -702,6 +702,8 @@ struct Window : torch::CustomClassHolder {
   at::Tensor lengths;  // undefined: none
   const int32_t* lengths_ptr() const { return lengths.defined() ? lengths.data_ptr<int32_t>() : nullptr; }
 };
+// Sizes as the library takes them: what is beyond 32 bits (a tensor that repeats a row can be) stays beyond its limits.
+int32_t size32(const at::Tensor& t, int d) { return (int32_t)std::min<int64_t>(t.size(d), 0x7fffffff); }
 int32_t type_of(const at::Tensor& t) { return t.scalar_type() == at::kHalf ? FBA_FP16 : FBA_BF16; }
 
 // -> o, its statistics and, where backward may come, what rounding o has left
@@ -716,7 +718,7 @@ std::tuple<at::Tensor, at::Tensor, at::Tensor> run_window_forward(const at::Tens
     return {o, lse, low};
   }
   const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = backward ? strided(low) : so;
-  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, backward ? &sl : nullptr, lse.data_ptr<float>(), w.lengths_ptr(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), kHeadDim, w.window,
+  check(lib.fba_window_fwd(&sq, &sk, &sv, &so, backward ? &sl : nullptr, lse.data_ptr<float>(), w.lengths_ptr(), size32(q, 0), size32(q, 1), size32(k, 1), size32(q, 2), size32(k, 2), kHeadDim, w.window,
                            w.sinks, w.causal, type_of(q), current_stream(q)));
   return {o, lse, low};
 }
@@ -809,14 +811,14 @@ std::vector<at::Tensor> window_gradients(const at::Tensor& given_q, const at::Te
     d_o = d_o.contiguous();
     q = q.contiguous();
   }
-  const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), q.size(0), q.size(1), k.size(1), q.size(2), k.size(2), w.window, w.sinks, w.causal);
+  const int64_t bytes = lib.fba_window_workspace_bytes(w.lengths.defined(), size32(q, 0), size32(q, 1), size32(k, 1), size32(q, 2), size32(k, 2), w.window, w.sinks, w.causal);
   SplitWorkspace ws(q, bytes);
   // What dQ leaves for dK and dV is the pass's own: several of one forward may run at a time.
   at::Tensor scratch = at::empty({2, q.size(0), q.size(1), q.size(2)}, lse.options());
   const fba_strided sq = strided(q), sk = strided(k), sv = strided(v), so = strided(o), sl = strided(low), sd = strided(d_o), dq = strided(grads[0]), dk = strided(grads[1]),
                     dv = strided(grads[2]);
-  check(lib.fba_window_bwd_apart(&sq, &sk, &sv, &so, &sl, &sd, lse.data_ptr<float>(), scratch.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, q.size(0), q.size(1), k.size(1),
-                           q.size(2), k.size(2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
+  check(lib.fba_window_bwd_apart(&sq, &sk, &sv, &so, &sl, &sd, lse.data_ptr<float>(), scratch.data_ptr<float>(), w.lengths_ptr(), &dq, &dk, &dv, ws.ptr(), bytes, size32(q, 0), size32(q, 1), size32(k, 1),
+                           size32(q, 2), size32(k, 2), kHeadDim, w.window, w.sinks, w.causal, type_of(q), current_stream(q)));
   return grads;
 }
 
