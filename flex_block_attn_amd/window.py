@@ -57,10 +57,12 @@ def _rows_dense(t):
 
 
 class WindowAttnFunc(torch.autograd.Function):
-    """The operator as a Python autograd function: for arguments that need preparation, calls that are traced and tensor subclasses."""
+    """The operator as a Python autograd function: for arguments that need preparation or are refused, calls that are traced and tensor subclasses."""
 
     @staticmethod
     def forward(ctx, q, k, v, window, sinks, causal, lengths):
+        window, sinks = _check_window_args(q, k, v, window, sinks, lengths)
+        causal, lengths = bool(causal), None if lengths is None else lengths.contiguous()
         q, k, v = (_rows_dense(t) for t in (q, k, v))
         o, lse, low = _lib.host().window_forward(q, k, v, window, sinks, causal, lengths)
         o = _typed_like(o, q)
@@ -96,5 +98,4 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     o = _lib.host().window_attention(q, k, v, window, sinks, bool(causal), lengths)
     if o is not None:
         return o
-    window, sinks = _check_window_args(q, k, v, window, sinks, lengths)
-    return WindowAttnFunc.apply(q, k, v, window, sinks, bool(causal), None if lengths is None else lengths.contiguous())
+    return WindowAttnFunc.apply(q, k, v, window, sinks, causal, lengths)
