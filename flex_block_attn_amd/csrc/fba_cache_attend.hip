@@ -430,13 +430,15 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttendParams p, i
     if (slot < len) {
       const int page = cache.page_of(b, slot);
       f32x4 w = {0.f, 0.f, 0.f, 0.f};
+      bool any = false;  // a sequence without a number adds nothing, and does not touch pages that may be another's
       const float* from = p.scores + ((int64_t)b * p.heads + hkv * group + h0) * cache.slots() + slot;
       for (int q = 0; q < n; ++q) {
         const f32x4 s = *reinterpret_cast<const f32x4*>(from + q * cache.slots());
+        any = any || lse[q] == lse[q];
 #pragma unroll
         for (int e = 0; e < 4; ++e) w[e] += lse[q] == lse[q] ? fast_exp2(s[e] - lse[q]) : 0.f;  // (no number: a page or a query that is none)
       }
-      if (page >= 0) {  // four slots are on one page
+      if (page >= 0 && any) {  // four slots are on one page
         f32x4* to = reinterpret_cast<f32x4*>(cache.weights + cache.row_of(page, hkv, slot));
         f32x4 sum = *to;
 #pragma unroll
