@@ -91,7 +91,7 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     padding (not read, zeros in o and in the gradients); q and k then have one length.  A row that sees no key is zeros.
 
     Scores of keys that a row does not see may be anything; v has to be finite there, and for gradients q, k and the gradient of o too (a weight of zero times infinity is no
-    number), padding excepted.
+    number), padding excepted.  How far such a value reaches, up to 32 rows and 128 keys beside those that see it, is stated in include/fba.h.
 
     Returns o, shaped like q.  Differentiable in q, k and v, once (differentiating a gradient raises).  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
     graph of leaves that the captured backward pass reaches, through views and projections too, may be alive then if it was made on the default stream (backward raises)."""

@@ -376,8 +376,11 @@ int32_t fba_tile_permute(const void* x, void* out, int64_t n_seq, int32_t T, int
  * count as the nearest of the two), its other rows are padding and row i stands at i.  Key j is visible to row i when both are tokens and
  *   causal != 0:  j <= p and (p - j < window or j < sinks)        causal = 0:  |p - j| < window or j < sinks
  * o = softmax(q k^T / sqrt(128)) v over the visible keys; rows without any, and padding, are zeros, and so are their gradients.  Padding of q, k, v and d_o
- * is not read.  A value of v that is no number or infinite reaches the rows that see it, and others of its 32-row neighbourhood; in backward one of q, k or d_o does so in dk,
- * dq and dk, and dv and dk.
+ * is not read.
+ * Keys that a row does not see count with a weight of zero, and zero times what is infinite or no number is no number.  So such a value reaches, beside the rows and keys that see
+ * each other: one of v in forward, one of k in dq, the rows of the 32 (from a multiple of 32 on) of which one sees a key of its slab, the 32 keys from a multiple of 32 on; one of q
+ * in dk, one of d_o in dv, all keys of the 128 (from a multiple of 128 on) of which one is seen by a row of its slab, 32 rows from a multiple of 32 on or the last 32 - with sinks
+ * among these 128, therefore, from any row behind them.  One of k in forward, or of v in backward, goes no further than the rows that see it and the keys that these see.
  *
  * Tensors are given with their strides, in elements, multiples of 8 (the last dimension is dense): q, o, d_o, dq [B, Hq, Sq, 128], k, v, dk, dv
  * [B, Hkv, Skv, 128], all of one type; 16-byte aligned.  stats: fp32 [3, B, Hq, Sq]; forward leaves log2 of the softmax denominators in the first
