@@ -424,20 +424,21 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
 }
 
 // Which launches.  Rows: dQ where tiles of 128 rows leave half of the compute units idle and more; forward, which reads less, up to seven eighths of them, and up to all where the
-// keys of a row are not many.  Keys: up to half of the compute units, as long as a tile does not have the rows to be cut into several items.
-// Tiles of 128 / of 32, in us:
-//   window, forward          64          128         256         512        1024        2048        4096      dQ, dK, dV  128         512         2048
-//     32 tiles (H1 S4096)    13 / 7      15 / 8      18 / 8      23 / 10     30 / 14     44 / 20     68 / 31              31 / 23     50 / 35     95 / 54
-//    100 (B2 H2 S3136)       14 / 8      16 / 10     19 / 11     24 / 14     37 / 18     64 / 27                          37 / 33     54 / 45    119 / 85
-//    128 (B4 H4 S1024)       14 / 8      16 / 10     19 / 11     24 / 14     27 / 17                                      37 / 33     53 / 44
-//    200 (B2 H4 S3136)       15 / 12     17 / 16     20 / 19     25 / 23     38 / 31     65 / 38                          41 / 48     62 / 68    152 / 135
-//    256 (H4 S8192)          16 / 13     18 / 17     21 / 20     26 / 25     33 / 36     48 / 57     78 / 103             45 / 51     67 / 72    151 / 162
-//    384 (H6 S8192)          22 / 20     24 / 24     28 / 29     36 / 36     50 / 51     77 / 84    125 / 152             62 / 71     97 / 105   231 / 244
-//    512 (H8 S8192)          24 / 25     26 / 31     29 / 36     37 / 46     51 / 66     79 / 110   128 / 200             65 / 83    100 / 121   238 / 283
-//   keys, dQ, dK, dV  window 128         512         2048
-//     16 tiles (H4/1 S2048)  46 / 32     53 / 47    110 / 101
-//     32 (H4/1 S4096)        63 / 48     85 / 84    159 / 203
-//    100 (B2 H8/2 S3136)     86 / 64    133 / 110   221 / 272
+// keys of a row are not many.  Keys: up to an eighth of the compute units, and up to half of them as long as a tile does not have the rows to be cut into several items.
+// Tiles of 128 / of 32, in us (causal, no sinks; backward: dQ, dK and dV, replayed from a graph):
+//   window, forward            128         256         512         1024        2048        4096        backward  128         512         2048
+//      32 tiles (H1 S4096)     15 / 8      18 / 9      22 / 10     29 / 14     44 / 20     67 / 32               35 / 27     54 / 40     98 / 60
+//     100 (B2 H2 S3136)        15 / 10     18 / 11     23 / 14     35 / 18     61 / 26                           43 / 39     60 / 52     123 / 89
+//     128 (B4 H4 S1024)        15 / 10     18 / 11     23 / 14     25 / 16                                       43 / 38     59 / 49
+//     200 (B2 H4 S3136)        16 / 15     18 / 18     23 / 22     35 / 30     62 / 38                           46 / 53     68 / 75     158 / 139
+//     256 (H4 S8192)           16 / 16     19 / 19     24 / 24     31 / 35     46 / 57     75 / 104              51 / 58     75 / 79     160 / 171
+//     384 (H6 S8192)           22 / 23     26 / 27     33 / 35     47 / 50     74 / 84     120 / 152             67 / 76     102 / 112   239 / 254
+//     512 (H8 S8192)           25 / 31     29 / 36     36 / 46     49 / 66     76 / 110    121 / 200             71 / 90     107 / 126   243 / 288
+//   keys, backward              window 128  512         1024        2048
+//      16 tiles (H4/1 S2048)   52 / 35     55 / 46     61 / 53     81 / 62
+//      20 (H8/1 S2560)         64 / 48     77 / 69     106 / 92    165 / 134
+//      32 (H4/1 S4096)         59 / 42     66 / 58     76 / 74     100 / 98
+//     100 (B2 H8/2 S3136)      79 / 60     110 / 103   148 / 154   216 / 242
 bool window_takes_few(const WindowParams& p, int compute_units, bool backward) {
   const int64_t tiles = (int64_t)p.B * p.Hq * ((p.Sq + kWindowTile - 1) / kWindowTile);
   if (2 * tiles <= compute_units) return true;
