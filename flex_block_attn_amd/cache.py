@@ -170,7 +170,7 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
     window = _NO_WINDOW if window is None else _whole(window, "window", 1)
     sinks = _whole(sinks, "sinks", 0)
     _no_gradients(**{"q": q, "cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights})
-    return _answered(_lib.host().cache_attention(_rows_dense(q), *given, window, sinks, bool(accumulate)))
+    return _answered(_lib.host().cache_attention(_rows_dense(q), *given, None if window == _NO_WINDOW else window, sinks, bool(accumulate)))
 
 
 def cache_evict(cache, table, lengths, budget, recent=0, sinks=0):

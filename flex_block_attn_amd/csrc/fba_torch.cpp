@@ -956,9 +956,10 @@ c10::optional<at::Tensor> cache_attention(pybind11::handle q_, pybind11::handle 
   int64_t window, sinks;
   if (!plain({q_, k_, v_, weights_, table_, lengths_}) || !int32_of(window_, kNoWindow, &window) || !int32_of(sinks_, -1, &sinks) || window < 1 || sinks < 0) return c10::nullopt;
   const at::Tensor q = tensor_of(q_), k = tensor_of(k_), v = tensor_of(v_), weights = tensor_of(weights_), table = tensor_of(table_), lengths = tensor_of(lengths_);
+  const bool windowed = !window_.is_none();
   pybind11::gil_scoped_release no_gil;
   fba_cache cache;
-  if (!cache_of(k, v, at::Tensor(), weights, table, lengths, &cache) || (accumulate && (!weights.defined() || window < kNoWindow))) return c10::nullopt;
+  if (!cache_of(k, v, at::Tensor(), weights, table, lengths, &cache) || (accumulate && (!weights.defined() || windowed))) return c10::nullopt;
   if (!q.defined() || q.device() != k.device() || q.scalar_type() != k.scalar_type() || !takes_strides(q) || q.size(0) != cache.batch || q.size(2) != 1 || q.numel() == 0 ||
       q.size(1) % cache.kv_heads != 0 || q.size(1) > 65535)
     return c10::nullopt;
