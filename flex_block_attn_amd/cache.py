@@ -128,6 +128,8 @@ def cache_append(cache, table, lengths, k, v, counts=None, positions=None, weigh
             raise TypeError(f"{name} must have the cache's type and device ({cache.k.dtype}, {cache.k.device}), got {t.dtype}, {t.device}")
         if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != kv_heads or t.shape[3] != HEAD_DIM or t.shape != k.shape:
             raise ValueError(f"k and v must have shape ({batch}, {kv_heads}, tokens, {HEAD_DIM}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.shape[2] > 1 << 28:
+        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a call may append 2^28 tokens at most, got {k.shape[2]}")
     _check_ints(counts, "counts", table)
     _check_ints(positions, "positions", table)
     if positions is not None and cache.positions is None:

@@ -25,3 +25,14 @@ def test_accumulate_takes_no_window_however_wide(gpu, window):
         assert int(fba.cache_attn_func(q, cache, table, n, window=window).count_nonzero()) == 0
         assert int(fba.cache_attn_func(q, cache, table, n, accumulate=True).count_nonzero()) == 0
     assert float(cache.weights.sum()) == pytest.approx(2 * 2 * 2, abs=1e-5)  # two calls, two kv heads of two query heads
+
+
+def test_more_tokens_than_a_call_may_append(gpu):
+    """A tensor that repeats one row can be as long; the error says what is wrong with it."""
+    import flex_block_attn_amd as fba
+    from flex_block_attn_amd import _lib
+
+    cache, table, n = _cache(gpu)
+    rows = torch.zeros((1, 2, 1, 128), dtype=torch.bfloat16, device=gpu).expand(1, 2, (1 << 28) + 1, 128)
+    with pytest.raises(_lib.FbaError, match="2\\^28 tokens"):
+        fba.cache_append(cache, table, n, rows, rows)
