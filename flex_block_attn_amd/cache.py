@@ -13,6 +13,9 @@ A step of a batch of sequences, which may be captured into a graph:
 are read on the GPU: a length that is negative or beyond the table, or a page outside of the pool, answers NaN or a length of -1 for that sequence.  A page that a call
 writes to may be in one place of the table only.
 
+Weights come from `cache_attn_func(accumulate=True)`, or from the caller: a prompt's rows have those that `cache_append` is given, zeros otherwise (`window_attn_func` leaves none).  An
+eviction right after a prompt without any goes by `sinks`, `recent` and, among equals, the lower slot.
+
 What a call writes to counts as changed in place: a backward pass that has saved it raises.
 """
 from dataclasses import dataclass
@@ -152,7 +155,7 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
     `window` of them and the first `sinks`.  (Slots are in the order of tokens as long as nothing has been evicted.)
 
     q: (batch, heads, 1, 128) of the cache's type, heads a multiple of kv_heads.  accumulate=True adds to cache.weights what softmax gave every slot, summed over the query
-    heads of a kv head; not with a window.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
+    heads of a kv head; not with a window, and with a workspace of 4 * batch * heads bytes for every slot that the table has room for, filled or not.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
     given = (cache.k, cache.v, cache.weights, table, lengths) if isinstance(cache, PagedCache) else None
     out = None if given is None else _lib.host().cache_attention(q, *given, window, sinks, bool(accumulate))
     if out is not None:
@@ -178,7 +181,7 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
 def cache_evict(cache, table, lengths, budget, recent=0, sinks=0):
     """Brings every sequence of more than `budget` slots down to that, every kv head for itself: tokens at positions below `sinks` and the `recent` last ones stay, then those
     with the largest weights (of equal ones the lower slot; NaN is the lowest).  Slots that are freed below the budget take the kept ones from behind it, in order: rows,
-    positions and weights; slots are in no order of tokens then.
+    positions and weights; slots are in no order of tokens then.  batch * kv_heads may be 65535 at most.
 
     Returns the new lengths, a tensor of its own: min(lengths, budget), and -1, with nothing moved, where a length or page makes no sense."""
     given = (cache.k, cache.v, cache.positions, cache.weights, table, lengths) if isinstance(cache, PagedCache) else None

@@ -9,7 +9,7 @@
 //   S^T[slot, q] = K Q^T,  P^T = exp2(c S^T - c m[q]),  O^T[d, q] += V^T P^T
 // P goes into the second product in two parts of the type, rounded and what rounding left: the matrix pipe has time to spare here, and what is lost of P then is
 // below what fp32 sums lose.  Sequences in several shares leave sums, which a second kernel joins.
-// That case moves 848 MB at 6.4 TB/s; 8 streams of 115200 slots through a window of 8192 and 128 sinks, 16 heads on 4: 136 MB in 27 us; one of 768 slots: 6.7 us, and 3 to join.
+// That case moves 848 MB at 6.4 TB/s; 8 streams of 115200 slots through a window of 8192 and 128 sinks, 16 heads on 4: 136 MB in 27 us; one of 768 slots: 6 us, and 3 to join.
 //
 // Accumulated weights need the denominator of all chunks: the first kernel leaves its scores (4 bytes for every head and slot, against 512 bytes of K and V), and the
 // second adds up exp2(score - log2 denominator) over the heads of the group.

@@ -1,4 +1,4 @@
-// Attention under a sliding window with sinks: parameters, launchers and the geometry that host and kernels share.
+// Attention under a sliding window with sinks: parameters, launchers, and what host and kernels say alike about rows, keys and work items.
 //
 // Query row i stands at position p = i + Skv - Sq (with lengths, where Sq = Skv: at i).  Key j is visible to it when both are within the
 // sequence's length and

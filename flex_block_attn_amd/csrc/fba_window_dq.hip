@@ -3,11 +3,11 @@
 // With P = exp(S/sqrt(128) - LSE), delta = rowsum(dO o O), dP = dO V^T, dS = P o (dP - delta) / sqrt(128):
 //   dQ = dS K,  dV = P^T dO,  dK = dS^T Q
 // Two kernels, each of which owns the rows it writes: this one walks the keys of 128 query rows (and works delta out, of which it has both factors at hand), the one in
-// fba_window_dkdv.hip the query rows of 128 keys.  Both form S and dP anew from what they have in LDS, 14 products where 10 are needed, and write nothing in between but
+// fba_window_dkdv.hip the query rows of 128 keys.  Both form S and dP anew from what they have in LDS, seven products where five are needed, and write nothing in between but
 // statistics: dS would be 2 bytes for every row and key of its window.
 //
-// Bound by issue and by the fetches from LDS (three a product's operand, by 128 rows' four waves each): the matrix pipe is busy 53 % of the time.  H24 S30720, window 1152 to both
-// sides, 384 sinks: 1.45 ms, 1.49 TFLOP of visible pairs in three products, 1.03 PFLOP/s.
+// Bound by issue and by the fetches from LDS (three a product's operand, by 128 rows' four waves each): the matrix pipe is busy 52 % of the time.  H24 S30720, window 1152 to both
+// sides, 384 sinks: 1.49 ms, 1.49 TFLOP of visible pairs in three products, 1.00 PFLOP/s.
 #include <type_traits>
 
 #include "fba_types.h"

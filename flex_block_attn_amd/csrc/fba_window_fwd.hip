@@ -9,9 +9,9 @@
 // A slab that all 32 rows of a wave see whole needs no mask, one that none of them sees no work; of a window's slabs only the first and the last two or so
 // are masked, by two compares for every score.
 //
-// Bound by issue: the matrix pipe is busy 50 % of the time and the VALU 41, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
-// time, with longer waits for copies none).  H24 S30720, window 1152 to both sides, 384 sinks: 1.07 ms, 0.99 TFLOP of visible pairs, 920 TFLOP/s; H24/6 S69120 window 1536, 128
-// sinks: 1.51 ms, 925 TFLOP/s, read from memory 0.47 GB; H24 S30720 window 128: 243 us, 0.95 GB.
+// Bound by issue: the matrix pipe is busy 50 % of the time and the VALU 42, and two waves on a SIMD cover little more of each other than that (without the barriers 5 % less
+// time, with longer waits for copies none).  H24 S30720, window 1152 to both sides, 384 sinks: 1.06 ms, 0.99 TFLOP of visible pairs, 930 TFLOP/s; H24/6 S69120 window 1536, 128
+// sinks: 1.52 ms, 920 TFLOP/s, read from memory 0.47 GB; H24 S30720 window 128: 243 us, 0.95 GB.
 #include <type_traits>
 
 #include "fba_types.h"
@@ -159,7 +159,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         }
     };
     // p_prev := P_t against the rows' reference m.  Where they add up to more than kMostSum, m has fallen behind: it is raised, with what has been summed, and they are formed anew.
-    // (The sum is there anyway; the maximum in front of every step costs H24/6 S69120 window 1536 1585 us instead of 1550.)
+    // (The sum is there anyway; the maximum in front of every step costs H24/6 S69120 window 1536 1585 us instead of 1550, both on a card slower than that of the figures above.)
     auto weights = [&]() {
       const typename Elem<T>::x2 one2 = {(T)1.f, (T)1.f};
       float sum[2];

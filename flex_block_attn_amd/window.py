@@ -93,7 +93,9 @@ def window_attn_func(q, k, v, window, sinks=0, causal=True, lengths=None):
     Scores of keys that a row does not see may be anything; v has to be finite there, and for gradients q, k and the gradient of o too (a weight of zero times infinity is no
     number), padding excepted.  How far such a value reaches, up to 32 rows and 128 keys beside those that see it, is stated in include/fba.h.
 
-    Returns o, shaped like q.  Differentiable in q, k and v, once (differentiating a gradient raises).  Gradients in fp16 need the usual scaling of the loss.  A step may be captured into a graph; no earlier
+    Returns o, shaped like q.  Differentiable in q, k and v, once (differentiating a gradient raises).  Gradients in fp16 need the usual scaling of the
+    loss: P and dS, before its factor 1 / sqrt(128), are rounded to the inputs' type, where fp16 ends at 65504 and has fewer digits below 2^-14, for rows whose weight is spread over more
+    than some 16000 keys therefore.  A step may be captured into a graph; no earlier
     graph of leaves that the captured backward pass reaches, through views and projections too, may be alive then if it was made on the default stream (backward raises)."""
     o = _lib.host().window_attention(q, k, v, window, sinks, bool(causal), lengths)
     if o is not None:

@@ -432,7 +432,8 @@ int32_t fba_window_bwd_apart(const fba_strided* q, const fba_strided* k, const f
  *   receives the i-th kept one from `budget` on: row, position and weight; all other slots stay as they are.  lengths_out[b] = min(lengths[b], budget); -1, and nothing
  *   moved, for a wrong length or page.  NaN is the lowest weight.  recent + sinks <= budget.
  * batch * heads, with accumulate and batch * kv_heads * ceil(slots of a sequence / 1024) added to it, may be 2^24 - 1 at most (work-groups of a launch).
- * Workspaces: as many bytes as the function of that name says, 16-byte aligned.  fba_cache_attn needs a multiple of the cache's scores with accumulate, little without.
+ * Workspaces: as many bytes as the function of that name says, 16-byte aligned.  fba_cache_attn needs, with accumulate, 4 * batch * heads bytes for every slot
+ * that the table has room for, filled or not, and little without.  fba_cache_evict: batch * kv_heads may be 65535 at most.
  */
 typedef struct {
   void* k;
