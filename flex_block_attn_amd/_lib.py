@@ -77,13 +77,22 @@ SIGNATURES = {
     "fba_cache_attn": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 5 + [_c_ptr, _c_i64, _c_ptr]),
     "fba_cache_evict_workspace_bytes": (_c_i64, [_c_ptr, _c_i32]),
     "fba_cache_evict": (_c_i32, [_c_ptr] + [_c_i32] * 3 + [_c_ptr] * 2 + [_c_i64, _c_ptr]),
+    "fba_rotary": (_c_i32, [_c_ptr] * 5 + [_c_i32] * 7 + [_c_ptr]),
+    "fba_cache_append_rotary": (_c_i32, [_c_ptr] * 5 + [_c_i32] + [_c_ptr] * 4 + [_c_i32] * 2 + [_c_ptr] * 2),
+    "fba_cache_read": (_c_i32, [_c_ptr] + [_c_i32] * 2 + [_c_ptr] * 2 + [_c_i32] + [_c_ptr]),
+    "fba_cache4_append": (_c_i32, [_c_ptr] * 5 + [_c_i32] + [_c_ptr] * 4 + [_c_i32] * 2 + [_c_ptr] * 2),
+    "fba_cache4_attn_workspace_bytes": (_c_i64, [_c_ptr] + [_c_i32] * 2),
+    "fba_cache4_attn": (_c_i32, [_c_ptr] * 3 + [_c_i32] * 5 + [_c_ptr, _c_i64, _c_ptr]),
+    "fba_cache4_evict_workspace_bytes": (_c_i64, [_c_ptr, _c_i32]),
+    "fba_cache4_evict": (_c_i32, [_c_ptr] + [_c_i32] * 3 + [_c_ptr] * 2 + [_c_i64, _c_ptr]),
+    "fba_cache4_read": (_c_i32, [_c_ptr] + [_c_i32] * 2 + [_c_ptr] * 2 + [_c_i32] + [_c_ptr]),
     "fba_bwd_stats": (_c_i32, [_c_ptr, _c_ptr, _c_ptr, _c_ptr, _c_i64, _c_i32, _c_ptr]),
     "fba_bwd_dq": (_c_i32, [_c_ptr] * 8 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),
     "fba_bwd_dkdv": (_c_i32, [_c_ptr] * 9 + [_c_i64] + [_c_i32] * 8 + [_c_ptr, _c_i64, _c_ptr]),
 }
 
 # fba_version() of the library these signatures describe (include/fba.h; bumped whenever an argument list changes)
-ABI_VERSION = 2013
+ABI_VERSION = 2014
 
 _lib = None
 _host = None

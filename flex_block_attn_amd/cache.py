@@ -16,6 +16,15 @@ writes to may be in one place of the table only.
 Weights come from `cache_attn_func(accumulate=True)`, or from the caller: a prompt's rows have those that `cache_append` is given, zeros otherwise (`window_attn_func` leaves none).  An
 eviction right after a prompt without any goes by `sinks`, `recent` and, among equals, the lower slot.
 
+Keys that carry their positions by rotation (positions.py) are turned on the way in, and the step's q beside them:
+
+    lengths, q = cache_append_rotary(cache, table, lengths, k, v, turn, q=q)
+
+A prompt's next chunk sees what is cached through `cache_read`, which hands rows back as dense tensors, for `window_attn_func`.
+
+The pool may hold 4 bits to a value instead of 16 (`paged_cache(bits=4)`): 136 bytes instead of 512 for a slot's key and value.  All calls take either; attention is then over what the 4
+bits stand for, which is exact in the pool's type.  The kernels are csrc/fba_cache_rotary.hip and csrc/fba_cache_attend4.hip.
+
 What a call writes to counts as changed in place: a backward pass that has saved it raises.
 """
 from dataclasses import dataclass
@@ -25,6 +34,7 @@ import torch
 
 from . import _lib
 from .interface import HEAD_DIM, _require_device
+from .positions import Rotary, _check_coordinates, _check_rotary
 from .window import _NO_WINDOW, _TYPES, _rows_dense, _whole
 
 
@@ -39,17 +49,37 @@ class PagedCache:
     weights: Optional[torch.Tensor] = None    # (pages, kv_heads, page_size) float32
 
 
-def paged_cache(pages, kv_heads, page_size=64, dtype=torch.bfloat16, device="cuda", evicting=False):
-    """An empty pool, with positions and weights if it is to be evicted from.  Its memory is not initialised: no call reads a slot that was not filled."""
+@dataclass
+class PagedCache4:
+    """The pool of pages in 4 bits: value 2j of a row in the low half of byte j, 2j + 1 in the high one, 0, 0.5, 1, 1.5, 2, 3, 4 or 6 with a sign (the fourth bit), times 2^(scale - 127),
+    a scale for every 32 values; 255: they are no numbers.  What is appended goes to the nearest, ties to the even code; 2^(scale - 127) is a quarter of the power of two below the
+    largest of the 32, or a half from 1.75 times that power on.  So a value v is off by a quarter of 2^(scale - 127) or of |v| at most (and what is beyond 7 * 2^125, in fp16 7 * 2^13,
+    becomes 6 * 2^125, 6 * 2^13); an infinity takes its 32 with it."""
+
+    k: torch.Tensor  # (pages, kv_heads, page_size, 64) uint8, contiguous; page_size a power of two, 16 at least
+    v: torch.Tensor
+    k_scales: torch.Tensor  # (pages, kv_heads, page_size, 4) uint8
+    v_scales: torch.Tensor
+    dtype: torch.dtype = torch.bfloat16       # of what it stands for, and of q, k, v and o; fixed for a pool
+    positions: Optional[torch.Tensor] = None  # (pages, kv_heads, page_size) int32
+    weights: Optional[torch.Tensor] = None    # (pages, kv_heads, page_size) float32
+
+
+def paged_cache(pages, kv_heads, page_size=64, dtype=torch.bfloat16, device="cuda", evicting=False, bits=16):
+    """An empty pool, with positions and weights if it is to be evicted from: a PagedCache, or with bits=4 a PagedCache4.  Its memory is not initialised: no call reads a slot that was
+    not filled."""
     page_size = _page_size(_whole(page_size, "page_size", 16))
     pages, kv_heads = _whole(pages, "pages", 1), _whole(kv_heads, "kv_heads", 1)
     if dtype not in _TYPES:
         raise TypeError(f"dtype must be bfloat16 or float16, got {dtype}")
-    k, v = (torch.empty((pages, kv_heads, page_size, HEAD_DIM), dtype=dtype, device=device) for _ in range(2))
+    if bits not in (4, 16):
+        raise ValueError(f"bits must be 4 or 16, got {bits}")
+    pool = (pages, kv_heads, page_size)
+    rows = lambda n, of: [torch.empty((*pool, n), dtype=of, device=device) for _ in range(2)]
+    k, v = rows(HEAD_DIM, dtype) if bits == 16 else rows(HEAD_DIM // 2, torch.uint8)
     _require_device(k, "the cache")
-    if not evicting:
-        return PagedCache(k, v)
-    return PagedCache(k, v, torch.empty(k.shape[:3], dtype=torch.int32, device=device), torch.empty(k.shape[:3], dtype=torch.float32, device=device))
+    slots = (torch.empty(pool, dtype=torch.int32, device=device), torch.empty(pool, dtype=torch.float32, device=device)) if evicting else ()
+    return PagedCache(k, v, *slots) if bits == 16 else PagedCache4(k, v, *rows(HEAD_DIM // 32, torch.uint8), dtype, *slots)
 
 
 def _page_size(n):
@@ -58,14 +88,25 @@ def _page_size(n):
     return n
 
 
+def _given(cache, table, lengths):
+    """The tensors of a call as the native side takes them, and the type of the cache's values; None for what is no cache."""
+    if isinstance(cache, PagedCache):
+        return (cache.k, cache.v, None, None, cache.positions, cache.weights, table, lengths, getattr(cache.k, "dtype", None))
+    if isinstance(cache, PagedCache4):
+        return (cache.k, cache.v, cache.k_scales, cache.v_scales, cache.positions, cache.weights, table, lengths, cache.dtype)
+    return None
+
+
 def _check_cache(cache, table, lengths):
-    """Raises for everything that the kernels do not take."""
-    if not isinstance(cache, PagedCache):
-        raise TypeError(f"cache must be a PagedCache, got {type(cache).__name__}")
-    k = cache.k
-    for name, t in (("cache.k", k), ("cache.v", cache.v), ("cache.positions", cache.positions), ("cache.weights", cache.weights), ("table", table), ("lengths", lengths)):
-        if t is None and name in ("cache.positions", "cache.weights"):
-            continue
+    """Raises for everything that the kernels do not take.  -> the type of the cache's values"""
+    if not isinstance(cache, (PagedCache, PagedCache4)):
+        raise TypeError(f"cache must be a PagedCache or a PagedCache4, got {type(cache).__name__}")
+    k, held = cache.k, isinstance(cache, PagedCache4)
+    tensors = [("k", k), ("v", cache.v), ("positions", cache.positions), ("weights", cache.weights)]
+    if held:
+        tensors += [("k_scales", cache.k_scales), ("v_scales", cache.v_scales)]
+    tensors = [("cache." + name, t) for name, t in tensors if t is not None or name not in ("positions", "weights")]
+    for name, t in (*tensors, ("table", table), ("lengths", lengths)):
         if not isinstance(t, torch.Tensor):
             raise TypeError(f"{name} must be a tensor, got {type(t).__name__}")
         _require_device(t, name)
@@ -73,13 +114,21 @@ def _check_cache(cache, table, lengths):
             raise ValueError(f"{name} must be on the cache's device ({k.device}), got {t.device}")
         if not t.is_contiguous():
             raise ValueError(f"{name} must be contiguous")
-    if k.dtype not in _TYPES or cache.v.dtype != k.dtype:
+    if held:
+        if cache.dtype not in _TYPES:
+            raise TypeError(f"cache.dtype must be bfloat16 or float16, got {cache.dtype}")
+        if any(t.dtype != torch.uint8 for t in (k, cache.v, cache.k_scales, cache.v_scales)):
+            raise TypeError("cache.k, cache.v, cache.k_scales and cache.v_scales must be uint8")
+    elif k.dtype not in _TYPES or cache.v.dtype != k.dtype:
         raise TypeError(f"cache.k and cache.v must both be bfloat16 or float16, got {k.dtype} and {cache.v.dtype}")
-    if k.dim() != 4 or k.shape[3] != HEAD_DIM or cache.v.shape != k.shape:
-        raise ValueError(f"cache.k and cache.v must have shape (pages, kv_heads, page_size, {HEAD_DIM}), got {tuple(k.shape)} and {tuple(cache.v.shape)}")
+    width = HEAD_DIM // 2 if held else HEAD_DIM
+    if k.dim() != 4 or k.shape[3] != width or cache.v.shape != k.shape:
+        raise ValueError(f"cache.k and cache.v must have shape (pages, kv_heads, page_size, {width}), got {tuple(k.shape)} and {tuple(cache.v.shape)}")
     _page_size(k.shape[2])
     if k.numel() == 0:
         raise ValueError(f"the cache must have a page and a head, got {tuple(k.shape)}")
+    if held and any(t.shape != (*k.shape[:3], HEAD_DIM // 32) for t in (cache.k_scales, cache.v_scales)):
+        raise ValueError(f"cache.k_scales and cache.v_scales must have shape {(*k.shape[:3], HEAD_DIM // 32)}, got {tuple(cache.k_scales.shape)} and {tuple(cache.v_scales.shape)}")
     for name, t, dtype in (("positions", cache.positions, torch.int32), ("weights", cache.weights, torch.float32)):
         if t is not None and (t.dtype != dtype or t.shape != k.shape[:3]):
             raise ValueError(f"cache.{name} must be {dtype} of shape {tuple(k.shape[:3])}, got {t.dtype} {tuple(t.shape)}")
@@ -89,9 +138,10 @@ def _check_cache(cache, table, lengths):
         raise ValueError(f"lengths must be int32 of shape ({table.shape[0]},), got {lengths.dtype} {tuple(lengths.shape)}")
     if table.shape[1] * k.shape[2] > 1 << 28 or table.shape[0] > 0x7fffff or k.shape[1] > 65535 or k.shape[0] > 0x7fffffff:
         raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a sequence may have 2^28 slots at most, a pool 2^31 - 1 pages of 65535 heads, got table {tuple(table.shape)}, cache {tuple(k.shape)}")
-    for name, t in (("cache.k", k), ("cache.v", cache.v), ("cache.positions", cache.positions), ("cache.weights", cache.weights)):
-        if t is not None and t.data_ptr() % 16:
+    for name, t in tensors:
+        if t.data_ptr() % 16:
             raise ValueError(f"{name} must be 16-byte aligned")
+    return cache.dtype if held else k.dtype
 
 
 def _check_ints(t, name, table):
@@ -112,6 +162,59 @@ def _answered(result):
     return result
 
 
+def _check_rows(table, kv_heads, like, dtype, k, v):
+    batch = table.shape[0]
+    for name, t in (("k", k), ("v", v)):
+        _require_device(t, name)
+        if t.dtype != dtype or t.device != like.device:
+            raise TypeError(f"{name} must have the cache's type and device ({dtype}, {like.device}), got {t.dtype}, {t.device}")
+        if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != kv_heads or t.shape[3] != HEAD_DIM or t.shape != k.shape:
+            raise ValueError(f"k and v must have shape ({batch}, {kv_heads}, tokens, {HEAD_DIM}), got {tuple(k.shape)} and {tuple(v.shape)}")
+    if k.shape[2] > 1 << 28:
+        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a call may append 2^28 tokens at most, got {k.shape[2]}")
+
+
+def _append(cache, table, lengths, k, v, counts, positions, weights, q=None, rotary=None, coordinates=None):
+    """-> (lengths, q turned)"""
+    given = _given(cache, table, lengths)
+    turn = (None, None, None, None) if rotary is None else (rotary.turns, rotary.axes, rotary.n_axes, rotary.interleaved) if isinstance(rotary, Rotary) else None
+    out = None if given is None or turn is None else _lib.host().cache_append(given, k, v, counts, positions, weights, q, *turn, coordinates)
+    if out is not None:
+        return out
+    dtype = _check_cache(cache, table, lengths)
+    _check_rows(table, cache.k.shape[1], cache.k, dtype, k, v)
+    batch, tokens = k.shape[0], k.shape[2]
+    _check_ints(counts, "counts", table)
+    _check_ints(positions, "positions", table)
+    if positions is not None and cache.positions is None and rotary is None:
+        raise ValueError("positions are given, but the cache has none")
+    if weights is not None:
+        if cache.weights is None:
+            raise ValueError("weights are given, but the cache has none")
+        if weights.dtype != torch.float32 or weights.shape != k.shape[:3] or weights.device != k.device:
+            raise ValueError(f"weights must be float32 of shape {tuple(k.shape[:3])} on {k.device}, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
+    if rotary is not None:
+        _check_rotary(rotary, k)
+        coordinates = _check_coordinates(coordinates, rotary, batch, tokens, k)
+    if q is not None:
+        _require_device(q, "q")
+        if q.dtype != dtype or q.device != k.device:
+            raise TypeError(f"q must have the cache's type and device ({dtype}, {k.device}), got {q.dtype}, {q.device}")
+        if q.dim() != 4 or q.shape[0] != batch or q.shape[2] != tokens or q.shape[3] != HEAD_DIM or not 1 <= q.shape[1] <= 65535:
+            raise ValueError(f"q must have shape ({batch}, heads, {tokens}, {HEAD_DIM}), 65535 heads at most, got {tuple(q.shape)}")
+    if (rotary is not None or isinstance(cache, PagedCache4)) and (batch * tokens > 1 << 27 or batch > 1 << 22):
+        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"all sequences together may have 2^27 new tokens, and a batch 2^22 of them, got {batch} x {tokens}")
+    _no_gradients(**{"cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights, "k": k, "v": v, "weights": weights, "q": q})
+    if tokens == 0:
+        right = (lengths >= 0) & (lengths <= table.shape[1] * cache.k.shape[2])
+        return torch.where(right if counts is None else right & (counts == 0), lengths, -1), None if q is None else torch.empty_like(q)
+    dense = lambda t: None if t is None else t.contiguous()
+    rows = lambda t: None if t is None else _rows_dense(t)
+    if rotary is not None:
+        turn = (*turn[:2], int(rotary.n_axes), bool(rotary.interleaved))
+    return _answered(_lib.host().cache_append(given, rows(k), rows(v), dense(counts), dense(positions), dense(weights), rows(q), *turn, coordinates))
+
+
 def cache_append(cache, table, lengths, k, v, counts=None, positions=None, weights=None):
     """Rows of new tokens go to the slots behind `lengths`: k, v (batch, kv_heads, tokens, 128), any strides with dense rows; of sequence b the first counts[b] (int32
     (batch,); None: all).  Where the cache has positions, the tokens' are positions[b], positions[b] + 1, ... (int32 (batch,); None: those of the slots, right
@@ -119,35 +222,36 @@ def cache_append(cache, table, lengths, k, v, counts=None, positions=None, weigh
 
     Returns the new lengths, a tensor of its own: lengths + counts, and -1 where length or count make no sense, there is no room (nothing is written then) or a page is
     outside of the pool (its rows are not written)."""
-    given = (cache.k, cache.v, cache.positions, cache.weights, table, lengths) if isinstance(cache, PagedCache) else None
-    out = None if given is None else _lib.host().cache_append(*given, k, v, counts, positions, weights)
+    return _append(cache, table, lengths, k, v, counts, positions, weights)[0]
+
+
+def cache_append_rotary(cache, table, lengths, k, v, rotary, q=None, counts=None, positions=None, weights=None, coordinates=None):
+    """`cache_append` with k turned by `rotary` (positions.py) on the way, and q (batch, heads, tokens, 128), if given, beside it; in one launch.  The tokens of sequence b stand at
+    positions[b], positions[b] + 1, ... on every axis (None: at their slots; a cache without positions takes them too), or at `coordinates`, int32 (tokens, n_axes) or
+    (batch, tokens, n_axes), which the cache's own positions do not follow.  A k that goes into 4 bits is rounded once.
+
+    Returns the new lengths, as `cache_append` does, and q turned (None without): its rows behind a sequence's count too, and no numbers for a sequence whose length or count makes no
+    sense."""
+    if not isinstance(rotary, Rotary):
+        raise TypeError(f"rotary must be a Rotary, got {type(rotary).__name__}")
+    return _append(cache, table, lengths, k, v, counts, positions, weights, q, rotary, coordinates)
+
+
+def cache_read(cache, table, lengths, slots, first=0):
+    """Slots first .. first + slots - 1 of every sequence as dense tensors k, v (batch, kv_heads, slots, 128) of the cache's type: what a prompt's next chunk attends to with
+    `window_attn_func`.  Rows behind a sequence's length are zeros; those of a page outside of the pool, and all of a sequence whose length makes no sense, are no numbers."""
+    given = _given(cache, table, lengths)
+    out = None if given is None else _lib.host().cache_read(given, slots, first)
     if out is not None:
         return out
-    _check_cache(cache, table, lengths)
-    batch, kv_heads = table.shape[0], cache.k.shape[1]
-    for name, t in (("k", k), ("v", v)):
-        _require_device(t, name)
-        if t.dtype != cache.k.dtype or t.device != cache.k.device:
-            raise TypeError(f"{name} must have the cache's type and device ({cache.k.dtype}, {cache.k.device}), got {t.dtype}, {t.device}")
-        if t.dim() != 4 or t.shape[0] != batch or t.shape[1] != kv_heads or t.shape[3] != HEAD_DIM or t.shape != k.shape:
-            raise ValueError(f"k and v must have shape ({batch}, {kv_heads}, tokens, {HEAD_DIM}), got {tuple(k.shape)} and {tuple(v.shape)}")
-    if k.shape[2] > 1 << 28:
-        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a call may append 2^28 tokens at most, got {k.shape[2]}")
-    _check_ints(counts, "counts", table)
-    _check_ints(positions, "positions", table)
-    if positions is not None and cache.positions is None:
-        raise ValueError("positions are given, but the cache has none")
-    if weights is not None:
-        if cache.weights is None:
-            raise ValueError("weights are given, but the cache has none")
-        if weights.dtype != torch.float32 or weights.shape != k.shape[:3] or weights.device != k.device:
-            raise ValueError(f"weights must be float32 of shape {tuple(k.shape[:3])} on {k.device}, got {weights.dtype} {tuple(weights.shape)} on {weights.device}")
-    _no_gradients(**{"cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights, "k": k, "v": v, "weights": weights})
-    if k.shape[2] == 0:
-        right = (lengths >= 0) & (lengths <= table.shape[1] * cache.k.shape[2])
-        return torch.where(right if counts is None else right & (counts == 0), lengths, -1)
-    dense = lambda t: None if t is None else t.contiguous()
-    return _answered(_lib.host().cache_append(*given, _rows_dense(k), _rows_dense(v), dense(counts), dense(positions), dense(weights)))
+    dtype = _check_cache(cache, table, lengths)
+    slots, first = _whole(slots, "slots", 0), _whole(first, "first", 0)
+    if slots > 1 << 28 or first > 1 << 28:
+        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"a sequence has 2^28 slots at most, got first {first} and slots {slots}")
+    _no_gradients(**{"cache.k": cache.k, "cache.v": cache.v})
+    if slots == 0:
+        return tuple(torch.empty((table.shape[0], cache.k.shape[1], 0, HEAD_DIM), dtype=dtype, device=cache.k.device) for _ in range(2))
+    return _answered(_lib.host().cache_read(given, slots, first))
 
 
 def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=False):
@@ -156,14 +260,14 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
 
     q: (batch, heads, 1, 128) of the cache's type, heads a multiple of kv_heads.  accumulate=True adds to cache.weights what softmax gave every slot, summed over the query
     heads of a kv head; not with a window, and with a workspace of 4 * batch * heads bytes for every slot that the table has room for, filled or not.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
-    given = (cache.k, cache.v, cache.weights, table, lengths) if isinstance(cache, PagedCache) else None
-    out = None if given is None else _lib.host().cache_attention(q, *given, window, sinks, bool(accumulate))
+    given = _given(cache, table, lengths)
+    out = None if given is None else _lib.host().cache_attention(q, given, window, sinks, bool(accumulate))
     if out is not None:
         return out
-    _check_cache(cache, table, lengths)
+    dtype = _check_cache(cache, table, lengths)
     _require_device(q, "q")
-    if q.dtype != cache.k.dtype or q.device != cache.k.device:
-        raise TypeError(f"q must have the cache's type and device ({cache.k.dtype}, {cache.k.device}), got {q.dtype}, {q.device}")
+    if q.dtype != dtype or q.device != cache.k.device:
+        raise TypeError(f"q must have the cache's type and device ({dtype}, {cache.k.device}), got {q.dtype}, {q.device}")
     if q.dim() != 4 or q.shape[0] != table.shape[0] or q.shape[2] != 1 or q.shape[3] != HEAD_DIM:
         raise ValueError(f"q must have shape ({table.shape[0]}, heads, 1, {HEAD_DIM}), got {tuple(q.shape)}")
     if q.shape[1] == 0 or q.shape[1] % cache.k.shape[1] or q.shape[1] > 65535:
@@ -175,7 +279,7 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
     window = _NO_WINDOW if window is None else _whole(window, "window", 1)
     sinks = _whole(sinks, "sinks", 0)
     _no_gradients(**{"q": q, "cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights})
-    return _answered(_lib.host().cache_attention(_rows_dense(q), *given, None if window == _NO_WINDOW else window, sinks, bool(accumulate)))
+    return _answered(_lib.host().cache_attention(_rows_dense(q), given, None if window == _NO_WINDOW else window, sinks, bool(accumulate)))
 
 
 def cache_evict(cache, table, lengths, budget, recent=0, sinks=0):
@@ -184,8 +288,8 @@ def cache_evict(cache, table, lengths, budget, recent=0, sinks=0):
     positions and weights; slots are in no order of tokens then.  batch * kv_heads may be 65535 at most.
 
     Returns the new lengths, a tensor of its own: min(lengths, budget), and -1, with nothing moved, where a length or page makes no sense."""
-    given = (cache.k, cache.v, cache.positions, cache.weights, table, lengths) if isinstance(cache, PagedCache) else None
-    out = None if given is None else _lib.host().cache_evict(*given, budget, recent, sinks)
+    given = _given(cache, table, lengths)
+    out = None if given is None else _lib.host().cache_evict(given, budget, recent, sinks)
     if out is not None:
         return out
     _check_cache(cache, table, lengths)
@@ -195,4 +299,4 @@ def cache_evict(cache, table, lengths, budget, recent=0, sinks=0):
     if recent + sinks > budget:
         raise ValueError(f"recent ({recent}) and sinks ({sinks}) must fit the budget ({budget}) together")
     _no_gradients(**{"cache.k": cache.k, "cache.v": cache.v, "cache.weights": cache.weights})
-    return _answered(_lib.host().cache_evict(*given, budget, recent, sinks))
+    return _answered(_lib.host().cache_evict(given, budget, recent, sinks))

@@ -1050,8 +1050,42 @@ int take_cache(fba::CacheView& to, const fba_cache* c) {
   return FBA_OK;
 }
 
-int take_attend(fba::AttendParams& p, const fba_cache* cache, int32_t heads, int32_t accumulate) {
-  if (int rc = take_cache(p.cache, cache)) return rc;
+// The same of a pool in 4 bits.
+int take_cache4(fba::CacheView& to, const fba_cache4* c) {
+  if (c == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  if (int rc = check_ptrs({{"k_scales", c->k_scales}, {"v_scales", c->v_scales}})) return rc;
+  if (int rc = take_cache(to, &c->cache)) return rc;
+  to.k_scales = c->k_scales;
+  to.v_scales = c->v_scales;
+  return FBA_OK;
+}
+
+int check_type(int32_t type) {
+  return type == FBA_BF16 || type == FBA_FP16 ? FBA_OK : fail(FBA_ERR_INVALID, "type must be FBA_BF16 or FBA_FP16, got %d", type);
+}
+
+// r null: nothing turns
+int take_rotation(fba::Rotation& to, const fba_rotation* r) {
+  to = fba::Rotation{};
+  if (r == nullptr) return FBA_OK;
+  if (r->turns == nullptr || r->axes == nullptr) return fail(FBA_ERR_INVALID, "turns or axes is null");
+  if ((reinterpret_cast<uintptr_t>(r->turns) & 7u) != 0 || ((reinterpret_cast<uintptr_t>(r->axes) | reinterpret_cast<uintptr_t>(r->at)) & 3u) != 0)
+    return fail(FBA_ERR_INVALID, "turns, axes or at is not aligned");
+  if (r->pairs < 8 || r->pairs > 64 || r->pairs % 8 != 0) return fail(FBA_ERR_INVALID, "pairs (%d) must be a multiple of 8, 64 at most", r->pairs);
+  if (r->n_axes < 1 || r->n_axes > 8) return fail(FBA_ERR_INVALID, "n_axes (%d) must be between 1 and 8", r->n_axes);
+  if (r->at_batch < 0 || r->at_batch > 1LL << 40) return fail(FBA_ERR_INVALID, "at_batch (%lld) must not be negative, nor beyond 2^40", (long long)r->at_batch);
+  to.turns = r->turns;
+  to.axes = r->axes;
+  to.at = r->at;
+  to.at_batch = r->at_batch;
+  to.n_axes = r->n_axes;
+  to.pairs = r->pairs;
+  to.interleaved = r->interleaved != 0;
+  return FBA_OK;
+}
+
+int take_attend(fba::AttendParams& p, const fba_cache* cache, int32_t heads, int32_t accumulate, const fba_cache4* cache4 = nullptr) {
+  if (int rc = cache4 != nullptr ? take_cache4(p.cache, cache4) : take_cache(p.cache, cache)) return rc;
   if (heads <= 0 || heads % cache->kv_heads != 0) return fail(FBA_ERR_INVALID, "heads (%d) must be a multiple of kv_heads (%d)", heads, cache->kv_heads);
   if (accumulate && cache->weights == nullptr) return fail(FBA_ERR_INVALID, "weights is null");
   if (heads > 65535) return fail(FBA_ERR_UNSUPPORTED, "heads (%d) may be 65535 at most", heads);
@@ -1069,8 +1103,8 @@ int check_ws(const void* ws, int64_t bytes, int64_t need) {
   return FBA_OK;
 }
 
-int take_evict(fba::EvictParams& p, const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks) {
-  if (int rc = take_cache(p.cache, cache)) return rc;
+int take_evict(fba::EvictParams& p, const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks, const fba_cache4* cache4 = nullptr) {
+  if (int rc = cache4 != nullptr ? take_cache4(p.cache, cache4) : take_cache(p.cache, cache)) return rc;
   if (budget < 1) return fail(FBA_ERR_INVALID, "budget (%d) must be at least 1", budget);
   if (recent < 0 || sinks < 0 || (int64_t)recent + sinks > budget)
     return fail(FBA_ERR_INVALID, "recent (%d) and sinks (%d) must not be negative, and fit the budget (%d) together", recent, sinks, budget);
@@ -1079,6 +1113,99 @@ int take_evict(fba::EvictParams& p, const fba_cache* cache, int32_t budget, int3
   p.recent = recent;
   p.sinks = sinks;
   return FBA_OK;
+}
+
+// cache4: null, or what `cache` is the first part of
+int run_attend(const fba_cache* cache, const fba_cache4* cache4, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate, int32_t type,
+               void* ws, int64_t ws_bytes, void* hip_stream) {
+  fba::AttendParams p{};
+  if (int rc = take_attend(p, cache, heads, accumulate, cache4)) return rc;
+  if (int rc = check_type(type)) return rc;
+  if (int rc = take_strided(p.q, q, "q")) return rc;
+  if (int rc = take_strided(p.o, o, "o")) return rc;
+  if (window < 1) return fail(FBA_ERR_INVALID, "window (%d) must be at least 1", window);
+  if (sinks < 0) return fail(FBA_ERR_INVALID, "sinks (%d) must not be negative", sinks);
+  if (accumulate && window < p.cache.slots()) return fail(FBA_ERR_INVALID, "weights are added up over the whole cache: window (%d) must reach over its %lld slots", window, (long long)p.cache.slots());
+  if (int rc = check_ws(ws, ws_bytes, fba::cache_attend_bytes(p, accumulate != 0))) return rc;
+  p.window = window;
+  p.sinks = sinks;
+  p.scale_log2e = 1.4426950408889634f / 11.313708498984761f;
+  const int64_t parts = (int64_t)p.slots * heads;
+  float* at = (float*)ws;
+  if (accumulate) {
+    p.scores = at;
+    at += (int64_t)cache->batch * heads * p.cache.slots();
+  }
+  p.part = at;
+  p.part_ml = p.part + parts * 128;
+  p.note = (int32_t*)(p.part_ml + parts * 2);
+  hipError_t e = (cache4 != nullptr ? fba::launch_cache_attend4 : fba::launch_cache_attend)(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache attention launch");
+}
+
+int run_evict(const fba_cache* cache, const fba_cache4* cache4, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream) {
+  fba::EvictParams p{};
+  if (int rc = take_evict(p, cache, budget, recent, sinks, cache4)) return rc;
+  if (cache->positions == nullptr || cache->weights == nullptr) return fail(FBA_ERR_INVALID, "positions or weights is null");
+  if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
+  if (lengths_out == cache->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
+  if (int rc = check_ws(ws, ws_bytes, fba::cache_evict_bytes(p))) return rc;
+  p.lengths_out = lengths_out;
+  p.moves = (int32_t*)ws;
+  hipError_t e = fba::launch_cache_evict(p, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache eviction launch");
+}
+
+// Does one launch take the tokens of all sequences?
+int check_tokens(int64_t batch, int64_t tokens) {
+  if (batch * tokens > 1LL << 27) return fail(FBA_ERR_UNSUPPORTED, "all sequences together may have 2^27 tokens, got %lld x %lld", (long long)batch, (long long)tokens);
+  return FBA_OK;
+}
+
+// cache or cache4 is null; q null: there is none
+int run_append_rotary(const fba_cache* cache, const fba_cache4* cache4, const fba_strided* k, const fba_strided* v, const fba_strided* q, const fba_strided* q_out, int32_t heads,
+                      const fba_rotation* rotation, const int32_t* counts, const int32_t* first, const float* weights, int32_t tokens, int32_t type, int32_t* lengths_out, void* hip_stream) {
+  fba::AppendRotaryParams p{};
+  if (int rc = cache4 != nullptr ? take_cache4(p.append.cache, cache4) : take_cache(p.append.cache, cache)) return rc;
+  const fba_cache* const c = cache4 != nullptr ? &cache4->cache : cache;
+  if (tokens <= 0 || tokens > 1 << 28) return fail(FBA_ERR_INVALID, "tokens (%d) must be positive, 2^28 at most", tokens);
+  if (int rc = check_type(type)) return rc;
+  if (int rc = take_strided(p.append.k, k, "k")) return rc;
+  if (int rc = take_strided(p.append.v, v, "v")) return rc;
+  if (heads < 0 || heads > 65535 || (heads > 0) != (q != nullptr)) return fail(FBA_ERR_INVALID, "heads (%d) must be those of q, 65535 at most, and 0 without", heads);
+  if (q != nullptr) {
+    if (int rc = take_strided(p.q, q, "q")) return rc;
+    if (int rc = take_strided(p.q_out, q_out, "q_out")) return rc;
+  }
+  if (int rc = take_rotation(p.rotation, rotation)) return rc;
+  if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
+  if (lengths_out == c->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
+  if (c->batch > (1 << 22)) return fail(FBA_ERR_UNSUPPORTED, "batch (%d) is more than a launch takes", c->batch);
+  if (int rc = check_tokens(c->batch, tokens)) return rc;
+  p.heads = heads;
+  p.append.counts = counts;
+  p.append.first = first;
+  p.append.weights = weights;
+  p.append.tokens = tokens;
+  p.append.lengths_out = lengths_out;
+  hipError_t e = fba::launch_cache_append_rotary(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache append launch");
+}
+
+int run_read(const fba_cache* cache, const fba_cache4* cache4, int32_t first, int32_t slots, const fba_strided* k, const fba_strided* v, int32_t type, void* hip_stream) {
+  fba::ReadParams p{};
+  if (int rc = cache4 != nullptr ? take_cache4(p.cache, cache4) : take_cache(p.cache, cache)) return rc;
+  if (first < 0 || first > 1 << 28) return fail(FBA_ERR_INVALID, "first (%d) must not be negative, 2^28 at most", first);
+  if (slots <= 0 || slots > 1 << 28) return fail(FBA_ERR_INVALID, "slots (%d) must be positive, 2^28 at most", slots);
+  if (int rc = check_type(type)) return rc;
+  if (int rc = take_strided(p.k, k, "k")) return rc;
+  if (int rc = take_strided(p.v, v, "v")) return rc;
+  const int64_t heads = (int64_t)p.cache.batch * p.cache.kv_heads, chunks = (slots + fba::kReadRows - 1) / fba::kReadRows;
+  if (heads * chunks > kMostWorkGroups) return fail(FBA_ERR_UNSUPPORTED, "%lld heads of all sequences with %d slots each are more than a launch takes", (long long)heads, slots);
+  p.first = first;
+  p.slots = slots;
+  hipError_t e = fba::launch_cache_read(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache read launch");
 }
 
 }  // namespace
@@ -1112,29 +1239,19 @@ int64_t fba_cache_attn_workspace_bytes(const fba_cache* cache, int32_t heads, in
 
 int32_t fba_cache_attn(const fba_cache* cache, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate,
                        int32_t type, void* ws, int64_t ws_bytes, void* hip_stream) {
+  return run_attend(cache, nullptr, q, o, heads, window, sinks, accumulate, type, ws, ws_bytes, hip_stream);
+}
+
+int64_t fba_cache4_attn_workspace_bytes(const fba_cache4* cache, int32_t heads, int32_t accumulate) {
   fba::AttendParams p{};
-  if (int rc = take_attend(p, cache, heads, accumulate)) return rc;
-  if (type != FBA_BF16 && type != FBA_FP16) return fail(FBA_ERR_INVALID, "type must be FBA_BF16 or FBA_FP16, got %d", type);
-  if (int rc = take_strided(p.q, q, "q")) return rc;
-  if (int rc = take_strided(p.o, o, "o")) return rc;
-  if (window < 1) return fail(FBA_ERR_INVALID, "window (%d) must be at least 1", window);
-  if (sinks < 0) return fail(FBA_ERR_INVALID, "sinks (%d) must not be negative", sinks);
-  if (accumulate && window < p.cache.slots()) return fail(FBA_ERR_INVALID, "weights are added up over the whole cache: window (%d) must reach over its %lld slots", window, (long long)p.cache.slots());
-  if (int rc = check_ws(ws, ws_bytes, fba::cache_attend_bytes(p, accumulate != 0))) return rc;
-  p.window = window;
-  p.sinks = sinks;
-  p.scale_log2e = 1.4426950408889634f / 11.313708498984761f;
-  const int64_t parts = (int64_t)p.slots * heads;
-  float* at = (float*)ws;
-  if (accumulate) {
-    p.scores = at;
-    at += (int64_t)cache->batch * heads * p.cache.slots();
-  }
-  p.part = at;
-  p.part_ml = p.part + parts * 128;
-  p.note = (int32_t*)(p.part_ml + parts * 2);
-  hipError_t e = fba::launch_cache_attend(p, type == FBA_FP16, (hipStream_t)hip_stream);
-  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache attention launch");
+  if (cache == nullptr || take_attend(p, &cache->cache, heads, accumulate, cache)) return -1;
+  return fba::cache_attend_bytes(p, accumulate != 0);
+}
+
+int32_t fba_cache4_attn(const fba_cache4* cache, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate,
+                        int32_t type, void* ws, int64_t ws_bytes, void* hip_stream) {
+  if (cache == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  return run_attend(&cache->cache, cache, q, o, heads, window, sinks, accumulate, type, ws, ws_bytes, hip_stream);
 }
 
 int64_t fba_cache_evict_workspace_bytes(const fba_cache* cache, int32_t budget) {
@@ -1144,16 +1261,66 @@ int64_t fba_cache_evict_workspace_bytes(const fba_cache* cache, int32_t budget) 
 }
 
 int32_t fba_cache_evict(const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream) {
+  return run_evict(cache, nullptr, budget, recent, sinks, lengths_out, ws, ws_bytes, hip_stream);
+}
+
+int64_t fba_cache4_evict_workspace_bytes(const fba_cache4* cache, int32_t budget) {
   fba::EvictParams p{};
-  if (int rc = take_evict(p, cache, budget, recent, sinks)) return rc;
-  if (cache->positions == nullptr || cache->weights == nullptr) return fail(FBA_ERR_INVALID, "positions or weights is null");
-  if (lengths_out == nullptr) return fail(FBA_ERR_INVALID, "lengths_out is null");
-  if (lengths_out == cache->lengths) return fail(FBA_ERR_INVALID, "lengths_out must not be the cache's lengths");
-  if (int rc = check_ws(ws, ws_bytes, fba::cache_evict_bytes(p))) return rc;
-  p.lengths_out = lengths_out;
-  p.moves = (int32_t*)ws;
-  hipError_t e = fba::launch_cache_evict(p, (hipStream_t)hip_stream);
-  return e == hipSuccess ? FBA_OK : hip_fail(e, "cache eviction launch");
+  if (cache == nullptr || take_evict(p, &cache->cache, budget, 0, 0, cache)) return -1;
+  return fba::cache_evict_bytes(p);
+}
+
+int32_t fba_cache4_evict(const fba_cache4* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream) {
+  if (cache == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  return run_evict(&cache->cache, cache, budget, recent, sinks, lengths_out, ws, ws_bytes, hip_stream);
+}
+
+int32_t fba_cache_append_rotary(const fba_cache* cache, const fba_strided* k, const fba_strided* v, const fba_strided* q, const fba_strided* q_out, int32_t heads,
+                                const fba_rotation* rotation, const int32_t* counts, const int32_t* first, const float* weights, int32_t tokens, int32_t type,
+                                int32_t* lengths_out, void* hip_stream) {
+  if (rotation == nullptr) return fail(FBA_ERR_INVALID, "rotation is null");
+  return run_append_rotary(cache, nullptr, k, v, q, q_out, heads, rotation, counts, first, weights, tokens, type, lengths_out, hip_stream);
+}
+
+int32_t fba_cache4_append(const fba_cache4* cache, const fba_strided* k, const fba_strided* v, const fba_strided* q, const fba_strided* q_out, int32_t heads,
+                          const fba_rotation* rotation, const int32_t* counts, const int32_t* first, const float* weights, int32_t tokens, int32_t type, int32_t* lengths_out,
+                          void* hip_stream) {
+  if (cache == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  return run_append_rotary(nullptr, cache, k, v, q, q_out, heads, rotation, counts, first, weights, tokens, type, lengths_out, hip_stream);
+}
+
+int32_t fba_cache_read(const fba_cache* cache, int32_t first, int32_t slots, const fba_strided* k, const fba_strided* v, int32_t type, void* hip_stream) {
+  return run_read(cache, nullptr, first, slots, k, v, type, hip_stream);
+}
+
+int32_t fba_cache4_read(const fba_cache4* cache, int32_t first, int32_t slots, const fba_strided* k, const fba_strided* v, int32_t type, void* hip_stream) {
+  if (cache == nullptr) return fail(FBA_ERR_INVALID, "cache is null");
+  return run_read(nullptr, cache, first, slots, k, v, type, hip_stream);
+}
+
+int32_t fba_rotary(const fba_strided* q, const fba_strided* q_out, const fba_strided* k, const fba_strided* k_out, const fba_rotation* rotation, int32_t inverse, int32_t B, int32_t Hq,
+                   int32_t Hk, int32_t S, int32_t head_dim, int32_t type, void* hip_stream) {
+  fba::RotaryParams p{};
+  if (head_dim != 128) return fail(FBA_ERR_INVALID, "head_dim must be 128, got %d", head_dim);
+  if (int rc = check_type(type)) return rc;
+  if (B <= 0 || Hq <= 0 || Hk < 0 || S <= 0 || Hq > 65535 || Hk > 65535) return fail(FBA_ERR_INVALID, "B, Hq and S must be positive, Hq and Hk 65535 at most (got %d %d %d %d)", B, Hq, Hk, S);
+  if (rotation == nullptr) return fail(FBA_ERR_INVALID, "rotation is null");
+  if (int rc = take_rotation(p.rotation, rotation)) return rc;
+  if (int rc = take_strided(p.q, q, "q")) return rc;
+  if (int rc = take_strided(p.q_out, q_out, "q_out")) return rc;
+  if ((Hk > 0) != (k != nullptr)) return fail(FBA_ERR_INVALID, "Hk (%d) must be the heads of k, and 0 without", Hk);
+  if (k != nullptr) {
+    if (int rc = take_strided(p.k, k, "k")) return rc;
+    if (int rc = take_strided(p.k_out, k_out, "k_out")) return rc;
+  }
+  if (int rc = check_tokens(B, S)) return rc;
+  p.rotation.back = inverse != 0;
+  p.heads = Hq;
+  p.kv_heads = Hk;
+  p.seq = S;
+  p.tokens = (uint32_t)B * (uint32_t)S;
+  hipError_t e = fba::launch_rotary(p, type == FBA_FP16, (hipStream_t)hip_stream);
+  return e == hipSuccess ? FBA_OK : hip_fail(e, "rotary launch");
 }
 
 }  // extern "C"

@@ -2,13 +2,19 @@
 //
 // A pool of pages [pages, kv heads, page size, 128]; a page holds page_size slots of every kv head.  Sequence b's slot s is slot s % page_size of page
 // table[b][s / page_size]; the first lengths[b] slots are filled.  positions and weights [pages, kv heads, page size] go with the slots.
+//
+// Held in 4 bits, a row is 64 bytes, value 2j in the low half of byte j, and four scales [pages, kv heads, page size, 4], one for each 32 columns: a value is 0, 0.5, 1, 1.5, 2, 3, 4
+// or 6, with a sign, times 2^(scale - 127), and no number where the scale is 255.
 #pragma once
 #include <hip/hip_runtime.h>
 #include <stdint.h>
 
+#include "fba_rotary.h"
 #include "fba_window.h"
 
 namespace fba {
+
+constexpr int kHeldRowBytes = 64;
 
 struct CacheView {
   char* k;
@@ -19,6 +25,8 @@ struct CacheView {
   const int32_t* lengths;  // [batch]
   int64_t pages;
   int kv_heads, page_log2, batch, max_pages;
+  uint8_t* k_scales;       // null: rows of 16-bit values
+  uint8_t* v_scales;
   __host__ __device__ int64_t slots() const { return (int64_t)max_pages << page_log2; }  // that a sequence has room for
   // A length that the table has room for.
   __host__ __device__ bool holds(int64_t n) const { return n >= 0 && n <= slots(); }
@@ -42,6 +50,21 @@ struct AppendParams {
   int32_t* lengths_out;
   int tokens;
   int row_wgs;
+};
+
+struct AppendRotaryParams {
+  AppendParams append;
+  Rotation rotation;         // of k and q; `at` null: the tokens' positions on every axis
+  Strided q, q_out;          // [batch, heads, tokens, 128]
+  int heads;                 // 0: no q
+  uint32_t parts, per;       // parts that kv heads and heads are cut into, heads of a part
+};
+
+struct ReadParams {
+  CacheView cache;
+  Strided k, v;              // [batch, kv heads, slots, 128]
+  int first, slots;
+  uint32_t chunks;           // of kReadRows slots, of a head
 };
 
 struct AttendParams {
@@ -70,9 +93,14 @@ struct EvictParams {
 };
 
 hipError_t launch_cache_append(AppendParams p, hipStream_t stream);
+hipError_t launch_cache_append_rotary(AppendRotaryParams p, bool half, hipStream_t stream);  // or into 4 bits
+constexpr int kReadRows = 64;
+hipError_t launch_cache_read(ReadParams p, bool half, hipStream_t stream);
 void plan_cache_attend(AttendParams& p, int compute_units);
 int64_t cache_attend_bytes(const AttendParams& p, bool accumulate);
 hipError_t launch_cache_attend(AttendParams p, bool half, hipStream_t stream);
+hipError_t launch_cache_attend4(AttendParams p, bool half, hipStream_t stream);
+hipError_t launch_cache_join(AttendParams p, bool half, hipStream_t stream);  // behind either
 int64_t cache_evict_bytes(EvictParams& p);
 hipError_t launch_cache_evict(EvictParams p, hipStream_t stream);
 

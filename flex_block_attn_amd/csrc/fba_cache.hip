@@ -1,4 +1,4 @@
-// What fills a paged cache and what makes room in it: gfx950.  Rows of 256 bytes are moved, 16 lanes to a row; bound by device memory, in small calls by the launch.
+// What fills a paged cache and what makes room in it: gfx950.  Rows of 256 bytes are moved, 16 lanes to a row (of 64 where they are held in 4 bits, and their scales); bound by device memory, in small calls by the launch.
 #include "fba_cache.h"
 #include "fba_common.h"
 
@@ -115,14 +115,31 @@ struct Ranks {
   }
 };
 
+// One row's sixteenth, of the pool of K or of V.
+FBA_DEVICE void move_piece(char* rows, bool held, int64_t to, int64_t from, int c) {
+  if (held) *reinterpret_cast<uint32_t*>(rows + to * kHeldRowBytes + c * 4) = *reinterpret_cast<const uint32_t*>(rows + from * kHeldRowBytes + c * 4);
+  else *reinterpret_cast<u32x4*>(rows + to * kRowBytes + c * 16) = *reinterpret_cast<const u32x4*>(rows + from * kRowBytes + c * 16);
+}
+FBA_DEVICE void move_scales(uint8_t* scales, int64_t to, int64_t from) {  // of a row, all four
+  reinterpret_cast<uint32_t*>(scales)[to] = reinterpret_cast<const uint32_t*>(scales)[from];
+}
+
 // The i-th freed slot gets the i-th kept one from behind the budget, row, position and weight: 16 lanes to a row, i = first, first + step, ...
 FBA_DEVICE void move_rows(const CacheView& cache, const int32_t* moves, int most, int b, int hkv, int c, int first, int step, int n) {
+  const bool held = cache.k_scales != nullptr;
   for (int i = first; i < n; i += step) {
     const int to_slot = moves[1 + i], from_slot = moves[1 + most + i];
     const int64_t to = cache.row_of(cache.page_of(b, to_slot), hkv, to_slot), from = cache.row_of(cache.page_of(b, from_slot), hkv, from_slot);
-    const u32x4 kr = *reinterpret_cast<const u32x4*>(cache.k + from * kRowBytes + c * 16), vr = *reinterpret_cast<const u32x4*>(cache.v + from * kRowBytes + c * 16);
-    *reinterpret_cast<u32x4*>(cache.k + to * kRowBytes + c * 16) = kr;
-    *reinterpret_cast<u32x4*>(cache.v + to * kRowBytes + c * 16) = vr;
+    if (held) {
+      move_piece(cache.k, true, to, from, c);
+      move_piece(cache.v, true, to, from, c);
+      if (c == 2) move_scales(cache.k_scales, to, from);
+      if (c == 3) move_scales(cache.v_scales, to, from);
+    } else {
+      const u32x4 kr = *reinterpret_cast<const u32x4*>(cache.k + from * kRowBytes + c * 16), vr = *reinterpret_cast<const u32x4*>(cache.v + from * kRowBytes + c * 16);
+      *reinterpret_cast<u32x4*>(cache.k + to * kRowBytes + c * 16) = kr;
+      *reinterpret_cast<u32x4*>(cache.v + to * kRowBytes + c * 16) = vr;
+    }
     if (c == 0) cache.positions[to] = cache.positions[from];
     if (c == 1) cache.weights[to] = cache.weights[from];
   }
@@ -267,10 +284,9 @@ __global__ __launch_bounds__(kSelectThreads) void cache_select_kernel(const Evic
         const int to_slot = __builtin_amdgcn_readlane(gone, __builtin_ctzll(__builtin_amdgcn_ballot_w64(frees && rank == i)));
         const int from_slot = p.budget + __builtin_ctzll(__builtin_amdgcn_ballot_w64(late && late_rank == i));
         const int64_t to = row_of(to_slot), from = row_of(from_slot);
-        if (lane < 32) {
-          char* const rows = (lane < 16 ? cache.k : cache.v) + (lane & 15) * 16;
-          *reinterpret_cast<u32x4*>(rows + to * kRowBytes) = *reinterpret_cast<const u32x4*>(rows + from * kRowBytes);
-        }
+        const bool held = cache.k_scales != nullptr;
+        if (lane < 32) move_piece(lane < 16 ? cache.k : cache.v, held, to, from, lane & 15);
+        if (held && (lane == 34 || lane == 35)) move_scales(lane == 34 ? cache.k_scales : cache.v_scales, to, from);
         if (lane == 32) cache.positions[to] = cache.positions[from];
         if (lane == 33) cache.weights[to] = cache.weights[from];
       }

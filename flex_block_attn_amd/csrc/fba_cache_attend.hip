@@ -13,53 +13,15 @@
 //
 // Accumulated weights need the denominator of all chunks: the first kernel leaves its scores (4 bytes for every head and slot, against 512 bytes of K and V), and the
 // second adds up exp2(score - log2 denominator) over the heads of the group.
-#include "fba_cache.h"
-#include "fba_types.h"
+#include "fba_cache_attend.h"
+
+#include <type_traits>
 
 namespace fba {
 
 namespace {
 
-constexpr int kTile = 32;
-constexpr int kTileLds = kTile * kRowBytes;  // 8 KiB
-constexpr int kWaves = 4;
-constexpr int kStage = 2 * kTileLds;         // of a wave: K tile | V tile
-constexpr int kLeastTiles = kWaves;          // of a share
-constexpr float kLazy = 8.f, kNoReference = -3e38f;
-
-// Tiles of a sequence that are read: those with sinks, then those from the window's start on.
-struct Tiles {
-  int n_sink, first, n;
-  FBA_DEVICE int at(int t) const { return t < n_sink ? t : first + t - n_sink; }
-};
-FBA_DEVICE Tiles tiles_of(int len, int window, int sinks) {
-  const int from = max(0, len - window), s = from > 0 ? min(sinks, len) : 0;
-  Tiles t;
-  t.n_sink = (s + kTile - 1) / kTile;
-  t.first = max(from / kTile, t.n_sink);
-  t.n = t.n_sink + max(0, (len + kTile - 1) / kTile - t.first);
-  return t;
-}
-
-FBA_DEVICE int length_of(const AttendParams& p, int b, bool* bad) {
-  const int n = p.cache.lengths[b];
-  *bad = !p.cache.holds(n);
-  return *bad ? 0 : n;
-}
-
-// A pointer that every lane has alike, in scalar registers.
-FBA_DEVICE const char* uniform(const char* p) {
-  const uint64_t v = (uint64_t)p;
-  return (const char*)((uint64_t)(uint32_t)__builtin_amdgcn_readfirstlane((int)(v >> 32)) << 32 | (uint32_t)__builtin_amdgcn_readfirstlane((int)v));
-}
-
-// The tiles of all sequences, one behind the other, dealt to `wgs` work-groups in even shares.  A sequence's part in share w has place w + b for its results: from one part to
-// the next w or b rises.
-struct Shares {
-  int total, wgs;
-  FBA_DEVICE int begin(int w) const { return (int)((int64_t)total * w / wgs); }
-  FBA_DEVICE int of(int tile) const { return (int)((((int64_t)tile + 1) * wgs - 1) / total); }
-};
+constexpr int kStage = 2 * kTileLds;  // of a wave: K tile | V tile
 
 template <int N>
 FBA_DEVICE void wait_copies() {  // until at most N are in flight; nothing moves across
@@ -80,52 +42,10 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   const int hkv = blockIdx.y / p.head_tiles, head0 = hkv * group + blockIdx.y % p.head_tiles * (16 * kHeadTiles);
   const int heads = min(16 * kHeadTiles, (hkv + 1) * group - head0);
 
-  // This work-group's share of the tiles of all sequences: all waves find it alike.
-  auto tiles_in = [&](int b) {
-    bool bad;
-    return b < cache.batch ? tiles_of(length_of(p, b, &bad), p.window, p.sinks).n : 0;
-  };
-  int total = 0;
-  const bool one = cache.batch == 1;              // (needs no sums over the wave: 8.1 us instead of 8.5 for 768 slots)
-  const int of_first = tiles_in(one ? 0 : lane);  // sequences 0 .. 63
-  if (one) total = __builtin_amdgcn_readfirstlane(of_first);
-  else
-    for (int b0 = 0; b0 < cache.batch; b0 += 64) total += wave_sum(b0 == 0 ? of_first : tiles_in(b0 + lane));
-  const Shares shares{total, min(p.target, max(1, (total + kLeastTiles - 1) / kLeastTiles))};
-  const int w = blockIdx.x;
-  if (w >= shares.wgs) return;
-  int tile = shares.begin(w);
-  const int end = shares.begin(w + 1);
-  const bool notes = w == 0 && blockIdx.y == 0;  // writes down which shares every sequence is in
-  int b = -1, start = 0;                         // the sequence of `tile`, its first tile
-  if (one) {
-    b = 0;
-    if (notes && tid == 0) {
-      p.note[0] = 0;
-      p.note[1] = total > 0 ? shares.of(total - 1) + 1 : 0;
-    }
-  }
-  for (int b0 = 0, before = 0; !one && b0 < cache.batch && (b < 0 || notes); b0 += 64) {
-    const int n = b0 == 0 ? of_first : tiles_in(b0 + lane);
-    int sum = n;  // of the lanes up to this one
-#pragma unroll
-    for (int d = 1; d < 64; d *= 2) {
-      const int other = __shfl_up(sum, d);
-      if (lane >= d) sum += other;
-    }
-    const unsigned long long past = __builtin_amdgcn_ballot_w64(before + sum > tile);
-    if (past != 0 && b < 0) {
-      const int at = __builtin_ctzll(past);
-      b = b0 + at;
-      start = before + __builtin_amdgcn_readlane(sum, at) - __builtin_amdgcn_readlane(n, at);
-    }
-    if (notes && wave == 0 && b0 + lane < cache.batch) {
-      const int first = n > 0 ? shares.of(before + sum - n) : 0;
-      p.note[2 * (b0 + lane)] = first + b0 + lane;
-      p.note[2 * (b0 + lane) + 1] = n > 0 ? shares.of(before + sum - 1) - first + 1 : 0;
-    }
-    before += __builtin_amdgcn_readlane(sum, 63);
-  }
+  Share share;
+  if (!find_share(p, tid, lane, wave, &share)) return;
+  const int w = share.w, end = share.end;
+  int tile = share.tile, b = share.b, start = share.start;
 
   // sequence by sequence
   for (; tile < end; ++b) {
@@ -300,49 +220,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(64 * kWaves, 64 * kWaves),
   }
   const bool any_bad = __builtin_amdgcn_ballot_w64(bad) != 0;
 
-  // The waves' sums: every wave's O [16 heads][128] and its references and denominators, in LDS, sixteen heads after the other.
-  float* const sums = reinterpret_cast<float*>(smem);         // [kWaves][16][128]
-  float* const ml = sums + kWaves * 16 * kHeadDim;            // [kWaves][16][2]
-#pragma unroll
-  for (int ht = 0; ht < kHeadTiles; ++ht) {
-    __syncthreads();
-    float l = l_run[ht];
-    l += __shfl_xor(l, 16);
-    l += __shfl_xor(l, 32);
-    const int row = wave * 16 + l16;
-#pragma unroll
-    for (int dt = 0; dt < 8; ++dt) *reinterpret_cast<f32x4*>(sums + row * kHeadDim + 16 * dt + 4 * g) = acc[ht][dt];
-    if (g == 0) {
-      ml[2 * row] = m_run[ht];
-      ml[2 * row + 1] = any_bad ? __builtin_nanf("") : l;
-    }
-    __syncthreads();
-    const int d = tid % (kHeadDim / 4) * 4;
-    for (int head = tid / (kHeadDim / 4); head < min(16, heads - 16 * ht); head += 64 * kWaves / (kHeadDim / 4)) {
-      float m = kNoReference, sum = 0.f;
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) m = fmaxf(m, ml[2 * (w * 16 + head)]);
-      f32x4 o = {0.f, 0.f, 0.f, 0.f};
-#pragma unroll
-      for (int w = 0; w < kWaves; ++w) {
-        const float f = fast_exp2(ml[2 * (w * 16 + head)] - m);
-        sum += f * ml[2 * (w * 16 + head) + 1];
-        o += f * *reinterpret_cast<const f32x4*>(sums + (w * 16 + head) * kHeadDim + d);
-      }
-      const int at_head = head0 + 16 * ht + head;
-      const int64_t at = (int64_t)(w + b) * p.heads + at_head;
-      if (alone) {
-        const float f = sum == 0.f ? 0.f : 1.f / sum;  // (NaN stays)
-        *reinterpret_cast<x4_of<T>*>(p.o.ptr + b * p.o.batch + at_head * p.o.head + 2 * d) = narrow4<T>(o[0] * f, o[1] * f, o[2] * f, o[3] * f);
-      } else {
-        *reinterpret_cast<f32x4*>(p.part + at * kHeadDim + d) = o;
-      }
-      if (d == 0) {
-        p.part_ml[2 * at] = m;
-        p.part_ml[2 * at + 1] = sum;
-      }
-    }
-  }  __syncthreads();  // the next sequence's copies go where the sums are
+  leave_sums<T, kHeadTiles>(p, smem, acc, m_run, l_run, any_bad, alone, b, w, head0, heads);  // (the next sequence's copies go where the sums are)
   }
 }
 
@@ -449,16 +327,12 @@ __global__ __launch_bounds__(256) void cache_join_kernel(const AttendParams p, i
   }
 }
 
-namespace {
-int head_tiles_of(int group) { return group <= 16 ? 1 : 2; }  // (four do not fit the registers of two waves on a SIMD)
-}  // namespace
-
 void plan_cache_attend(AttendParams& p, int compute_units) {
   const int group = p.heads / p.cache.kv_heads, per = 16 * head_tiles_of(group);
   p.head_tiles = (group + per - 1) / per;
-  // Two work-groups are on a compute unit at a time (64 KiB of LDS each), and as many shares there are.
-  const int rows = p.cache.kv_heads * p.head_tiles;
-  p.target = 2 * compute_units / rows > 0 ? 2 * compute_units / rows : 1;
+  // Two work-groups are on a compute unit at a time (64 KiB of LDS each; of 4 bits kResident4 where a work-group has one tile of heads), and as many shares there are.
+  const int rows = p.cache.kv_heads * p.head_tiles, resident = p.cache.k_scales != nullptr && head_tiles_of(group) == 1 ? kResident4 : 2;
+  p.target = resident * compute_units / rows > 0 ? resident * compute_units / rows : 1;
   // no more than there may be tiles for
   const int64_t most = (p.cache.batch * ((p.cache.slots() + kTile - 1) / kTile) + kLeastTiles - 1) / kLeastTiles;
   if (p.target > most) p.target = (int)most;
@@ -477,14 +351,19 @@ static hipError_t launch_attend(const AttendParams& p, hipStream_t stream) {
   void (*fn)(const AttendParams) = tiles == 1 ? (scores ? &cache_attend_kernel<T, 1, true> : &cache_attend_kernel<T, 1, false>)
                                               : (scores ? &cache_attend_kernel<T, 2, true> : &cache_attend_kernel<T, 2, false>);
   constexpr int smem = kWaves * kStage;  // (more than the sums at the end take)
-  static_assert(smem >= kWaves * 16 * (kHeadDim + 2) * 4, "room for the sums");
+  static_assert(smem >= kSumsLds, "room for the sums");
   hipError_t e = hipFuncSetAttribute(reinterpret_cast<const void*>(fn), hipFuncAttributeMaxDynamicSharedMemorySize, smem);
   if (e != hipSuccess) return e;
   hipLaunchKernelGGL(fn, dim3(p.target, p.cache.kv_heads * p.head_tiles), dim3(64 * kWaves), smem, stream, p);
   if ((e = hipGetLastError()) != hipSuccess) return e;
+  return launch_cache_join(p, std::is_same<T, _Float16>::value, stream);
+}
+
+hipError_t launch_cache_join(AttendParams p, bool half, hipStream_t stream) {
   const int out_wgs = p.cache.batch * p.heads;
-  const int spans = scores ? (int)((p.cache.slots() + kSpan - 1) / kSpan) : 0;
-  hipLaunchKernelGGL(cache_join_kernel<T>, dim3(out_wgs + spans * p.cache.kv_heads * p.cache.batch), dim3(256), 0, stream, p, out_wgs, spans);
+  const int spans = p.scores != nullptr ? (int)((p.cache.slots() + kSpan - 1) / kSpan) : 0;
+  void (*fn)(const AttendParams, int, int) = half ? &cache_join_kernel<_Float16> : &cache_join_kernel<__bf16>;
+  hipLaunchKernelGGL(fn, dim3(out_wgs + spans * p.cache.kv_heads * p.cache.batch), dim3(256), 0, stream, p, out_wgs, spans);
   return hipGetLastError();
 }
 

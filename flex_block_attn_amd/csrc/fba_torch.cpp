@@ -19,6 +19,7 @@
 #include <c10/core/Event.h>
 #include <c10/core/impl/VirtualGuardImpl.h>
 #include <c10/hip/HIPStream.h>
+#include <torch/csrc/Dtype.h>
 #include <torch/csrc/Exceptions.h>
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
@@ -47,7 +48,9 @@ constexpr int64_t kXcds = 8;
   X(fba_version) X(fba_last_error) X(fba_split_workspace_bytes) X(fba_lists_cut) X(fba_pair_slots_bounds) X(fba_tile_slots_bounds)        \
   X(fba_fwd) X(fba_fwd_tiled) X(fba_fwd_blocks) X(fba_fwd_blocks_use) X(fba_fwd_mask_copy) X(fba_fwd_takes_mask) X(fba_bwd_mask) X(fba_bwd_takes_mask) X(fba_bwd) X(fba_bwd_handover) X(fba_bwd_tiled_cut) X(fba_bwd_dense) \
   X(fba_resize_rows) X(fba_resize_mask) X(fba_window_fwd) X(fba_window_workspace_bytes) X(fba_window_bwd_apart) \
-  X(fba_cache_append) X(fba_cache_attn_workspace_bytes) X(fba_cache_attn) X(fba_cache_evict_workspace_bytes) X(fba_cache_evict)
+  X(fba_cache_append) X(fba_cache_attn_workspace_bytes) X(fba_cache_attn) X(fba_cache_evict_workspace_bytes) X(fba_cache_evict) \
+  X(fba_rotary) X(fba_cache_append_rotary) X(fba_cache_read) X(fba_cache4_append) X(fba_cache4_attn_workspace_bytes) X(fba_cache4_attn) \
+  X(fba_cache4_evict_workspace_bytes) X(fba_cache4_evict) X(fba_cache4_read)
 
 struct Library {
 #define DECLARE(f) decltype(&::f) f = nullptr;
@@ -903,10 +906,9 @@ std::vector<at::Tensor> window_backward(const at::Tensor& q, const at::Tensor& k
 }
 
 // ---------------------------------------------------------------------------------------------------------------------
-// the paged cache
+// tensors of a call as Python hands them over
 // ---------------------------------------------------------------------------------------------------------------------
-// Tensors of a call as Python hands them over: nothing where one is no plain tensor.
-bool plain(std::initializer_list<pybind11::handle> objects) {
+bool plain(std::initializer_list<pybind11::handle> objects) {  // nothing but plain tensors and None
   for (pybind11::handle o : objects)
     if (!o.is_none() && !THPVariable_CheckTypeExact(Py_TYPE(o.ptr()))) return false;
   return true;
@@ -916,26 +918,7 @@ at::Tensor tensor_of(pybind11::handle o) { return o.is_none() ? at::Tensor() : a
 bool is_ints(const at::Tensor& t, const at::Tensor& like, int64_t n) {
   return t.device() == like.device() && t.scalar_type() == at::kInt && t.dim() == 1 && t.size(0) == n && t.is_contiguous();
 }
-
-// The cache as the library takes it; false where something does not fit, which Python then reports.
-bool cache_of(const at::Tensor& k, const at::Tensor& v, const at::Tensor& positions, const at::Tensor& weights, const at::Tensor& table, const at::Tensor& lengths,
-              fba_cache* c) {
-  if (!k.defined() || !v.defined() || !table.defined() || !lengths.defined()) return false;
-  if (!k.is_cuda() || k.dim() != 4 || k.size(3) != kHeadDim || !k.is_contiguous() || (k.scalar_type() != at::kBFloat16 && k.scalar_type() != at::kHalf)) return false;
-  if (v.device() != k.device() || v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || !v.is_contiguous()) return false;
-  for (const at::Tensor* t : {&positions, &weights})
-    if (t->defined() && (t->device() != k.device() || t->scalar_type() != (t == &positions ? at::kInt : at::kFloat) || t->sizes() != k.sizes().slice(0, 3) || !t->is_contiguous()))
-      return false;
-  const int64_t page = k.size(2);
-  if (k.numel() == 0 || k.size(0) > 0x7fffffffLL || k.size(1) > 65535 || page < 16 || page > 1 << 28 || (page & (page - 1)) != 0) return false;
-  if (table.device() != k.device() || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || table.numel() == 0) return false;
-  if (table.size(0) > 0x7fffff || table.size(1) * page > 1LL << 28 || !is_ints(lengths, k, table.size(0))) return false;
-  for (const at::Tensor* t : {&k, &v, &positions, &weights})
-    if (t->defined() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) != 0) return false;
-  *c = {k.data_ptr(), v.data_ptr(), positions.defined() ? positions.data_ptr<int32_t>() : nullptr, weights.defined() ? weights.data_ptr<float>() : nullptr,
-        table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), k.size(0), (int32_t)k.size(1), (int32_t)page, (int32_t)table.size(0), (int32_t)table.size(1)};
-  return true;
-}
+const int32_t* ints_of(const at::Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; }
 
 bool wants_grad(std::initializer_list<const at::Tensor*> tensors) {
   if (!at::GradMode::is_enabled()) return false;
@@ -950,76 +933,289 @@ void written(std::initializer_list<const at::Tensor*> tensors) {
     if (t->defined() && !t->is_inference()) torch::autograd::impl::bump_version(*t);  // (what is made in inference mode has no version)
 }
 
+bool is_type(at::ScalarType t) { return t == at::kBFloat16 || t == at::kHalf; }
+
+// ---------------------------------------------------------------------------------------------------------------------
+// positions by rotation
+// ---------------------------------------------------------------------------------------------------------------------
+struct Rotation {
+  at::Tensor turns, axes, at;  // `at` undefined: none
+  int64_t n_axes;
+  bool interleaved;
+};
+
+// Do the kernels take it, on `like`'s device, for so many sequences of so many tokens?
+bool takes_rotation(const Rotation& r, const at::Tensor& like, int64_t batch, int64_t tokens) {
+  if (!r.turns.defined() || !r.axes.defined() || r.turns.device() != like.device() || r.turns.scalar_type() != at::kLong || r.turns.dim() != 1 || !r.turns.is_contiguous()) return false;
+  const int64_t pairs = r.turns.size(0);
+  if (pairs < 8 || pairs > kHeadDim / 2 || pairs % 8 != 0 || !is_ints(r.axes, like, pairs) || r.n_axes < 1 || r.n_axes > 8) return false;
+  if (!r.at.defined()) return true;
+  const at::Tensor& t = r.at;
+  if (t.device() != like.device() || t.scalar_type() != at::kInt || !t.is_contiguous() || (t.dim() != 2 && t.dim() != 3)) return false;
+  return (t.dim() == 2 || t.size(0) == batch) && t.size(-2) == tokens && t.size(-1) == r.n_axes;
+}
+fba_rotation rotation_of(const Rotation& r) {
+  const bool each = r.at.defined() && r.at.dim() == 3;
+  return {r.turns.data_ptr<int64_t>(), r.axes.data_ptr<int32_t>(), ints_of(r.at), each ? r.at.size(1) * r.at.size(2) : 0, (int32_t)r.turns.size(0), (int32_t)r.n_axes, r.interleaved};
+}
+
+at::Tensor like_rows(const at::Tensor& t) {
+  at::Tensor out = at::empty_like(t);
+  return takes_strides(out) ? out : at::empty(t.sizes(), t.options());
+}
+
+// Both turned, in one launch; either may be undefined.
+std::pair<at::Tensor, at::Tensor> run_rotary(const at::Tensor& q, const at::Tensor& k, const Rotation& r, bool inverse) {
+  const at::Tensor &a = q.defined() ? q : k, &b = q.defined() ? k : q;
+  const c10::DeviceGuard guard(a.device());
+  at::Tensor a_out = like_rows(a), b_out = b.defined() ? like_rows(b) : at::Tensor();
+  if (a.numel() > 0) {
+    const bool both = b.defined() && b.numel() > 0;
+    const fba_strided sa = strided(a), sao = strided(a_out), sb = both ? strided(b) : sa, sbo = both ? strided(b_out) : sao;
+    const fba_rotation rotation = rotation_of(r);
+    check(lib.fba_rotary(&sa, &sao, both ? &sb : nullptr, both ? &sbo : nullptr, &rotation, inverse, size32(a, 0), size32(a, 1), both ? size32(b, 1) : 0, size32(a, 2), kHeadDim, type_of(a),
+                         current_stream(a)));
+  } else if (b.defined() && b.numel() > 0) {
+    b_out = run_rotary(b, at::Tensor(), r, inverse).first;
+  }
+  return q.defined() ? std::make_pair(a_out, b_out) : std::make_pair(b_out, a_out);
+}
+
+// The rotation is linear, and its gradient the rotation back: as often as it is asked for.
+using MaybeTensor = c10::optional<at::Tensor>;
+MaybeTensor maybe(const at::Tensor& t) { return t.defined() ? MaybeTensor(t) : c10::nullopt; }
+struct Rotary : torch::autograd::Function<Rotary> {
+  // (an argument that may be missing is an optional one: the node asks all others for their device)
+  static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& q, const MaybeTensor& maybe_k, const at::Tensor& turns, const at::Tensor& axes,
+                                                const MaybeTensor& maybe_at, int64_t n_axes, bool interleaved, bool inverse) {
+    const at::Tensor k = maybe_k.value_or(at::Tensor()), at = maybe_at.value_or(at::Tensor());
+    auto [q_out, k_out] = run_rotary(q, k, {turns, axes, at, n_axes, interleaved}, inverse);
+    ctx->set_materialize_grads(false);
+    ctx->save_for_backward({turns, axes, at});
+    ctx->saved_data["args"] = std::vector<int64_t>{n_axes, interleaved, inverse, k.defined()};
+    ctx->saved_data["sizes"] = q.sizes().vec();
+    return k.defined() ? torch::autograd::variable_list{q_out, k_out} : torch::autograd::variable_list{q_out};
+  }
+  static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list grads) {
+    const auto saved = ctx->get_saved_variables();
+    const auto args = ctx->saved_data["args"].toIntVector();
+    const auto sizes = ctx->saved_data["sizes"].toIntVector();
+    torch::autograd::variable_list out(8);
+    at::Tensor g[2];
+    for (int i = 0; i < 2; ++i) {
+      if (i < (int)grads.size() && grads[i].defined() && ctx->needs_input_grad(i)) g[i] = grads[i];
+      if (g[i].defined() && !takes_strides(g[i])) g[i] = g[i].contiguous();
+    }
+    if (!g[0].defined() && !g[1].defined()) return out;
+    const Rotation r{saved[0], saved[1], saved[2], args[0], args[1] != 0};
+    const at::Tensor& some = g[0].defined() ? g[0] : g[1];
+    TORCH_CHECK_VALUE(takes_rotation(r, some, sizes[0], sizes[2]), "saved tensors must come back as they were");
+    refuse_nodes_of_the_default_stream(some);
+    if (at::GradMode::is_enabled()) {
+      const auto turned = apply(some, g[0].defined() ? maybe(g[1]) : c10::nullopt, saved[0], saved[1], maybe(saved[2]), args[0], args[1] != 0, args[2] == 0);
+      out[g[0].defined() ? 0 : 1] = turned[0];
+      if (g[0].defined() && g[1].defined()) out[1] = turned[1];
+    } else {
+      std::tie(out[0], out[1]) = run_rotary(g[0], g[1], r, args[2] == 0);
+    }
+    return out;
+  }
+};
+
+using Turned = std::tuple<at::Tensor, MaybeTensor>;
+Turned turned_of(const at::Tensor& q, const at::Tensor& k) { return {q, maybe(k)}; }
+
+// rotary_func for arguments that need no preparation; nothing for all others, which Python then prepares or reports.
+c10::optional<Turned> rotary(pybind11::handle q_, pybind11::handle k_, pybind11::handle turns_, pybind11::handle axes_, pybind11::handle n_axes, pybind11::handle interleaved, pybind11::handle at_,
+                             bool inverse) {
+  Rotation r;
+  if (!plain({q_, k_, turns_, axes_, at_}) || !int32_of(n_axes, -1, &r.n_axes) || !PyBool_Check(interleaved.ptr())) return c10::nullopt;
+  r.interleaved = interleaved.ptr() == Py_True;
+  const at::Tensor q = tensor_of(q_), k = tensor_of(k_);
+  r.turns = tensor_of(turns_);
+  r.axes = tensor_of(axes_);
+  r.at = tensor_of(at_);
+  pybind11::gil_scoped_release no_gil;
+  if (!q.defined() || (k.defined() ? transformed({&q, &k}) : transformed({&q}))) return c10::nullopt;
+  for (const at::Tensor* t : {&q, &k})
+    if (t->defined() && (!t->is_cuda() || t->device() != q.device() || t->scalar_type() != q.scalar_type() || !takes_strides(*t) || t->size(0) != q.size(0) || t->size(2) != q.size(2) ||
+                         t->size(1) > 65535))
+      return c10::nullopt;
+  if (!is_type(q.scalar_type()) || q.numel() == 0 || !takes_rotation(r, q, q.size(0), q.size(2))) return c10::nullopt;
+  if (wants_grad({&q, &k})) {
+    const auto out = Rotary::apply(q, maybe(k), r.turns, r.axes, maybe(r.at), r.n_axes, r.interleaved, inverse);
+    return turned_of(out[0], k.defined() ? out[1] : at::Tensor());
+  }
+  const auto out = run_rotary(q, k, r, inverse);
+  return turned_of(out.first, out.second);
+}
+
+// For the Python autograd function; arguments have been checked and prepared.
+Turned rotary_forward(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& turns, const at::Tensor& axes, int64_t n_axes, bool interleaved,
+                      const c10::optional<at::Tensor>& at, bool inverse) {
+  const Rotation r{turns, axes, at.value_or(at::Tensor()), n_axes, interleaved};
+  TORCH_CHECK_VALUE(q.numel() == 0 || (takes_strides(q) && (!k || k->numel() == 0 || takes_strides(*k)) && takes_rotation(r, q, q.size(0), q.size(2))), "arguments are not as they were");
+  refuse_nodes_of_the_default_stream(q);  // (backward comes through here too)
+  const auto out = run_rotary(q, k.value_or(at::Tensor()), r, inverse);
+  return turned_of(out.first, out.second);
+}
+
+// ---------------------------------------------------------------------------------------------------------------------
+// the paged cache
+// ---------------------------------------------------------------------------------------------------------------------
+// A cache as Python hands it over, and as the library takes it.
+struct Cache {
+  at::Tensor k, v, k_scales, v_scales, positions, weights, table, lengths;
+  at::ScalarType type;  // of the values
+  fba_cache4 c{};
+  bool held() const { return k_scales.defined(); }
+  const fba_cache* rows() const { return &c.cache; }
+};
+
+// False where something does not fit, which Python then reports.
+bool take_cache(Cache& cache) {
+  const at::Tensor &k = cache.k, &v = cache.v, &positions = cache.positions, &weights = cache.weights, &table = cache.table, &lengths = cache.lengths;
+  if (!k.defined() || !v.defined() || !table.defined() || !lengths.defined() || cache.k_scales.defined() != cache.v_scales.defined()) return false;
+  const bool held = cache.held();
+  if (!k.is_cuda() || k.dim() != 4 || k.size(3) != (held ? kHeadDim / 2 : kHeadDim) || !k.is_contiguous() || !is_type(cache.type) || k.scalar_type() != (held ? at::kByte : cache.type)) return false;
+  if (v.device() != k.device() || v.scalar_type() != k.scalar_type() || v.sizes() != k.sizes() || !v.is_contiguous()) return false;
+  for (const at::Tensor* t : {&positions, &weights})
+    if (t->defined() && (t->device() != k.device() || t->scalar_type() != (t == &positions ? at::kInt : at::kFloat) || t->sizes() != k.sizes().slice(0, 3) || !t->is_contiguous()))
+      return false;
+  for (const at::Tensor* t : {&cache.k_scales, &cache.v_scales})
+    if (held && (t->device() != k.device() || t->scalar_type() != at::kByte || t->dim() != 4 || t->sizes().slice(0, 3) != k.sizes().slice(0, 3) || t->size(3) != kHeadDim / 32 || !t->is_contiguous()))
+      return false;
+  const int64_t page = k.size(2);
+  if (k.numel() == 0 || k.size(0) > 0x7fffffffLL || k.size(1) > 65535 || page < 16 || page > 1 << 28 || (page & (page - 1)) != 0) return false;
+  if (table.device() != k.device() || table.scalar_type() != at::kInt || table.dim() != 2 || !table.is_contiguous() || table.numel() == 0) return false;
+  if (table.size(0) > 0x7fffff || table.size(1) * page > 1LL << 28 || !is_ints(lengths, k, table.size(0))) return false;
+  for (const at::Tensor* t : std::initializer_list<const at::Tensor*>{&k, &v, &positions, &weights, &cache.k_scales, &cache.v_scales})
+    if (t->defined() && (reinterpret_cast<uintptr_t>(t->data_ptr()) & 15) != 0) return false;
+  cache.c.cache = {k.data_ptr(), v.data_ptr(), positions.defined() ? positions.data_ptr<int32_t>() : nullptr, weights.defined() ? weights.data_ptr<float>() : nullptr,
+                   table.data_ptr<int32_t>(), lengths.data_ptr<int32_t>(), k.size(0), (int32_t)k.size(1), (int32_t)page, (int32_t)table.size(0), (int32_t)table.size(1)};
+  if (held) {
+    cache.c.k_scales = cache.k_scales.data_ptr<uint8_t>();
+    cache.c.v_scales = cache.v_scales.data_ptr<uint8_t>();
+  }
+  return true;
+}
+
+// What Python hands over of a cache: k, v, k_scales, v_scales (None: 16 bits), positions, weights, table, lengths, and the type of its values.
+bool unpack_cache(const pybind11::tuple& given, Cache& cache) {
+  at::Tensor* const to[8] = {&cache.k, &cache.v, &cache.k_scales, &cache.v_scales, &cache.positions, &cache.weights, &cache.table, &cache.lengths};
+  if (given.size() != 9 || !THPDtype_Check(PyTuple_GET_ITEM(given.ptr(), 8))) return false;
+  for (int i = 0; i < 8; ++i) {
+    const pybind11::handle o = PyTuple_GET_ITEM(given.ptr(), i);
+    if (!plain({o})) return false;
+    *to[i] = tensor_of(o);
+  }
+  cache.type = reinterpret_cast<THPDtype*>(PyTuple_GET_ITEM(given.ptr(), 8))->scalar_type;
+  return true;
+}
+
 // The entry points of cache.py: nothing for arguments that do not fit, which Python then prepares or reports.
-c10::optional<at::Tensor> cache_attention(pybind11::handle q_, pybind11::handle k_, pybind11::handle v_, pybind11::handle weights_, pybind11::handle table_,
-                                          pybind11::handle lengths_, pybind11::handle window_, pybind11::handle sinks_, bool accumulate) {
+c10::optional<at::Tensor> cache_attention(pybind11::handle q_, const pybind11::tuple& given, pybind11::handle window_, pybind11::handle sinks_, bool accumulate) {
   int64_t window, sinks;
-  if (!plain({q_, k_, v_, weights_, table_, lengths_}) || !int32_of(window_, kNoWindow, &window) || !int32_of(sinks_, -1, &sinks) || window < 1 || sinks < 0) return c10::nullopt;
-  const at::Tensor q = tensor_of(q_), k = tensor_of(k_), v = tensor_of(v_), weights = tensor_of(weights_), table = tensor_of(table_), lengths = tensor_of(lengths_);
+  Cache cache;
+  if (!plain({q_}) || !unpack_cache(given, cache) || !int32_of(window_, kNoWindow, &window) || !int32_of(sinks_, -1, &sinks) || window < 1 || sinks < 0) return c10::nullopt;
+  const at::Tensor q = tensor_of(q_);
   const bool windowed = !window_.is_none();
   pybind11::gil_scoped_release no_gil;
-  fba_cache cache;
-  if (!cache_of(k, v, at::Tensor(), weights, table, lengths, &cache) || (accumulate && (!weights.defined() || windowed))) return c10::nullopt;
-  if (!q.defined() || q.device() != k.device() || q.scalar_type() != k.scalar_type() || !takes_strides(q) || q.size(0) != cache.batch || q.size(2) != 1 || q.numel() == 0 ||
-      q.size(1) % cache.kv_heads != 0 || q.size(1) > 65535)
+  if (!take_cache(cache) || (accumulate && (!cache.weights.defined() || windowed))) return c10::nullopt;
+  if (!q.defined() || q.device() != cache.k.device() || q.scalar_type() != cache.type || !takes_strides(q) || q.size(0) != cache.rows()->batch || q.size(2) != 1 || q.numel() == 0 ||
+      q.size(1) % cache.rows()->kv_heads != 0 || q.size(1) > 65535)
     return c10::nullopt;
-  if (transformed({&q, &k, &v}) || wants_grad({&q, &k, &v, &weights})) return c10::nullopt;
+  if (transformed({&q, &cache.k, &cache.v}) || wants_grad({&q, &cache.k, &cache.v, &cache.weights})) return c10::nullopt;
   const c10::DeviceGuard guard(q.device());
   at::Tensor o = at::empty(q.sizes(), q.options());
-  const int64_t bytes = lib.fba_cache_attn_workspace_bytes(&cache, q.size(1), accumulate);
+  const int64_t bytes = cache.held() ? lib.fba_cache4_attn_workspace_bytes(&cache.c, q.size(1), accumulate) : lib.fba_cache_attn_workspace_bytes(cache.rows(), q.size(1), accumulate);
   if (bytes < 0) raise_call_error(FBA_ERR_UNSUPPORTED);
   SplitWorkspace ws(q, bytes);
   const fba_strided sq = strided(q), so = strided(o);
-  check(lib.fba_cache_attn(&cache, &sq, &so, q.size(1), window, sinks, accumulate, type_of(q), ws.ptr(), bytes, current_stream(q)));
-  if (accumulate) written({&weights});
+  if (cache.held()) check(lib.fba_cache4_attn(&cache.c, &sq, &so, q.size(1), window, sinks, accumulate, type_of(q), ws.ptr(), bytes, current_stream(q)));
+  else check(lib.fba_cache_attn(cache.rows(), &sq, &so, q.size(1), window, sinks, accumulate, type_of(q), ws.ptr(), bytes, current_stream(q)));
+  if (accumulate) written({&cache.weights});
   return o;
 }
 
-c10::optional<at::Tensor> cache_append(pybind11::handle cache_k_, pybind11::handle cache_v_, pybind11::handle positions_, pybind11::handle weights_, pybind11::handle table_,
-                                       pybind11::handle lengths_, pybind11::handle k_, pybind11::handle v_, pybind11::handle counts_, pybind11::handle first_,
-                                       pybind11::handle given_) {
-  if (!plain({cache_k_, cache_v_, positions_, weights_, table_, lengths_, k_, v_, counts_, first_, given_})) return c10::nullopt;
-  const at::Tensor ck = tensor_of(cache_k_), cv = tensor_of(cache_v_), positions = tensor_of(positions_), weights = tensor_of(weights_), table = tensor_of(table_),
-                   lengths = tensor_of(lengths_), k = tensor_of(k_), v = tensor_of(v_), counts = tensor_of(counts_), first = tensor_of(first_), given = tensor_of(given_);
+// turns None: nothing turns (16 bits: then there is no q either).  Returns the new lengths and, where it is given, q turned.
+c10::optional<Turned> cache_append(const pybind11::tuple& given, pybind11::handle k_, pybind11::handle v_, pybind11::handle counts_, pybind11::handle first_, pybind11::handle weights_,
+                                   pybind11::handle q_, pybind11::handle turns_, pybind11::handle axes_, pybind11::handle n_axes, pybind11::handle interleaved, pybind11::handle at_) {
+  Cache cache;
+  Rotation r;
+  if (!unpack_cache(given, cache) || !plain({k_, v_, counts_, first_, weights_, q_, turns_, axes_, at_}) || !int32_of(n_axes, 0, &r.n_axes)) return c10::nullopt;
+  if (!interleaved.is_none() && !PyBool_Check(interleaved.ptr())) return c10::nullopt;
+  r.interleaved = interleaved.ptr() == Py_True;
+  const at::Tensor k = tensor_of(k_), v = tensor_of(v_), counts = tensor_of(counts_), first = tensor_of(first_), new_weights = tensor_of(weights_), q = tensor_of(q_);
+  r.turns = tensor_of(turns_);
+  r.axes = tensor_of(axes_);
+  r.at = tensor_of(at_);
   pybind11::gil_scoped_release no_gil;
-  fba_cache cache;
-  if (!cache_of(ck, cv, positions, weights, table, lengths, &cache) || !k.defined() || !v.defined()) return c10::nullopt;
-  for (const at::Tensor* t : {&k, &v})
-    if (t->device() != ck.device() || t->scalar_type() != ck.scalar_type() || !takes_strides(*t) || t->sizes() != k.sizes()) return c10::nullopt;
-  if (k.size(0) != cache.batch || k.size(1) != cache.kv_heads || k.size(2) < 1 || k.size(2) > 1 << 28) return c10::nullopt;
-  if ((counts.defined() && !is_ints(counts, ck, cache.batch)) || (first.defined() && (!positions.defined() || !is_ints(first, ck, cache.batch)))) return c10::nullopt;
-  if (given.defined() && (!weights.defined() || given.device() != ck.device() || given.scalar_type() != at::kFloat || given.sizes() != k.sizes().slice(0, 3) || !given.is_contiguous()))
+  if (!take_cache(cache) || !k.defined() || !v.defined()) return c10::nullopt;
+  const int64_t batch = cache.rows()->batch;
+  for (const at::Tensor* t : {&k, &v, &q})
+    if (t->defined() && (t->device() != cache.k.device() || t->scalar_type() != cache.type || !takes_strides(*t))) return c10::nullopt;
+  if (v.sizes() != k.sizes() || k.size(0) != batch || k.size(1) != cache.rows()->kv_heads || k.size(2) < 1 || k.size(2) > 1 << 28) return c10::nullopt;
+  const bool turns = r.turns.defined();
+  if (q.defined() && (!turns || q.size(0) != batch || q.size(2) != k.size(2) || q.size(1) < 1 || q.size(1) > 65535)) return c10::nullopt;
+  if (turns ? !takes_rotation(r, k, batch, k.size(2)) : r.axes.defined() || r.at.defined()) return c10::nullopt;
+  // (where nothing has positions, they say nothing)
+  if ((counts.defined() && !is_ints(counts, cache.k, batch)) || (first.defined() && ((!cache.positions.defined() && !turns) || !is_ints(first, cache.k, batch)))) return c10::nullopt;
+  if (new_weights.defined() && (!cache.weights.defined() || new_weights.device() != cache.k.device() || new_weights.scalar_type() != at::kFloat ||
+                                new_weights.sizes() != k.sizes().slice(0, 3) || !new_weights.is_contiguous()))
     return c10::nullopt;
-  if (transformed({&ck, &cv, &k, &v}) || wants_grad({&ck, &cv, &weights, &k, &v, &given})) return c10::nullopt;
-  const c10::DeviceGuard guard(ck.device());
-  at::Tensor out = at::empty_like(lengths);
-  const fba_strided sk = strided(k), sv = strided(v);
-  auto ints_of = [](const at::Tensor& t) { return t.defined() ? t.data_ptr<int32_t>() : nullptr; };
-  check(lib.fba_cache_append(&cache, &sk, &sv, ints_of(counts), ints_of(first), given.defined() ? given.data_ptr<float>() : nullptr, k.size(2), out.data_ptr<int32_t>(),
-                             current_stream(ck)));
-  written({&ck, &cv, &positions, &weights});
+  if (transformed({&cache.k, &cache.v, &k, &v}) || (q.defined() && transformed({&q})) || wants_grad({&cache.k, &cache.v, &cache.weights, &k, &v, &new_weights, &q})) return c10::nullopt;
+  const c10::DeviceGuard guard(cache.k.device());
+  at::Tensor out = at::empty_like(cache.lengths), q_out = q.defined() ? like_rows(q) : at::Tensor();
+  const fba_strided sk = strided(k), sv = strided(v), sq = q.defined() ? strided(q) : sk, sqo = q.defined() ? strided(q_out) : sk;
+  const float* const w = new_weights.defined() ? new_weights.data_ptr<float>() : nullptr;
+  const fba_rotation rotation = turns ? rotation_of(r) : fba_rotation{};
+  const int32_t heads = q.defined() ? (int32_t)q.size(1) : 0;
+  if (cache.held())
+    check(lib.fba_cache4_append(&cache.c, &sk, &sv, q.defined() ? &sq : nullptr, q.defined() ? &sqo : nullptr, heads, turns ? &rotation : nullptr, ints_of(counts), ints_of(first), w, k.size(2),
+                                type_of(k), out.data_ptr<int32_t>(), current_stream(cache.k)));
+  else if (turns)
+    check(lib.fba_cache_append_rotary(cache.rows(), &sk, &sv, q.defined() ? &sq : nullptr, q.defined() ? &sqo : nullptr, heads, &rotation, ints_of(counts), ints_of(first), w, k.size(2), type_of(k),
+                                      out.data_ptr<int32_t>(), current_stream(cache.k)));
+  else
+    check(lib.fba_cache_append(cache.rows(), &sk, &sv, ints_of(counts), ints_of(first), w, k.size(2), out.data_ptr<int32_t>(), current_stream(cache.k)));
+  written({&cache.k, &cache.v, &cache.k_scales, &cache.v_scales, &cache.positions, &cache.weights});
+  return turned_of(out, q_out);
+}
+
+c10::optional<at::Tensor> cache_evict(const pybind11::tuple& given, pybind11::handle budget_, pybind11::handle recent_, pybind11::handle sinks_) {
+  int64_t budget, recent, sinks;
+  Cache cache;
+  if (!unpack_cache(given, cache) || !int32_of(budget_, -1, &budget) || !int32_of(recent_, -1, &recent) || !int32_of(sinks_, -1, &sinks) || budget < 1 || recent < 0 || sinks < 0 ||
+      recent + sinks > budget)
+    return c10::nullopt;
+  pybind11::gil_scoped_release no_gil;
+  if (!cache.positions.defined() || !cache.weights.defined() || !take_cache(cache)) return c10::nullopt;
+  if (transformed({&cache.k, &cache.v}) || wants_grad({&cache.k, &cache.v, &cache.weights})) return c10::nullopt;
+  const c10::DeviceGuard guard(cache.k.device());
+  const int64_t bytes = cache.held() ? lib.fba_cache4_evict_workspace_bytes(&cache.c, budget) : lib.fba_cache_evict_workspace_bytes(cache.rows(), budget);
+  if (bytes < 0) raise_call_error(FBA_ERR_UNSUPPORTED);
+  SplitWorkspace ws(cache.k, bytes);
+  at::Tensor out = at::empty_like(cache.lengths);
+  if (cache.held()) check(lib.fba_cache4_evict(&cache.c, budget, recent, sinks, out.data_ptr<int32_t>(), ws.ptr(), bytes, current_stream(cache.k)));
+  else check(lib.fba_cache_evict(cache.rows(), budget, recent, sinks, out.data_ptr<int32_t>(), ws.ptr(), bytes, current_stream(cache.k)));
+  written({&cache.k, &cache.v, &cache.k_scales, &cache.v_scales, &cache.positions, &cache.weights});
   return out;
 }
 
-c10::optional<at::Tensor> cache_evict(pybind11::handle k_, pybind11::handle v_, pybind11::handle positions_, pybind11::handle weights_, pybind11::handle table_,
-                                      pybind11::handle lengths_, pybind11::handle budget_, pybind11::handle recent_, pybind11::handle sinks_) {
-  int64_t budget, recent, sinks;
-  if (!plain({k_, v_, positions_, weights_, table_, lengths_}) || !int32_of(budget_, -1, &budget) || !int32_of(recent_, -1, &recent) || !int32_of(sinks_, -1, &sinks) || budget < 1 ||
-      recent < 0 || sinks < 0 || recent + sinks > budget)
-    return c10::nullopt;
-  const at::Tensor k = tensor_of(k_), v = tensor_of(v_), positions = tensor_of(positions_), weights = tensor_of(weights_), table = tensor_of(table_), lengths = tensor_of(lengths_);
+c10::optional<std::tuple<at::Tensor, at::Tensor>> cache_read(const pybind11::tuple& given, pybind11::handle slots_, pybind11::handle first_) {
+  int64_t slots, first;
+  Cache cache;
+  if (!unpack_cache(given, cache) || !int32_of(slots_, -1, &slots) || !int32_of(first_, -1, &first) || slots < 1 || slots > 1 << 28 || first < 0 || first > 1 << 28) return c10::nullopt;
   pybind11::gil_scoped_release no_gil;
-  fba_cache cache;
-  if (!positions.defined() || !weights.defined() || !cache_of(k, v, positions, weights, table, lengths, &cache)) return c10::nullopt;
-  if (transformed({&k, &v}) || wants_grad({&k, &v, &weights})) return c10::nullopt;
-  const c10::DeviceGuard guard(k.device());
-  const int64_t bytes = lib.fba_cache_evict_workspace_bytes(&cache, budget);
-  if (bytes < 0) raise_call_error(FBA_ERR_UNSUPPORTED);
-  SplitWorkspace ws(k, bytes);
-  at::Tensor out = at::empty_like(lengths);
-  check(lib.fba_cache_evict(&cache, budget, recent, sinks, out.data_ptr<int32_t>(), ws.ptr(), bytes, current_stream(k)));
-  written({&k, &v, &positions, &weights});
-  return out;
+  if (!take_cache(cache) || transformed({&cache.k, &cache.v}) || wants_grad({&cache.k, &cache.v})) return c10::nullopt;
+  const c10::DeviceGuard guard(cache.k.device());
+  const auto options = cache.k.options().dtype(cache.type);
+  at::Tensor k = at::empty({cache.rows()->batch, cache.rows()->kv_heads, slots, kHeadDim}, options), v = at::empty_like(k);
+  const fba_strided sk = strided(k), sv = strided(v);
+  if (cache.held()) check(lib.fba_cache4_read(&cache.c, first, slots, &sk, &sv, type_of(k), current_stream(k)));
+  else check(lib.fba_cache_read(cache.rows(), first, slots, &sk, &sv, type_of(k), current_stream(k)));
+  return std::make_tuple(k, v);
 }
 
 }  // namespace
@@ -1037,6 +1233,9 @@ PYBIND11_MODULE(TORCH_EXTENSION_NAME, m) {
   m.def("cache_attention", &cache_attention);
   m.def("cache_append", &cache_append);
   m.def("cache_evict", &cache_evict);
+  m.def("cache_read", &cache_read);
+  m.def("rotary", &rotary);
+  m.def("rotary_forward", &rotary_forward, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("window_attention", &window_attention);
   m.def("window_forward", &window_forward, pybind11::call_guard<pybind11::gil_scoped_release>());
   m.def("window_backward", &window_backward, pybind11::call_guard<pybind11::gil_scoped_release>());

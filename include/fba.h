@@ -36,7 +36,7 @@ extern "C" {
 
 /* Library version: major * 1000 + minor; the minor number goes up whenever an argument list in this header changes, so a
  * binding can refuse a library built from another header (flex_block_attn_amd/_lib.py does). */
-#define FBA_VERSION 2013
+#define FBA_VERSION 2014
 int32_t fba_version(void);
 
 /* Message for the last non-OK return on the calling thread ("" if none). The pointer stays valid until the next
@@ -452,6 +452,65 @@ int32_t fba_cache_attn(const fba_cache* cache, const fba_strided* q, const fba_s
                        int32_t type, void* ws, int64_t ws_bytes, void* hip_stream);
 int64_t fba_cache_evict_workspace_bytes(const fba_cache* cache, int32_t budget);
 int32_t fba_cache_evict(const fba_cache* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream);
+
+/*
+ * Positions by rotation (no counterpart in the reference).
+ *
+ * Pair i of a row (a, b), columns (2i, 2i + 1) if interleaved, (i, i + pairs) if not, becomes (a cos w - b sin w, a sin w + b cos w), w = 2 pi turns[i] / 2^64 * p[axes[i]], where p is where
+ * the row's token stands on each of n_axes axes (time, height and width of a video's token; one axis for text).  The columns from 2 * pairs on stay as they are.
+ *   turns  [pairs] the turns that one step on the pair's axis makes, times 2^64, modulo 2^64: the angle of any 32-bit position, below zero too, is exact to 2^-64 of a turn for it
+ *   axes   [pairs] which axis; one that is not below n_axes counts as the last
+ *   at     int32 [batch, tokens, n_axes], sequences at_batch elements apart (0: all alike), or null: where tokens stand is then stated with each function, on all axes alike
+ * All three in device memory; pairs a multiple of 8, 64 at most, n_axes 8 at most.
+ *
+ * fba_rotary: q_out = q [B, Hq, S, 128] turned, k_out = k [B, Hk, S, 128] alike (null, with Hk = 0: q alone), by -w if inverse != 0, which is also the gradient.  at null: row t stands
+ *   at t.  Worked out in fp32 (angles as stated), rounded once.  All rows are turned, those of padding too.  Tensors with strides as for fba_window_fwd; outputs must not overlap inputs.
+ *   B * S may be 2^27 at most.
+ */
+typedef struct {
+  const int64_t* turns;
+  const int32_t* axes;
+  const int32_t* at;
+  int64_t at_batch;
+  int32_t pairs, n_axes, interleaved;
+} fba_rotation;
+int32_t fba_rotary(const fba_strided* q, const fba_strided* q_out, const fba_strided* k, const fba_strided* k_out, const fba_rotation* rotation, int32_t inverse, int32_t B, int32_t Hq,
+                   int32_t Hk, int32_t S, int32_t head_dim, int32_t type, void* hip_stream);
+
+/*
+ * A paged cache in 4 bits: `cache` as above, but k and v [pages, kv_heads, page_size, 64] bytes, value 2j of a row in the low half of byte j, 2j + 1 in the high one, and k_scales, v_scales
+ * [pages, kv_heads, page_size, 4], one for each 32 values.  A value is m * 2^(scale - 127), m = 0, 0.5, 1, 1.5, 2, 3, 4, 6 for the low three bits 0 .. 7, below zero with the fourth;
+ * scale 255: all 32 are no numbers.  What is appended is rounded so: e = floor(log2(the largest of the 32)) - 2, one more from 1.75 of its binade on, brought into -125 .. 125 (type
+ * FBA_BF16) or -13 .. 13 (FBA_FP16), scale = e + 127, or 255 where one of the 32 is infinite or no number; m to the nearest, ties to the even code.  So a value v is off by at most
+ * max(2^(e-2), |v| / 4) (2^(e-2) up to 2^(e+1), half of a step above), but for fp16 values above 7 * 2^13, which become 6 * 2^13, bf16 ones above 7 * 2^125 alike, and values below the
+ * smallest normal number of the type, which may become zero.  type is that of q, k, v and o, and fixed for a pool: its values are exact in it.
+ *
+ * fba_cache4_append, fba_cache4_attn, fba_cache4_evict: as the functions of 16 bits, attention over the values that the pool stands for.  fba_cache4_append takes a rotation too (null: none).
+ * fba_cache_append_rotary: as fba_cache_append, with k turned on the way, and q_out = q [batch, heads, tokens, 128] turned alike (null, with heads = 0: there is none), the rows behind
+ *   counts[b] too, no numbers for a sequence whose length or count makes no sense.  Where rotation->at is null, the token t of sequence b stands at first[b] + t (first null:
+ *   lengths[b] + t) on all axes; positions of the cache are that in either case.  A k that goes into 4 bits is turned in 64 bits, so that it is rounded once.
+ * fba_cache_read, fba_cache4_read: slots first .. first + slots - 1 of every sequence to k, v [batch, kv_heads, slots, 128]: what a prompt's next chunk attends to with
+ *   fba_window_fwd.  Zeros behind the sequence's length, no numbers in the rows of a page outside of the pool, and in all rows of a sequence whose length makes no sense.
+ * batch may be 2^22 and batch * tokens 2^27 at most where tokens are appended, batch * kv_heads * ceil(slots / 64) 2^24 - 1 where slots are read.
+ */
+typedef struct {
+  fba_cache cache;
+  uint8_t* k_scales;
+  uint8_t* v_scales;
+} fba_cache4;
+int32_t fba_cache_append_rotary(const fba_cache* cache, const fba_strided* k, const fba_strided* v, const fba_strided* q, const fba_strided* q_out, int32_t heads,
+                                const fba_rotation* rotation, const int32_t* counts, const int32_t* first, const float* weights, int32_t tokens, int32_t type,
+                                int32_t* lengths_out, void* hip_stream);
+int32_t fba_cache_read(const fba_cache* cache, int32_t first, int32_t slots, const fba_strided* k, const fba_strided* v, int32_t type, void* hip_stream);
+int32_t fba_cache4_append(const fba_cache4* cache, const fba_strided* k, const fba_strided* v, const fba_strided* q, const fba_strided* q_out, int32_t heads,
+                          const fba_rotation* rotation, const int32_t* counts, const int32_t* first, const float* weights, int32_t tokens, int32_t type, int32_t* lengths_out,
+                          void* hip_stream);
+int64_t fba_cache4_attn_workspace_bytes(const fba_cache4* cache, int32_t heads, int32_t accumulate);
+int32_t fba_cache4_attn(const fba_cache4* cache, const fba_strided* q, const fba_strided* o, int32_t heads, int32_t window, int32_t sinks, int32_t accumulate, int32_t type, void* ws,
+                        int64_t ws_bytes, void* hip_stream);
+int64_t fba_cache4_evict_workspace_bytes(const fba_cache4* cache, int32_t budget);
+int32_t fba_cache4_evict(const fba_cache4* cache, int32_t budget, int32_t recent, int32_t sinks, int32_t* lengths_out, void* ws, int64_t ws_bytes, void* hip_stream);
+int32_t fba_cache4_read(const fba_cache4* cache, int32_t first, int32_t slots, const fba_strided* k, const fba_strided* v, int32_t type, void* hip_stream);
 
 /*
  * Diagnostic, no counterpart in the reference: `work_groups` x 4 waves each issue `iters` x 4 independent
