@@ -15,7 +15,7 @@ constexpr float kLazy = 8.f, kNoReference = -3e38f;
 
 inline int head_tiles_of(int group) { return group <= 16 ? 1 : 2; }  // query heads of a work-group, in sixteens (four do not fit the registers of two waves on a SIMD)
 
-constexpr int kResident4 = 4;
+constexpr int kResident4 = 3;  // work-groups on a compute unit, of 4 bits and 16 heads
 
 // Tiles of a sequence that are read: those with sinks, then those from the window's start on.
 struct Tiles {

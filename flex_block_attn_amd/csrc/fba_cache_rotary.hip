@@ -43,20 +43,33 @@ __global__ __launch_bounds__(256) void cache_append_rotary_kernel(const AppendRo
   const int h0 = part * p.per, end = min(h0 + (int)p.per, cache.kv_heads + p.heads);
   if (t >= n && (n >= 0 ? end <= cache.kv_heads : p.heads == 0)) return;  // behind the sequence's last one, and no q
   const int position = (a.first != nullptr ? a.first[b] : len) + t;
+  const int page = t < n ? cache.page_of(b, len + t) : -1;
+  // rows of K and V, two heads ahead
+  const char* const k_from = a.k.ptr + b * a.k.batch + (int64_t)t * a.k.row + c * 16;
+  const char* const v_from = a.v.ptr + b * a.v.batch + (int64_t)t * a.v.row + c * 16;
+  const int kv_end = page >= 0 ? min(end, cache.kv_heads) : h0;
+  x8_of<T> k_rows[2], v_rows[2];
+  auto fetch = [&](int h, int i) {
+    if (h >= kv_end) return;
+    k_rows[i] = *reinterpret_cast<const x8_of<T>*>(k_from + h * a.k.head);
+    v_rows[i] = *reinterpret_cast<const x8_of<T>*>(v_from + h * a.v.head);
+  };
+  fetch(h0, 0);
+  fetch(h0 + 1, 1);
   using F = typename std::conditional<kHeld, double, float>::type;
   Turn<F> turn;
-  if (p.rotation.turns != nullptr) {
-    turn.init(p.rotation, b, t, position, c);
-  } else {
-    turn.on = false;
-  }
   const bool turns = p.rotation.turns != nullptr, interleaved = p.rotation.interleaved != 0;
-  const int page = t < n ? cache.page_of(b, len + t) : -1;
-  if (page >= 0)
-    for (int h = h0; h < min(end, cache.kv_heads); ++h) {
+  turn.on = false;
+  if (turns) turn.init(p.rotation, b, t, position, c);
+  for (int h1 = h0; h1 < kv_end; h1 += 2)
+#pragma unroll
+    for (int i = 0; i < 2; ++i) {
+      const int h = h1 + i;
+      if (h >= kv_end) break;
       const int64_t to = cache.row_of(page, h, len + t);
-      x8_of<T> kr = *reinterpret_cast<const x8_of<T>*>(a.k.ptr + b * a.k.batch + h * a.k.head + (int64_t)t * a.k.row + c * 16);
-      const x8_of<T> vr = *reinterpret_cast<const x8_of<T>*>(a.v.ptr + b * a.v.batch + h * a.v.head + (int64_t)t * a.v.row + c * 16);
+      x8_of<T> kr = k_rows[i];
+      const x8_of<T> vr = v_rows[i];
+      fetch(h + 2, i);
       if constexpr (kHeld) {
         float kf[8], vf[8];
 #pragma unroll
