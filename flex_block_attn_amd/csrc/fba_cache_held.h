@@ -10,26 +10,46 @@ inline constexpr int kScaleLimit = 125;
 template <>
 inline constexpr int kScaleLimit<_Float16> = 13;
 
-// Eight columns of a lane -> their codes; four lanes, from a multiple of four on, have a group.  The scale is the largest value's exponent less two, and one more from 1.75 of its
-// binade on, so that nothing is beyond 7 times the scale and the largest code, 6, is off by less than a seventh; rounding is to the nearest, ties to the even code (the
-// conversion's own).
-template <typename T>
-FBA_DEVICE uint32_t to_4_bits(const float (&x)[8], uint32_t* scale) {
-  uint32_t most = 0;
-#pragma unroll
-  for (int e = 0; e < 8; ++e) most = max(most, __builtin_bit_cast(uint32_t, x[e]) & 0x7fffffffu);
-  most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0xb1, 0xf, 0xf, false));  // the lane beside, in the pair
-  most = max(most, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)most, 0x4e, 0xf, 0xf, false));  // the pair beside, in the four
-  const int e = min(max((int)((most + 0x200000u) >> 23) - 2, 127 - kScaleLimit<T>), 127 + kScaleLimit<T>);
-  *scale = most >= 0x7f800000u ? 255u : (uint32_t)e;
-  const float by = __builtin_bit_cast(float, (uint32_t)e << 23);
-  uint32_t codes = 0;
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0], x[1], by, 0);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2], x[3], by, 1);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4], x[5], by, 2);
-  codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6], x[7], by, 3);
-  return codes;
+// The largest of the four lanes that have a group, from a multiple of four on.
+FBA_DEVICE uint32_t of_group(uint32_t x) {
+  x = max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0xb1, 0xf, 0xf, false));    // the lane beside, in the pair
+  return max(x, (uint32_t)__builtin_amdgcn_update_dpp(0, (int)x, 0x4e, 0xf, 0xf, false));  // the pair beside, in the four
 }
+FBA_DEVICE uint32_t bits_of(float x) { return __builtin_bit_cast(uint32_t, x); }
+
+// Eight columns of a lane -> their codes; four lanes have a group.  The scale is the largest value's exponent less two, and one more from 1.75 of its binade on, so that nothing is
+// beyond 7 times the scale and the largest code, 6, is off by less than a seventh; rounding is to the nearest, ties to the even code (the conversion's own).
+//
+// `off`: how far the values may be from what is meant.  Rounding is monotone, so a code is sure if off less and off more give the same one.
+template <typename T>
+struct To4Bits {
+  uint32_t codes, scale;
+  bool sure;  // whether no code of this lane, and not the group's scale, could be another (a value around zero may be taken for unsure)
+  FBA_DEVICE static uint32_t round(const float (&x)[8], float by, float off) {
+    uint32_t codes = 0;
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[0] + off, x[1] + off, by, 0);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[2] + off, x[3] + off, by, 1);
+    codes = __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[4] + off, x[5] + off, by, 2);
+    return __builtin_amdgcn_cvt_scalef32_pk_fp4_f32(codes, x[6] + off, x[7] + off, by, 3);
+  }
+  template <bool kOff>
+  FBA_DEVICE void hold(const float (&x)[8], float off) {
+    uint32_t most = 0;
+#pragma unroll
+    for (int i = 0; i < 8; ++i) most = max(most, bits_of(x[i]) & 0x7fffffffu);
+    most = of_group(most);
+    const int e = min(max((int)((most + 0x200000u) >> 23) - 2, 127 - kScaleLimit<T>), 127 + kScaleLimit<T>);
+    scale = most >= 0x7f800000u ? 255u : (uint32_t)e;
+    const float by = __builtin_bit_cast(float, (uint32_t)e << 23);
+    if constexpr (kOff) {
+      codes = round(x, by, -off);
+      const float largest = __builtin_bit_cast(float, most);
+      sure = codes == round(x, by, off) && largest < 7.f * by - off && (largest > 3.5f * by + off || e == 127 - kScaleLimit<T>);
+    } else {
+      codes = round(x, by, 0.f);
+    }
+  }
+};
 
 template <typename T>
 struct FromFp4;

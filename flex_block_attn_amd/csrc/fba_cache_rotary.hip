@@ -5,15 +5,16 @@
 #include "fba_cache_held.h"
 #include "fba_turn.h"
 
-#include <type_traits>
-
 namespace fba {
 
 // Work-groups 0 .. batch - 1 work out the new lengths; behind them sixteen lanes have a part of a token's heads, so that sines and cosines are worked out once for all of them:
-// first the kv heads, K and V together, then those of q.  What becomes 4 bits is turned in 64 bits: a difference in the last of 32 would, next to a border between two codes, be
-// one of a whole code.  (The arithmetic hides behind the memory either way.)
+// first the kv heads, K and V together, then those of q.
+//
+// What becomes 4 bits is what 64 bits say: an error in the last of 32 would, next to a border between two codes, be one of a whole code.  It is turned in 32, and again in 64 where a
+// code or a scale is so near to a border that it could depend on it, which a wave comes to once in some hundred rows, or where angles are zero.  6 heads of 2 x 30720 tokens with their
+// positions: 65 us for what a copy takes 49 for (64 bits throughout: 71); waves wait for memory in 6 of 10 cycles, and the vector unit is busy in half of them.
 template <typename T, bool kHeld>
-__global__ __launch_bounds__(256) void cache_append_rotary_kernel(const AppendRotaryParams p) {
+__global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(4))) void cache_append_rotary_kernel(const AppendRotaryParams p) {
   const AppendParams& a = p.append;
   const CacheView& cache = a.cache;
   const int tid = threadIdx.x, c = tid & 15;
@@ -44,32 +45,36 @@ __global__ __launch_bounds__(256) void cache_append_rotary_kernel(const AppendRo
   if (t >= n && (n >= 0 ? end <= cache.kv_heads : p.heads == 0)) return;  // behind the sequence's last one, and no q
   const int position = (a.first != nullptr ? a.first[b] : len) + t;
   const int page = t < n ? cache.page_of(b, len + t) : -1;
-  // rows of K and V, two heads ahead
+  // Rows of K and V, a head or two ahead (4 bits have no registers for two at four waves on a SIMD).  Every round of the loop issues as many loads and stores, whatever its lanes have, so
+  // that none waits for stores of the round before: behind the last head it is fetched again.
+  constexpr int kAhead = kHeld ? 1 : 2;
   const char* const k_from = a.k.ptr + b * a.k.batch + (int64_t)t * a.k.row + c * 16;
   const char* const v_from = a.v.ptr + b * a.v.batch + (int64_t)t * a.v.row + c * 16;
   const int kv_end = page >= 0 ? min(end, cache.kv_heads) : h0;
-  x8_of<T> k_rows[2], v_rows[2];
+  x8_of<T> k_rows[kAhead], v_rows[kAhead];
   auto fetch = [&](int h, int i) {
-    if (h >= kv_end) return;
+    h = min(h, kv_end - 1);
     k_rows[i] = *reinterpret_cast<const x8_of<T>*>(k_from + h * a.k.head);
     v_rows[i] = *reinterpret_cast<const x8_of<T>*>(v_from + h * a.v.head);
   };
-  fetch(h0, 0);
-  fetch(h0 + 1, 1);
-  using F = typename std::conditional<kHeld, double, float>::type;
-  Turn<F> turn;
-  const bool turns = p.rotation.turns != nullptr, interleaved = p.rotation.interleaved != 0;
-  turn.on = false;
-  if (turns) turn.init(p.rotation, b, t, position, c);
-  for (int h1 = h0; h1 < kv_end; h1 += 2)
+  if (h0 < kv_end)
 #pragma unroll
-    for (int i = 0; i < 2; ++i) {
+    for (int i = 0; i < kAhead; ++i) fetch(h0 + i, i);
+  Turn turn;
+  const bool turns = p.rotation.turns != nullptr, interleaved = p.rotation.interleaved != 0;
+  const Columns columns(p.rotation, c);
+  turn.on = false;
+  if (turns) turn.init(p.rotation, columns, b, t, position);
+  const int64_t row0 = cache.row_of(page, h0, len + t), rows = 1ll << cache.page_log2;  // (a head's rows of a page are one behind the other)
+  int64_t to = row0;
+  for (int h1 = h0; h1 < kv_end; h1 += kAhead)
+#pragma unroll
+    for (int i = 0; i < kAhead; ++i) {
       const int h = h1 + i;
-      if (h >= kv_end) break;
-      const int64_t to = cache.row_of(page, h, len + t);
+      if (i > 0 && h >= kv_end) break;
       x8_of<T> kr = k_rows[i];
       const x8_of<T> vr = v_rows[i];
-      fetch(h + 2, i);
+      fetch(h + kAhead, i);
       if constexpr (kHeld) {
         float kf[8], vf[8];
 #pragma unroll
@@ -77,38 +82,69 @@ __global__ __launch_bounds__(256) void cache_append_rotary_kernel(const AppendRo
           kf[e] = (float)kr[e];
           vf[e] = (float)vr[e];
         }
+        To4Bits<T> k4, v4;
         if (turns) {
           const x8_of<T> y = paired<T>(kr, turn, interleaved);
+          float off = 0.f;  // of what is turned in 32 bits: less than 2^-21 (|a| + |b|)
+#pragma unroll
+          for (int e = 0; e < 8; ++e) off = fmaxf(off, fabsf(kf[e]));
+          off += interleaved ? off : __shfl(off, turn.from);
+          off = turn.on ? off * 0x1p-21f : 0.f;
           if (turn.on) {
 #pragma unroll
-            for (int e = 0; e < 8; ++e) kf[e] = cut((double)kf[e] * turn.own[e] + (double)(float)y[e] * turn.other[e]);
+            for (int e = 0; e < 8; ++e) kf[e] = kf[e] * turn.own[e] + (float)y[e] * turn.other[e];
           }
+          k4.template hold<true>(kf, __builtin_bit_cast(float, of_group(bits_of(off))));
+          if (__builtin_amdgcn_ballot_w64(!k4.sure) != 0) {
+            if (turn.on) {
+              int seldom = c, where = t, stands = position;  // (nothing of this is worked out ahead, in registers that the loop would go without)
+              pin(seldom);
+              pin(where);
+              pin(stands);
+              const Columns again(p.rotation, seldom);
+#pragma unroll
+              for (int e = 0; e < 8; ++e) {
+                uint64_t phase[1];
+                phases_of(p.rotation, again.pair(p.rotation, e), b, where, stands, phase);
+                double sin, cos;
+                sincos_of(phase[0], &sin, &cos);
+                kf[e] = cut((double)(float)kr[e] * cos + (double)(float)y[e] * (again.leads(p.rotation, e) ? -sin : sin));
+                __builtin_amdgcn_sched_barrier(0);
+              }
+            }
+            k4.template hold<false>(kf, 0.f);
+          }
+        } else {
+          k4.template hold<false>(kf, 0.f);
         }
-        uint32_t k_scale, v_scale;
-        const uint32_t k_codes = to_4_bits<T>(kf, &k_scale), v_codes = to_4_bits<T>(vf, &v_scale);
-        *reinterpret_cast<uint32_t*>(cache.k + to * kHeldRowBytes + c * 4) = k_codes;
-        *reinterpret_cast<uint32_t*>(cache.v + to * kHeldRowBytes + c * 4) = v_codes;
-        if ((c & 3) == 0) {
-          cache.k_scales[to * 4 + (c >> 2)] = (uint8_t)k_scale;
-          cache.v_scales[to * 4 + (c >> 2)] = (uint8_t)v_scale;
-        }
+        v4.template hold<false>(vf, 0.f);
+        *reinterpret_cast<uint32_t*>(cache.k + to * kHeldRowBytes + c * 4) = k4.codes;
+        *reinterpret_cast<uint32_t*>(cache.v + to * kHeldRowBytes + c * 4) = v4.codes;
+        cache.k_scales[to * 4 + (c >> 2)] = (uint8_t)k4.scale;  // (by all four lanes of a group)
+        cache.v_scales[to * 4 + (c >> 2)] = (uint8_t)v4.scale;
       } else {
         if (turns) kr = turned<T>(kr, turn, interleaved);
         *reinterpret_cast<x8_of<T>*>(cache.k + to * kRowBytes + c * 16) = kr;
         *reinterpret_cast<x8_of<T>*>(cache.v + to * kRowBytes + c * 16) = vr;
       }
-      if (c == 0 && cache.positions != nullptr) cache.positions[to] = position;
-      if (c == 1 && cache.weights != nullptr) cache.weights[to] = a.weights != nullptr ? a.weights[((int64_t)b * cache.kv_heads + h) * a.tokens + t] : 0.f;
+      to += rows;
+    }
+  // positions and weights, sixteen heads at a time
+  if (cache.positions != nullptr || cache.weights != nullptr)
+    for (int h = h0 + c; h < kv_end; h += 16) {
+      const int64_t row = row0 + (h - h0) * rows;
+      if (cache.positions != nullptr) cache.positions[row] = position;
+      if (cache.weights != nullptr) cache.weights[row] = a.weights != nullptr ? a.weights[((int64_t)b * cache.kv_heads + h) * a.tokens + t] : 0.f;
     }
   const char* const from = p.q.ptr + b * p.q.batch + (int64_t)t * p.q.row + c * 16;
-  char* const to = p.q_out.ptr + b * p.q_out.batch + (int64_t)t * p.q_out.row + c * 16;
+  char* const q_to = p.q_out.ptr + b * p.q_out.batch + (int64_t)t * p.q_out.row + c * 16;
   for (int h = max(h0 - cache.kv_heads, 0); h < end - cache.kv_heads; ++h) {
     x8_of<T> r = *reinterpret_cast<const x8_of<T>*>(from + h * p.q.head);
     if (turns) r = turned<T>(r, turn, interleaved);
     if (n < 0)
 #pragma unroll
       for (int e = 0; e < 8; ++e) r[e] = (T)__builtin_nanf("");
-    *reinterpret_cast<x8_of<T>*>(to + h * p.q_out.head) = r;
+    *reinterpret_cast<x8_of<T>*>(q_to + h * p.q_out.head) = r;
   }
 }
 

@@ -14,8 +14,8 @@ __global__ __launch_bounds__(256) void rotary_kernel(const RotaryParams p) {
   if (part >= p.parts) return;
   const uint32_t b = n / (uint32_t)p.seq;
   const int t = (int)(n - b * (uint32_t)p.seq);
-  Turn<float> turn;
-  turn.init(p.rotation, b, t, t, c);
+  Turn turn;
+  turn.init(p.rotation, Columns(p.rotation, c), b, t, t);
   const bool interleaved = p.rotation.interleaved != 0;
   const int first = part * p.per, end = min(first + (int)p.per, p.heads + p.kv_heads);
   auto rows = [&](const Strided& x, const Strided& out, int h0, int h1) {

@@ -28,52 +28,75 @@ FBA_DEVICE void sincos_of(uint64_t phase, double* sin, double* cos) {
   *cos = (quarter + 1) & 2 ? -v : v;
 }
 
+// Where a lane's eight columns, 8 c .. 8 c + 7, turn: their pairs, and the lane that has what they are paired with.
+struct Columns {
+  int half, c;  // lanes that have a half of the pairs
+  FBA_DEVICE Columns(const Rotation& r, int c) : half(r.pairs >> 3), c(c) {}
+  FBA_DEVICE bool on() const { return c < 2 * half; }
+  FBA_DEVICE bool first() const { return c < half; }
+  FBA_DEVICE int pair(const Rotation& r, int e) const { return r.interleaved ? 4 * c + e / 2 : 8 * (first() ? c : c - half) + e; }
+  // (a, b) -> (a cos - b sin, b cos + a sin): whether column e is an a
+  FBA_DEVICE bool leads(const Rotation& r, int e) const { return r.interleaved ? e % 2 == 0 : first(); }
+  FBA_DEVICE int partner(const Rotation& r) const { return (int)(threadIdx.x & 63) + (r.interleaved || !on() ? 0 : first() ? half : -half); }
+};
+
+// The angles of `kPairs` consecutive pairs for a token, in turns times 2^64.  `position`: where it stands on every axis, where the rotation says nothing.
+template <int kPairs>
+FBA_DEVICE void phases_of(const Rotation& r, int i0, int64_t b, int t, int position, uint64_t (&phases)[kPairs]) {
+  int32_t at[kPairs];
+  if (r.at != nullptr) {  // (all axes are on their way at a time, then all coordinates)
+    const int32_t* const where = r.at + b * r.at_batch + (int64_t)t * r.n_axes;
+    uint32_t axes[kPairs];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) axes[i] = (uint32_t)r.axes[i0 + i];
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) at[i] = where[min(axes[i], (uint32_t)r.n_axes - 1)];  // (an axis that there is not counts as the last)
+  } else {
+#pragma unroll
+    for (int i = 0; i < kPairs; ++i) at[i] = position;
+  }
+#pragma unroll
+  for (int i = 0; i < kPairs; ++i) phases[i] = (uint64_t)r.turns[i0 + i] * (uint64_t)(int64_t)at[i];
+}
+
 // What a lane's eight columns of a token's rows are multiplied by: x own + (what they are paired with) other.
-template <typename F>
 struct Turn {
-  F own[8], other[8];
+  float own[8], other[8];
   int from;  // lane of the wave that has the columns these are paired with
   bool on;   // these columns turn at all
 
-  // Columns 8 c .. 8 c + 7; `position`: on every axis, where the rotation says nothing.
-  FBA_DEVICE void init(const Rotation& r, int64_t b, int t, int position, int c) {
-    const int half = r.pairs >> 3;  // lanes that have a half of the pairs
-    on = c < 2 * half;
-    from = threadIdx.x & 63;
+  FBA_DEVICE void init(const Rotation& r, const Columns& columns, int64_t b, int t, int position) {
+    on = columns.on();
+    from = columns.partner(r);
     if (!on) return;
-    const bool first = c < half;
-    if (!r.interleaved) from += first ? half : -half;
-    const int32_t* const at = r.at != nullptr ? r.at + b * r.at_batch + (int64_t)t * r.n_axes : nullptr;
-    auto pair = [&](int i, F* sin, F* cos) {
-      // (an axis that there is not counts as the last)
-      const int32_t p = at != nullptr ? at[min((uint32_t)r.axes[i], (uint32_t)r.n_axes - 1)] : position;
-      sincos_of((uint64_t)r.turns[i] * (uint64_t)(int64_t)p, sin, cos);
-      if (r.back) *sin = -*sin;
-    };
     if (r.interleaved) {
+      uint64_t phases[4];
+      phases_of(r, columns.pair(r, 0), b, t, position, phases);
 #pragma unroll
       for (int e = 0; e < 8; e += 2) {
-        F s, co;
-        pair(4 * c + e / 2, &s, &co);
+        float s, co;
+        sincos_of(phases[e / 2], &s, &co);
+        if (r.back) s = -s;
         own[e] = own[e + 1] = co;
         other[e] = -s;
         other[e + 1] = s;
       }
     } else {
-      const int i0 = 8 * (first ? c : c - half);
+      uint64_t phases[8];
+      phases_of(r, columns.pair(r, 0), b, t, position, phases);
 #pragma unroll
       for (int e = 0; e < 8; ++e) {
-        F s;
-        pair(i0 + e, &s, &own[e]);
-        other[e] = first ? -s : s;
+        float s;
+        sincos_of(phases[e], &s, &own[e]);
+        other[e] = columns.first() != (r.back != 0) ? -s : s;
       }
     }
   }
 };
 
 // The columns that a lane's own are paired with.  All sixteen lanes of the row take part.
-template <typename T, typename F>
-FBA_DEVICE x8_of<T> paired(x8_of<T> x, const Turn<F>& turn, bool interleaved) {
+template <typename T>
+FBA_DEVICE x8_of<T> paired(x8_of<T> x, const Turn& turn, bool interleaved) {
   if (interleaved) return __builtin_shufflevector(x, x, 1, 0, 3, 2, 5, 4, 7, 6);
   u32x4 bits = __builtin_bit_cast(u32x4, x);
 #pragma unroll
@@ -82,13 +105,13 @@ FBA_DEVICE x8_of<T> paired(x8_of<T> x, const Turn<F>& turn, bool interleaved) {
 }
 
 // A lane's columns of a row, turned in 32 bits and rounded once.
-template <typename T, typename F>
-FBA_DEVICE x8_of<T> turned(x8_of<T> x, const Turn<F>& turn, bool interleaved) {
+template <typename T>
+FBA_DEVICE x8_of<T> turned(x8_of<T> x, const Turn& turn, bool interleaved) {
   const x8_of<T> y = paired<T>(x, turn, interleaved);
   if (!turn.on) return x;
   float o[8];
 #pragma unroll
-  for (int e = 0; e < 8; ++e) o[e] = (float)x[e] * (float)turn.own[e] + (float)y[e] * (float)turn.other[e];
+  for (int e = 0; e < 8; ++e) o[e] = (float)x[e] * turn.own[e] + (float)y[e] * turn.other[e];
   return __builtin_shufflevector(narrow4<T>(o[0], o[1], o[2], o[3]), narrow4<T>(o[4], o[5], o[6], o[7]), 0, 1, 2, 3, 4, 5, 6, 7);
 }
 
