@@ -74,11 +74,12 @@ FBA_DEVICE x8_of<T> from_4_bits(uint32_t codes, float scale) {
 }
 
 // A double to a float whose last bits say whether something was cut off, so that a second rounding, to far fewer bits, is the same as a single one of the double: 21 bits are kept,
-// and the last one is set if anything behind it was.
+// and the last one is set if anything behind it was.  What is finite stays so.
 FBA_DEVICE float cut(double x) {
   const uint64_t bits = __builtin_bit_cast(uint64_t, x);
   const uint32_t high = (uint32_t)(bits >> 32) | ((uint32_t)bits != 0 ? 1u : 0u);
-  return (float)__builtin_bit_cast(double, (uint64_t)high << 32);
+  const float f = (float)__builtin_bit_cast(double, (uint64_t)high << 32);
+  return (high & 0x7ff00000u) != 0x7ff00000u ? fminf(fmaxf(f, -0x1.fffffep127f), 0x1.fffffep127f) : f;
 }
 
 }  // namespace fba

@@ -43,7 +43,7 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
   const int n = tokens_of(b, &len);
   const int h0 = part * p.per, end = min(h0 + (int)p.per, cache.kv_heads + p.heads);
   if (t >= n && (n >= 0 ? end <= cache.kv_heads : p.heads == 0)) return;  // behind the sequence's last one, and no q
-  const int position = (a.first != nullptr ? a.first[b] : len) + t;
+  const int position = (int)((uint32_t)(a.first != nullptr ? a.first[b] : len) + (uint32_t)t);
   const int page = t < n ? cache.page_of(b, len + t) : -1;
   // Rows of K and V, a head or two ahead (4 bits have no registers for two at four waves on a SIMD).  Every round of the loop issues as many loads and stores, whatever its lanes have, so
   // that none waits for stores of the round before: behind the last head it is fetched again.
@@ -85,11 +85,11 @@ __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_pe
         To4Bits<T> k4, v4;
         if (turns) {
           const x8_of<T> y = paired<T>(kr, turn, interleaved);
-          float off = 0.f;  // of what is turned in 32 bits: less than 2^-21 (|a| + |b|)
+          float off = 0.f;  // of what is turned in 32 bits: less than 2^-21 (|a| + |b|), and 2^-124 for what is too small for them
 #pragma unroll
           for (int e = 0; e < 8; ++e) off = fmaxf(off, fabsf(kf[e]));
           off += interleaved ? off : __shfl(off, turn.from);
-          off = turn.on ? off * 0x1p-21f : 0.f;
+          off = turn.on && off > 0.f ? off * 0x1p-21f + 0x1p-124f : 0.f;
           if (turn.on) {
 #pragma unroll
             for (int e = 0; e < 8; ++e) kf[e] = kf[e] * turn.own[e] + (float)y[e] * turn.other[e];

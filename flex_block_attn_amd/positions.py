@@ -42,7 +42,7 @@ def rotary(dims=(HEAD_DIM,), theta=10000.0, interleaved=True, frequencies=None, 
     frequencies = [float(f) for f in frequencies]
     if len(frequencies) != sum(dims) // 2 or not all(map(math.isfinite, frequencies)):
         raise ValueError(f"frequencies must be {sum(dims) // 2} finite numbers, got {len(frequencies)}")
-    turns = [(int(f / (2 * math.pi) * 2**64) + 2**63) % 2**64 - 2**63 for f in frequencies]  # (a float times a power of two is exact)
+    turns = [(int(math.fmod(f / (2 * math.pi), 1.0) * 2**64) + 2**63) % 2**64 - 2**63 for f in frequencies]  # (whole turns off, times a power of two: both exact)
     turns, axes = torch.tensor(turns, dtype=torch.int64), torch.tensor([x for x, d in enumerate(dims) for _ in range(d // 2)], dtype=torch.int32)
     return Rotary(turns.to(device), axes.to(device), len(dims), bool(interleaved))
 

@@ -481,14 +481,14 @@ int32_t fba_rotary(const fba_strided* q, const fba_strided* q_out, const fba_str
  * A paged cache in 4 bits: `cache` as above, but k and v [pages, kv_heads, page_size, 64] bytes, value 2j of a row in the low half of byte j, 2j + 1 in the high one, and k_scales, v_scales
  * [pages, kv_heads, page_size, 4], one for each 32 values.  A value is m * 2^(scale - 127), m = 0, 0.5, 1, 1.5, 2, 3, 4, 6 for the low three bits 0 .. 7, below zero with the fourth;
  * scale 255: all 32 are no numbers.  What is appended is rounded so: e = floor(log2(the largest of the 32)) - 2, one more from 1.75 of its binade on, brought into -125 .. 125 (type
- * FBA_BF16) or -13 .. 13 (FBA_FP16), scale = e + 127, or 255 where one of the 32 is infinite or no number; m to the nearest, ties to the even code.  So a value v is off by at most
- * max(2^(e-2), |v| / 4) (2^(e-2) up to 2^(e+1), half of a step above), but for fp16 values above 7 * 2^13, which become 6 * 2^13, bf16 ones above 7 * 2^125 alike, and values below the
- * smallest normal number of the type, which may become zero.  type is that of q, k, v and o, and fixed for a pool: its values are exact in it.
+ * FBA_BF16) or -13 .. 13 (FBA_FP16), scale = e + 127, or 255 where one of the 32 is infinite or no number; m to the nearest, ties to the even code.  So a value v is off by a
+ * quarter of 2^e or of |v| at most, but for fp16 values above 7 * 2^13, which become 6 * 2^13, bf16 ones above 7 * 2^125 alike, and values below the smallest normal number of the type,
+ * which may become zero.  type is that of q, k, v and o, and fixed for a pool: its values are exact in it.
  *
  * fba_cache4_append, fba_cache4_attn, fba_cache4_evict: as the functions of 16 bits, attention over the values that the pool stands for.  fba_cache4_append takes a rotation too (null: none).
  * fba_cache_append_rotary: as fba_cache_append, with k turned on the way, and q_out = q [batch, heads, tokens, 128] turned alike (null, with heads = 0: there is none), the rows behind
  *   counts[b] too, no numbers for a sequence whose length or count makes no sense.  Where rotation->at is null, the token t of sequence b stands at first[b] + t (first null:
- *   lengths[b] + t) on all axes; positions of the cache are that in either case.  A k that goes into 4 bits is turned in 64 bits, so that it is rounded once.
+ *   lengths[b] + t) on all axes; positions of the cache are that in either case.  A k that goes into 4 bits is what 64 bits say, rounded once.
  * fba_cache_read, fba_cache4_read: slots first .. first + slots - 1 of every sequence to k, v [batch, kv_heads, slots, 128]: what a prompt's next chunk attends to with
  *   fba_window_fwd.  Zeros behind the sequence's length, no numbers in the rows of a page outside of the pool, and in all rows of a sequence whose length makes no sense.
  * batch may be 2^22 and batch * tokens 2^27 at most where tokens are appended, batch * kv_heads * ceil(slots / 64) 2^24 - 1 where slots are read.

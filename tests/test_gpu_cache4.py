@@ -212,6 +212,70 @@ def test_append_with_the_rotation(gpu, bits, dtype, dims, interleaved, where, pa
     assert torch.equal(again, out) and torch.equal(bare.k.view(torch.int8), cache.k.view(torch.int8)) and torch.equal(bare.v.view(torch.int8), cache.v.view(torch.int8)) and (q is None or torch.equal(same, turned))
 
 
+def held_at_once(x, dtype):
+    """`held`, all groups at a time, on x's device.  Exact: a power of two, a difference of two numbers of few bits and a comparison each."""
+    groups = x.reshape(-1, 32)
+    most = groups.abs().amax(1)
+    e = torch.frexp(most)[1].long() - 3
+    e = torch.where(most >= 1.75 * torch.exp2((e + 2).double()), e + 1, e)
+    e = torch.where(most > 0, e, torch.full_like(e, -LIMIT[dtype])).clamp(-LIMIT[dtype], LIMIT[dtype])
+    unit = torch.exp2(e.double())[:, None]
+    small = groups.abs() / unit
+    borders = torch.tensor([0.25, 0.75, 1.25, 1.75, 2.5, 3.5, 5.0], dtype=torch.float64, device=x.device)
+    up = torch.tensor([False, True, False, True, False, True, False], device=x.device)  # a tie goes to the even code
+    code = ((small[..., None] > borders) | ((small[..., None] == borders) & up)).sum(-1)
+    values = torch.where(groups < 0, -1.0, 1.0) * STEPS.to(x.device)[code] * unit
+    return values.reshape(x.shape), (e + 127).reshape(*x.shape[:-1], 4)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float16])
+@pytest.mark.parametrize("interleaved", [False, True])
+@pytest.mark.parametrize("kind", ["many", "quarter turns", "small", "large"])
+def test_a_turned_key_is_held_as_64_bits_say(gpu, dtype, interleaved, kind):
+    """Where 32 bits would not do: many values, of which some come near to a border between two codes; values on the borders, at rest or turned by whole quarters, which both sides do
+    exactly; values around the smallest and the largest normal numbers of the type."""
+    import flex_block_attn_amd as fba
+
+    B, Hk, T, page = 2, 3, 2000 if kind == "many" else 150, 64
+    cache, table, g = make(gpu, B, Hk, T, page, dtype)
+    turn = fba.rotary((32, 64) if kind == "many" else (128,), interleaved=interleaved, device=gpu)
+    stand = torch.randint(-5000, 5000, (B, T, turn.n_axes), generator=g, dtype=torch.int32).to(gpu)
+    k = torch.randn((B, Hk, T, 128), generator=g)
+    if kind == "quarter turns":
+        turn.turns.fill_(2**62)
+        k = sample("ties", (B, Hk, T, 128), dtype, g)
+    elif kind == "small":  # (fp16 holds no more than 2^-15 of its smallest scale's codes)
+        k = k * 2.0 ** torch.randint(*((-14, -8) if dtype == torch.float16 else (-120, -96)), (B, Hk, T, 1), generator=g)
+        k = torch.where(k.abs() < torch.finfo(dtype).tiny, 0.0, k)
+        k[:, :, ::5] = 0.0
+    elif kind == "large":
+        top = torch.finfo(dtype).max
+        k = (k.double() * top).clamp(-top, top)
+    k = k.to(dtype).to(gpu)
+    print(f"held turned {dtype} {interleaved} {kind}", flush=True)
+    n, _ = fba.cache_append_rotary(cache, table, ints([0] * B, gpu), k, k, turn, coordinates=stand)
+    assert n.tolist() == [T] * B
+    if kind == "quarter turns":
+        x = k.double()
+        first, second = (slice(0, None, 2), slice(1, None, 2)) if interleaved else (slice(0, 64), slice(64, 128))
+        quarter = (stand % 4)[:, None]  # (B, 1, T, 1)
+        a, b = x[..., first], x[..., second]
+        want = x.clone()
+        pick = lambda *of: torch.where(quarter == 0, of[0], torch.where(quarter == 1, of[1], torch.where(quarter == 2, of[2], of[3])))
+        want[..., first], want[..., second] = pick(a, -b, -a, b), pick(b, a, -b, -a)
+    else:
+        want = exact(k, turn, stand)[0].to(gpu)
+    values, scales = held_at_once(want, dtype)
+    some = want[:1, :1, :40].cpu()
+    assert torch.equal(held(some, dtype)[0], values[:1, :1, :40].cpu()) and torch.equal(held(some, dtype)[1], scales[:1, :1, :40].cpu())
+    tiny = torch.finfo(dtype).tiny if dtype == torch.bfloat16 else 0.0
+    for b in range(B):
+        c, s = rows(cache.k, table, b, T), rows(cache.k_scales, table, b, T)
+        assert torch.equal(s.long(), scales[b])
+        got = decoded(c, s)
+        assert bool(((got == values[b]) | (want[b].abs() < tiny) & (got == 0)).all())
+
+
 @pytest.mark.parametrize("bits", [4, 16])
 def test_append_where_there_is_no_room(gpu, bits):
     """Lengths, counts and pages that make no sense are answered with -1 and a q of no numbers: nothing is written but rows on good pages of a table with a bad one."""

@@ -97,6 +97,8 @@ def test_rotary_makes_turns_of_frequencies():
     r = fba.rotary((16,), frequencies=[2 * math.pi * 0.75, -2 * math.pi * 0.25, 2 * math.pi * 3.5, 0.0, 1.0, -1.0, 100.0, 1e-9], interleaved=False, device="cpu")
     assert r.turns.tolist()[:4] == [-(2**62), -(2**62), -(2**63), 0] and not r.interleaved
     assert r.turns[4] == -r.turns[5]
+    r = fba.rotary((16,), frequencies=[1e300, -1e300, 2 * math.pi * 1e9, 0.0, 0.0, 0.0, 0.0, 0.0], device="cpu")  # as far as floats go
+    assert r.turns[0] == -r.turns[1] and r.turns[2] == 0
 
 
 @pytest.mark.parametrize("grid,tile", [((2, 4, 6), None), ((2, 4, 6), (1, 2, 3)), ((6, 8, 8), (6, 8, 8)), ((4, 4), (2, 4)), ((5,), None)])
