@@ -11,8 +11,8 @@ namespace fba {
 // first the kv heads, K and V together, then those of q.
 //
 // What becomes 4 bits is what 64 bits say: an error in the last of 32 would, next to a border between two codes, be one of a whole code.  It is turned in 32, and again in 64 where a
-// code or a scale is so near to a border that it could depend on it, which a wave comes to once in some hundred rows, or where angles are zero.  6 heads of 2 x 30720 tokens with their
-// positions: 65 us for what a copy takes 49 for (64 bits throughout: 71); waves wait for memory in 6 of 10 cycles, and the vector unit is busy in half of them.
+// code or a scale is so near to a border that it could depend on it, which a wave comes to once in some hundred rows, or where angles are zero.  6 heads of 2 x 30720 tokens: 53 us for what
+// a copy takes 49 for (without the rotation 50), and 65 right behind a read that has left as much to be written out (64 bits throughout: 71).
 template <typename T, bool kHeld>
 __global__ __attribute__((amdgpu_flat_work_group_size(256, 256), amdgpu_waves_per_eu(4))) void cache_append_rotary_kernel(const AppendRotaryParams p) {
   const AppendParams& a = p.append;

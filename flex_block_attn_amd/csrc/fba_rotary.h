@@ -28,7 +28,9 @@ struct RotaryParams {
 
 hipError_t launch_rotary(RotaryParams p, bool half, hipStream_t stream);
 
-// How many parts the heads of `tokens` tokens are cut into: 16 lanes do one part of one token, which fill the GPU's waves from some 2^14 parts on.
+// How many parts the heads of `tokens` tokens are cut into: 16 lanes do one part of one token, and 2^14 parts are a wave for every place that the GPU has for one at half of its occupancy.
+// 24 + 24 heads of 1000 tokens with 2^12, 2^13, 2^14, 2^15 and 2^16 parts: 6.6, 6.3, 6.9, 7.4 and 10.0 us; 8 + 2 of 6272: 8.5, 9.4, 9.4, 11.4 and 16.6; 6 of 12000 into 4 bits: 18.2, 18.4,
+// 16.9, 19.3 and 25.4; with one part each 13.9, 8.6 and 18.4, and for 64 new tokens, 40 heads, 14.8 instead of 5.3.
 inline uint32_t rotary_parts(int64_t tokens, int64_t heads) {
   const int64_t want = tokens > 0 ? (16384 + tokens - 1) / tokens : 1;
   return (uint32_t)(want < heads ? want : heads > 0 ? heads : 1);
