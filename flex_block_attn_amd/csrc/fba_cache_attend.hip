@@ -334,7 +334,8 @@ void plan_cache_attend(AttendParams& p, int compute_units) {
   const int rows = p.cache.kv_heads * p.head_tiles, resident = p.cache.k_scales != nullptr && head_tiles_of(group) == 1 ? kResident4 : 2;
   p.target = resident * compute_units / rows > 0 ? resident * compute_units / rows : 1;
   // no more than there may be tiles for
-  const int64_t most = (p.cache.batch * ((p.cache.slots() + kTile - 1) / kTile) + kLeastTiles - 1) / kLeastTiles;
+  int64_t most = (p.cache.batch * ((p.cache.slots() + kTile - 1) / kTile) + kLeastTiles - 1) / kLeastTiles;
+  if (p.cache.k_scales != nullptr && most < p.cache.batch) most = p.cache.batch;
   if (p.target > most) p.target = (int)most;
   p.slots = p.target + p.cache.batch;
 }
