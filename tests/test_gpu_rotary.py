@@ -330,3 +330,34 @@ def test_a_video_layer(gpu):
     back = fba.rotary_func(*by_hand[:2], turn, coordinates=raster, inverse=True)
     for x, y in zip(grads, (*back, by_hand[2])):
         assert torch.equal(x, y)
+
+
+def test_calls_that_are_seldom(gpu):
+    """Heads and sequences that share memory, coordinates that Python prepares, nothing to turn, inference mode, checkpoints and saved tensors that were elsewhere meanwhile."""
+    import flex_block_attn_amd as fba
+    from torch.utils.checkpoint import checkpoint
+
+    turn = fba.rotary((64,), interleaved=False, device=gpu)
+    q, k = random((2, 4, 33, 128), torch.bfloat16, gpu, 1), random((2, 1, 33, 128), torch.bfloat16, gpu, 2)
+    given, where = places("shared", 2, 33, 1, gpu)
+    call = lambda q, k, given=given: fba.rotary_func(q, k, turn, coordinates=given)
+    want = call(q, k)
+    check(want[0], q, turn, where)
+    check(want[1], k, turn, where)
+    assert torch.equal(call(q, k.expand(-1, 4, -1, -1))[1], want[1].expand(-1, 4, -1, -1))
+    for same in (given.expand(2, 33, 1), given.repeat(1, 2)[:, :1]):
+        assert torch.equal(call(q, k, same)[0], want[0])
+    assert torch.equal(call(torch.cat([q.flatten()[:1], q.flatten()])[1:].view_as(q), None)[0], want[0])  # rows that are not aligned
+    assert [tuple(x.shape) for x in call(q[:, :, :0], k[:, :, :0], given[:0])] == [(2, 4, 0, 128), (2, 1, 0, 128)]
+    none, some = call(q[:, :0], k)
+    assert none.shape == (2, 0, 33, 128) and torch.equal(some, want[1])
+    with torch.inference_mode():
+        assert torch.equal(call(q.clone(), k)[0], want[0])
+    q, k = q.clone().requires_grad_(True), k.clone().requires_grad_(True)
+    grads = lambda out: torch.autograd.grad([(o.float() ** 2).sum() for o in out], (q, k))
+    first = grads(call(q, k))
+    again = grads(checkpoint(call, q, k, use_reentrant=False))
+    with torch.autograd.graph.save_on_cpu():
+        out = call(q, k)
+    for x in (again, grads(out)):
+        assert all(torch.equal(a, b) for a, b in zip(x, first))
