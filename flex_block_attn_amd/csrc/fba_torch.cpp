@@ -954,6 +954,14 @@ bool takes_rotation(const Rotation& r, const at::Tensor& like, int64_t batch, in
   if (t.device() != like.device() || t.scalar_type() != at::kInt || !t.is_contiguous() || (t.dim() != 2 && t.dim() != 3)) return false;
   return (t.dim() == 2 || t.size(0) == batch) && t.size(-2) == tokens && t.size(-1) == r.n_axes;
 }
+// The same of a call for q and k, which may be undefined, but for what strides have to be.
+bool takes_rotary(const at::Tensor& q, const at::Tensor& k, const Rotation& r) {
+  for (const at::Tensor* t : {&q, &k})
+    if (t->defined() && (!t->is_cuda() || t->device() != q.device() || t->scalar_type() != q.scalar_type() || t->dim() != 4 || t->size(3) != kHeadDim || t->size(0) != q.size(0) ||
+                         t->size(2) != q.size(2) || t->size(1) > 65535))
+      return false;
+  return is_type(q.scalar_type()) && takes_rotation(r, q, q.size(0), q.size(2));
+}
 fba_rotation rotation_of(const Rotation& r) {
   const bool each = r.at.defined() && r.at.dim() == 3;
   return {r.turns.data_ptr<int64_t>(), r.axes.data_ptr<int32_t>(), ints_of(r.at), each ? r.at.size(1) * r.at.size(2) : 0, (int32_t)r.turns.size(0), (int32_t)r.n_axes, r.interleaved};
@@ -1037,11 +1045,7 @@ c10::optional<Turned> rotary(pybind11::handle q_, pybind11::handle k_, pybind11:
   r.at = tensor_of(at_);
   pybind11::gil_scoped_release no_gil;
   if (!q.defined() || (k.defined() ? transformed({&q, &k}) : transformed({&q}))) return c10::nullopt;
-  for (const at::Tensor* t : {&q, &k})
-    if (t->defined() && (!t->is_cuda() || t->device() != q.device() || t->scalar_type() != q.scalar_type() || !takes_strides(*t) || t->size(0) != q.size(0) || t->size(2) != q.size(2) ||
-                         t->size(1) > 65535))
-      return c10::nullopt;
-  if (!is_type(q.scalar_type()) || q.numel() == 0 || !takes_rotation(r, q, q.size(0), q.size(2))) return c10::nullopt;
+  if (q.numel() == 0 || !takes_strides(q) || (k.defined() && !takes_strides(k)) || !takes_rotary(q, k, r)) return c10::nullopt;
   if (wants_grad({&q, &k})) {
     const auto out = Rotary::apply(q, maybe(k), r.turns, r.axes, maybe(r.at), r.n_axes, r.interleaved, inverse);
     return turned_of(out[0], k.defined() ? out[1] : at::Tensor());
@@ -1054,9 +1058,10 @@ c10::optional<Turned> rotary(pybind11::handle q_, pybind11::handle k_, pybind11:
 Turned rotary_forward(const at::Tensor& q, const c10::optional<at::Tensor>& k, const at::Tensor& turns, const at::Tensor& axes, int64_t n_axes, bool interleaved,
                       const c10::optional<at::Tensor>& at, bool inverse) {
   const Rotation r{turns, axes, at.value_or(at::Tensor()), n_axes, interleaved};
-  TORCH_CHECK_VALUE(q.numel() == 0 || (takes_strides(q) && (!k || k->numel() == 0 || takes_strides(*k)) && takes_rotation(r, q, q.size(0), q.size(2))), "arguments are not as they were");
+  const at::Tensor k_ = k.value_or(at::Tensor());
+  TORCH_CHECK_VALUE(takes_rotary(q, k_, r) && (q.numel() == 0 || takes_strides(q)) && (!k || k->numel() == 0 || takes_strides(*k)), "arguments are not as they were");
   refuse_nodes_of_the_default_stream(q);  // (backward comes through here too)
-  const auto out = run_rotary(q, k.value_or(at::Tensor()), r, inverse);
+  const auto out = run_rotary(q, k_, r, inverse);
   return turned_of(out.first, out.second);
 }
 

@@ -83,11 +83,31 @@ def _check_coordinates(coordinates, rotary, batch, tokens, like):
     return coordinates.contiguous()
 
 
+def _check_rotary_args(q, k, rotary, coordinates):
+    """Raises for everything that the kernel does not take.  -> coordinates, dense"""
+    for name, t in (("q", q), ("k", k)):
+        if name == "k" and t is None:
+            continue
+        _require_device(t, name)
+        if t.dtype not in _TYPES:
+            raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
+        if t.dtype != q.dtype or t.device != q.device:
+            raise ValueError(f"{name} must have q's type and device ({q.dtype}, {q.device}), got {t.dtype}, {t.device}")
+        if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2] or t.shape[1] > 65535:
+            raise ValueError(f"{name} must have shape (batch, heads, seq, {HEAD_DIM}), batch and seq those of q, 65535 heads at most, got {tuple(t.shape)}")
+    _check_rotary(rotary, q)
+    if q.shape[0] * q.shape[2] > 1 << 27:
+        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"all sequences together may have 2^27 tokens, got {q.shape[0]} x {q.shape[2]}")
+    return _check_coordinates(coordinates, rotary, q.shape[0], q.shape[2], q)
+
+
 class RotaryFunc(torch.autograd.Function):
-    """The operator as a Python autograd function: for arguments that need preparation, calls that are traced and tensor subclasses."""
+    """The operator as a Python autograd function: for arguments that need preparation or are refused, calls that are traced and tensor subclasses."""
 
     @staticmethod
     def forward(ctx, q, k, turns, axes, n_axes, interleaved, coordinates, inverse):
+        coordinates = _check_rotary_args(q, k, Rotary(turns, axes, n_axes, interleaved), coordinates)
+        n_axes, interleaved, inverse = int(n_axes), bool(interleaved), bool(inverse)
         ctx.set_materialize_grads(False)
         ctx.save_for_backward(turns, axes, coordinates)
         ctx.args = (n_axes, interleaved, inverse)
@@ -122,18 +142,6 @@ def rotary_func(q, k, rotary, coordinates=None, inverse=False):
     out = None if of is None else _lib.host().rotary(q, k, *of, coordinates, bool(inverse))
     if out is not None:
         return out
-    for name, t in (("q", q), ("k", k)):
-        if name == "k" and t is None:
-            continue
-        _require_device(t, name)
-        if t.dtype not in _TYPES:
-            raise TypeError(f"{name} must be bfloat16 or float16, got {t.dtype}")
-        if t.dtype != q.dtype or t.device != q.device:
-            raise ValueError(f"{name} must have q's type and device ({q.dtype}, {q.device}), got {t.dtype}, {t.device}")
-        if t.dim() != 4 or t.shape[3] != HEAD_DIM or t.shape[0] != q.shape[0] or t.shape[2] != q.shape[2] or t.shape[1] > 65535:
-            raise ValueError(f"{name} must have shape (batch, heads, seq, {HEAD_DIM}), batch and seq those of q, 65535 heads at most, got {tuple(t.shape)}")
-    _check_rotary(rotary, q)
-    if q.shape[0] * q.shape[2] > 1 << 27:
-        raise _lib.FbaError(_lib.FBA_ERR_UNSUPPORTED, f"all sequences together may have 2^27 tokens, got {q.shape[0]} x {q.shape[2]}")
-    coordinates = _check_coordinates(coordinates, rotary, q.shape[0], q.shape[2], q)
-    return RotaryFunc.apply(q, k, rotary.turns, rotary.axes, int(rotary.n_axes), bool(rotary.interleaved), coordinates, bool(inverse))
+    if of is None:
+        raise TypeError(f"rotary must be a Rotary, got {type(rotary).__name__}")
+    return RotaryFunc.apply(q, k, *of, coordinates, inverse)
