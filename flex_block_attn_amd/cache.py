@@ -88,21 +88,22 @@ def _page_size(n):
     return n
 
 
-def _given(cache, table, lengths):
-    """The tensors of a call as the native side takes them, and the type of the cache's values; None for what is no cache."""
+def _given(cache, table, lengths, positions=True):
+    """The tensors of a call as the native side takes them, and the type of the cache's values; None for what is no cache.  positions=False: a call that has no use for the cache's."""
     if isinstance(cache, PagedCache):
-        return (cache.k, cache.v, None, None, cache.positions, cache.weights, table, lengths, getattr(cache.k, "dtype", None))
+        return (cache.k, cache.v, None, None, cache.positions if positions else None, cache.weights, table, lengths, getattr(cache.k, "dtype", None))
     if isinstance(cache, PagedCache4):
-        return (cache.k, cache.v, cache.k_scales, cache.v_scales, cache.positions, cache.weights, table, lengths, cache.dtype)
+        return (cache.k, cache.v, cache.k_scales, cache.v_scales, cache.positions if positions else None, cache.weights, table, lengths, cache.dtype)
     return None
 
 
-def _check_cache(cache, table, lengths):
-    """Raises for everything that the kernels do not take.  -> the type of the cache's values"""
+def _check_cache(cache, table, lengths, positions=True):
+    """Raises for everything that the kernels do not take; positions=False: of a call that has no use for the cache's.  -> the type of the cache's values"""
     if not isinstance(cache, (PagedCache, PagedCache4)):
         raise TypeError(f"cache must be a PagedCache or a PagedCache4, got {type(cache).__name__}")
     k, held = cache.k, isinstance(cache, PagedCache4)
-    tensors = [("k", k), ("v", cache.v), ("positions", cache.positions), ("weights", cache.weights)]
+    own = cache.positions if positions else None
+    tensors = [("k", k), ("v", cache.v), ("positions", own), ("weights", cache.weights)]
     if held:
         tensors += [("k_scales", cache.k_scales), ("v_scales", cache.v_scales)]
     tensors = [("cache." + name, t) for name, t in tensors if t is not None or name not in ("positions", "weights")]
@@ -129,7 +130,7 @@ def _check_cache(cache, table, lengths):
         raise ValueError(f"the cache must have a page and a head, got {tuple(k.shape)}")
     if held and any(t.shape != (*k.shape[:3], HEAD_DIM // 32) for t in (cache.k_scales, cache.v_scales)):
         raise ValueError(f"cache.k_scales and cache.v_scales must have shape {(*k.shape[:3], HEAD_DIM // 32)}, got {tuple(cache.k_scales.shape)} and {tuple(cache.v_scales.shape)}")
-    for name, t, dtype in (("positions", cache.positions, torch.int32), ("weights", cache.weights, torch.float32)):
+    for name, t, dtype in (("positions", own, torch.int32), ("weights", cache.weights, torch.float32)):
         if t is not None and (t.dtype != dtype or t.shape != k.shape[:3]):
             raise ValueError(f"cache.{name} must be {dtype} of shape {tuple(k.shape[:3])}, got {t.dtype} {tuple(t.shape)}")
     if table.dtype != torch.int32 or table.dim() != 2 or table.numel() == 0:
@@ -260,11 +261,11 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
 
     q: (batch, heads, 1, 128) of the cache's type, heads a multiple of kv_heads.  accumulate=True adds to cache.weights what softmax gave every slot, summed over the query
     heads of a kv head; not with a window, and with a workspace of 4 * batch * heads bytes for every slot that the table has room for, filled or not.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
-    given = _given(cache, table, lengths)
+    given = _given(cache, table, lengths, positions=False)
     out = None if given is None else _lib.host().cache_attention(q, given, window, sinks, bool(accumulate))
     if out is not None:
         return out
-    dtype = _check_cache(cache, table, lengths)
+    dtype = _check_cache(cache, table, lengths, positions=False)
     _require_device(q, "q")
     if q.dtype != dtype or q.device != cache.k.device:
         raise TypeError(f"q must have the cache's type and device ({dtype}, {cache.k.device}), got {q.dtype}, {q.device}")
