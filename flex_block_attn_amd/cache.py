@@ -20,7 +20,14 @@ Keys that carry their positions by rotation (positions.py) are turned on the way
 
     lengths, q = cache_append_rotary(cache, table, lengths, k, v, turn, q=q)
 
-A prompt's next chunk sees what is cached through `cache_read`, which hands rows back as dense tensors, for `window_attn_func`.
+A prompt's next chunk sees what is cached through `cache_read`, which hands rows back as dense tensors, for `window_attn_func`:
+
+    lengths, q = cache_append_rotary(cache, table, lengths, k, v, turn, q=q, counts=counts)
+    o = window_attn_func(q, *cache_read(cache, table, lengths, before + tokens), window)
+
+`window_attn_func` takes the queries for the last rows that it is given, of all sequences alike.  So this is for sequences that had one length, `before`, in front of the chunk; counts may
+differ (o behind a sequence's count is of nothing).  Where `before` differs the queries of a shorter sequence would stand behind its end, and see rows of zeros and tokens that come after
+them: such sequences go one by one, each with table[b:b + 1], lengths[b:b + 1], as many slots as it has, and its own queries.
 
 The pool may hold 4 bits to a value instead of 16 (`paged_cache(bits=4)`): 136 bytes instead of 512 for a slot's key and value.  All calls take either; attention is then over what the 4
 bits stand for, which is exact in the pool's type.  The kernels are csrc/fba_cache_rotary.hip and csrc/fba_cache_attend4.hip.
@@ -240,7 +247,7 @@ def cache_append_rotary(cache, table, lengths, k, v, rotary, q=None, counts=None
 
 def cache_read(cache, table, lengths, slots, first=0):
     """Slots first .. first + slots - 1 of every sequence as dense tensors k, v (batch, kv_heads, slots, 128) of the cache's type: what a prompt's next chunk attends to with
-    `window_attn_func`.  Rows behind a sequence's length are zeros; those of a page outside of the pool, and all of a sequence whose length makes no sense, are no numbers."""
+    `window_attn_func`, where all sequences had one length in front of it (else one by one: the head of this file).  Rows behind a sequence's length are zeros; those of a page outside of the pool, and all of a sequence whose length makes no sense, are no numbers."""
     given = _given(cache, table, lengths)
     out = None if given is None else _lib.host().cache_read(given, slots, first)
     if out is not None:

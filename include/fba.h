@@ -490,7 +490,8 @@ int32_t fba_rotary(const fba_strided* q, const fba_strided* q_out, const fba_str
  *   counts[b] too, no numbers for a sequence whose length or count makes no sense.  Where rotation->at is null, the token t of sequence b stands at first[b] + t (first null:
  *   lengths[b] + t) on all axes; positions of the cache are that in either case.  A k that goes into 4 bits is what 64 bits say, rounded once.
  * fba_cache_read, fba_cache4_read: slots first .. first + slots - 1 of every sequence to k, v [batch, kv_heads, slots, 128]: what a prompt's next chunk attends to with
- *   fba_window_fwd.  Zeros behind the sequence's length, no numbers in the rows of a page outside of the pool, and in all rows of a sequence whose length makes no sense.
+ *   fba_window_fwd, whose queries are the last of the rows, of all sequences alike: of sequences that had one length in front of the chunk, slots being that length and the chunk's
+ *   tokens; of others, one call for each.  Zeros behind the sequence's length, no numbers in the rows of a page outside of the pool, and in all rows of a sequence whose length makes no sense.
  * batch may be 2^22 and batch * tokens 2^27 at most where tokens are appended, batch * kv_heads * ceil(slots / 64) 2^24 - 1 where slots are read.
  */
 typedef struct {
