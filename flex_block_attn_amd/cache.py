@@ -239,7 +239,7 @@ def cache_append_rotary(cache, table, lengths, k, v, rotary, q=None, counts=None
     (batch, tokens, n_axes), which the cache's own positions do not follow.  A k that goes into 4 bits is rounded once.
 
     Returns the new lengths, as `cache_append` does, and q turned (None without): its rows behind a sequence's count too, and no numbers for a sequence whose length or count makes no
-    sense."""
+    sense or that has no room (but q turned where only a page is outside of the pool)."""
     if not isinstance(rotary, Rotary):
         raise TypeError(f"rotary must be a Rotary, got {type(rotary).__name__}")
     return _append(cache, table, lengths, k, v, counts, positions, weights, q, rotary, coordinates)

@@ -487,7 +487,7 @@ int32_t fba_rotary(const fba_strided* q, const fba_strided* q_out, const fba_str
  *
  * fba_cache4_append, fba_cache4_attn, fba_cache4_evict: as the functions of 16 bits, attention over the values that the pool stands for.  fba_cache4_append takes a rotation too (null: none).
  * fba_cache_append_rotary: as fba_cache_append, with k turned on the way, and q_out = q [batch, heads, tokens, 128] turned alike (null, with heads = 0: there is none), the rows behind
- *   counts[b] too, no numbers for a sequence whose length or count makes no sense.  Where rotation->at is null, the token t of sequence b stands at first[b] + t (first null:
+ *   counts[b] too, no numbers for a sequence whose length or count makes no sense or that has no room (turned where only a page is outside of the pool).  Where rotation->at is null, the token t of sequence b stands at first[b] + t (first null:
  *   lengths[b] + t) on all axes; positions of the cache are that in either case.  A k that goes into 4 bits is what 64 bits say, rounded once.
  * fba_cache_read, fba_cache4_read: slots first .. first + slots - 1 of every sequence to k, v [batch, kv_heads, slots, 128]: what a prompt's next chunk attends to with
  *   fba_window_fwd, whose queries are the last of the rows, of all sequences alike: of sequences that had one length in front of the chunk, slots being that length and the chunk's
