@@ -9,10 +9,10 @@
 // the scores, its V behind its decoding.
 //
 // 8 streams of 115200 slots, 16 heads on 4: 501 MB in 84 us, 6.0 TB/s.  Its loads alone take 78 (72 without the scales, whose bytes are 6 % of all and come 64 at a time); what is left is
-// that loads, some 240 vector instructions, 24 matrix instructions and 16 KiB through LDS for each tile, each at half of its unit's rate, do not hide behind each other entirely.  Without LDS
-// (wrong results) 78 us.  Measured and not kept: four waves on a SIMD, whose 128 registers spill (94); two, with two to four tiles ahead (88 to 91); each four columns of a matrix
-// instruction with tiles of their own, for groups of four heads, so that softmax is a quarter of the work (155 vector instructions: 91, and 44 instead of 32 us for 64 short sequences);
-// eight waves in step (94); a tile's scales in one load, transposed across the wave (91); LDS rows padded instead of swizzled (86).
+// that loads, some 200 vector instructions (23.1 M counted, 115200 tiles), 24 matrix instructions and 16 KiB through LDS for each tile, the vector unit busy for 56 % of the time and the
+// matrix unit for 26, do not hide behind each other entirely.  Without LDS (wrong results) 78 us.  Measured and not kept: four waves on a SIMD, whose 128 registers spill (94); two, with
+// two to four tiles ahead (88 to 91); each four columns of a matrix instruction with tiles of their own, for groups of four heads, so that softmax is a quarter of the work (91, and 44
+// instead of 32 us for 64 short sequences); eight waves in step (94); a tile's scales in one load, transposed across the wave (91); LDS rows padded instead of swizzled (86).
 // Scores cost 32 ragged sequences, 24 heads on 6, 52 -> 72 us: 27 MB written, read again and added up.  Stored in every lane, a tile's heads one behind the other, 71; the kernel of 16 bits,
 // which shares their layout, was 2 us of 102 slower then, and it was not kept.
 #include "fba_cache_attend.h"
