@@ -267,7 +267,7 @@ def cache_attn_func(q, cache, table, lengths, window=None, sinks=0, accumulate=F
     `window` of them and the first `sinks`.  (Slots are in the order of tokens as long as nothing has been evicted.)
 
     q: (batch, heads, 1, 128) of the cache's type, heads a multiple of kv_heads.  accumulate=True adds to cache.weights what softmax gave every slot, summed over the query
-    heads of a kv head; not with a window, and with a workspace of 4 * batch * heads bytes for every slot that the table has room for, filled or not.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
+    heads of a kv head; not with a window, and with a workspace of 4 * batch * heads bytes for every slot that the table has room for, filled or not.  The cache's positions are not looked at.  Returns o, shaped like q: zeros for a sequence without slots, NaN for one whose length or pages make no sense."""
     given = _given(cache, table, lengths, positions=False)
     out = None if given is None else _lib.host().cache_attention(q, given, window, sinks, bool(accumulate))
     if out is not None:
